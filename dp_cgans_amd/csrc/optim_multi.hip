@@ -1,0 +1,399 @@
+// Many tensors in one launch: the global gradient norm with its clip factor, and a decoupled-weight-decay Adam step
+// with states in 32 or in 8 bits.  A PLAN (device memory of the caller) lists the tensors and cuts them into chunks;
+// block b of a launch works on chunk b, so a launch costs the same for one tensor as for hundreds.
+#include "dpc_common.h"
+#include "../../include/dpcgan_hip.h"
+#include <math.h>
+#include <string.h>
+
+#define MT_BLOCK8 128           // elements that share one scale of an 8-bit state = 16 lanes x 8 elements
+#define MT_SUB 2048             // elements one block handles per pass: 256 threads x 8
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// One tensor of a plan, as the kernels see it.
+struct MtRec {
+  void* p; const void* g; void* m; void* v;
+  float* ms; float* vs;                 // scales of the 8-bit states (null: 32-bit states)
+  void* cp;
+  const uint16_t* dith;
+  int64_t n;
+  int64_t draw8;                        // first Philox block of this tensor (one block per 8 elements)
+  int32_t p_t, g_t, c_t;
+  float wd;
+  int32_t vec;                          // 8-element accesses are aligned in every buffer
+  int32_t pad;
+};
+// Chunk b of a plan: elements [start, start + chunk) of tensor t.
+struct MtChunk { int32_t t; int32_t pad; int64_t start; };
+
+struct MtPlan { const MtRec* rec; const MtChunk* chunk; int blocks; int chunk_len; };
+
+static int64_t mt_align(int64_t x) { return (x + 255) & ~(int64_t)255; }
+
+// 8 consecutive elements as floats; elements past `left` come back 0.
+__device__ __forceinline__ f32x8 mt_load(const void* base, int64_t i, int type, bool whole, int left) {
+  f32x8 o;
+  if (whole) {
+    if (type == DPC_F32) {
+      const f32x4* q = reinterpret_cast<const f32x4*>((const float*)base + i);
+      const f32x4 a = q[0], b = q[1];
+      o = f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    } else if (type == DPC_BF16) {
+      o = __builtin_convertvector(*reinterpret_cast<const bf16x8*>((const uint16_t*)base + i), f32x8);
+    } else {
+      o = __builtin_convertvector(*reinterpret_cast<const f16x8*>((const uint16_t*)base + i), f32x8);
+    }
+    return o;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    o[e] = 0.f;
+    if (e < left) {
+      if (type == DPC_F32) o[e] = ((const float*)base)[i + e];
+      else if (type == DPC_BF16) o[e] = (float)((const __bf16*)base)[i + e];
+      else o[e] = (float)((const _Float16*)base)[i + e];
+    }
+  }
+  return o;
+}
+
+__device__ __forceinline__ void mt_store(void* base, int64_t i, int type, bool whole, int left, f32x8 x) {
+  if (whole) {
+    if (type == DPC_F32) {
+      f32x4* q = reinterpret_cast<f32x4*>((float*)base + i);
+      q[0] = f32x4{x[0], x[1], x[2], x[3]};
+      q[1] = f32x4{x[4], x[5], x[6], x[7]};
+    } else if (type == DPC_BF16) {
+      *reinterpret_cast<bf16x8*>((uint16_t*)base + i) = __builtin_convertvector(x, bf16x8);
+    } else {
+      *reinterpret_cast<f16x8*>((uint16_t*)base + i) = __builtin_convertvector(x, f16x8);
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (e < left) {
+      if (type == DPC_F32) ((float*)base)[i + e] = x[e];
+      else if (type == DPC_BF16) ((__bf16*)base)[i + e] = (__bf16)x[e];
+      else ((_Float16*)base)[i + e] = (_Float16)x[e];
+    }
+  }
+}
+
+// ---- global norm ---------------------------------------------------------------------------------------------------
+// sum of g^2 in fp64 (the square of an fp32 gradient overflows at 2e19 and vanishes below 1e-23): one partial per
+// block, chunks b, b + gridDim, ... in that order, so the sum does not depend on which block ends first.
+__global__ __launch_bounds__(256) void grad_sumsq_kernel(MtPlan pl, double* part) {
+  __shared__ double red[16];
+  double s = 0.0;
+  for (int c = blockIdx.x; c < pl.blocks; c += gridDim.x) {
+    const MtChunk ch = pl.chunk[c];
+    const MtRec r = pl.rec[ch.t];
+    const int64_t end = min(ch.start + (int64_t)pl.chunk_len, r.n);
+    for (int64_t i = ch.start + 8 * threadIdx.x; i < end; i += MT_SUB) {
+      const int left = (int)min((int64_t)8, end - i);
+      const f32x8 g = mt_load(r.g, i, r.g_t, r.vec && left == 8, left);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s = fma((double)g[e], (double)g[e], s);
+    }
+  }
+  s = dpc_block_sum(s, red);
+  if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+
+// out = {norm, coef}; a norm that is not finite gives coef 0 (the step that reads it is not taken) and leaves *t alone.
+__global__ __launch_bounds__(256) void grad_clip_kernel(const double* part, int n, double max_norm, double gscale, float* out, int32_t* t) {
+  __shared__ double red[16];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += 256) s += part[i];
+  s = dpc_block_sum(s, red);
+  if (threadIdx.x == 0) {
+    const double norm = gscale * sqrt(s);
+    const bool ok = norm <= 1.7976931348623157e308;        // false for NaN too
+    out[0] = (float)norm;
+    out[1] = ok ? (float)(norm > max_norm ? gscale * (max_norm / norm) : gscale) : 0.f;
+    if (ok && t) *t += 1;
+  }
+}
+
+// ---- AdamW ---------------------------------------------------------------------------------------------------------
+struct AdamwArgs {
+  MtPlan pl;
+  float lr, b1, b2, c1, c2, eps;        // c = 1 - b, taken in fp64
+  double b1d, b2d;
+  float step_size, inv_bc2s;            // lr / (1 - b1^t), 1 / sqrt(1 - b2^t) where the step count is the host's
+  const float* coef; float gscale;
+  const int32_t* t_dev; int t_host;
+  const uint64_t* rng; uint32_t site;
+};
+
+// One element in full precision: the new moment, root and parameter.  Contraction off: the vector and the element-wise
+// paths give the same bits.
+__device__ __forceinline__ float adamw_one(const AdamwArgs& a, float g, float p, float& m, float& v, float& r, float keep,
+                                           float step_size, float inv_bc2s) {
+#pragma clang fp contract(off)
+  m = a.b1 * m + a.c1 * g;
+  v = a.b2 * v + a.c2 * g * g;
+  r = sqrtf(v);
+  return p * keep - step_size * (m / (r * inv_bc2s + a.eps));
+}
+
+// x in [0, 448] to the e4m3 code below or above it, above where the fraction between them plus d / 65536 reaches 1.
+// Normal values: d is added to the 20 mantissa bits that go; below 2^-6 the grid is 2^-9.
+__device__ __forceinline__ uint32_t mt_code8(float x, uint32_t d) {
+  const uint32_t big = ((__builtin_bit_cast(uint32_t, x) + (d << 4)) >> 20) - (120u << 3);
+  const uint32_t small = (uint32_t)(x * 512.f + (float)d * (1.f / 65536.f));
+  return min(x >= 0.015625f ? big : small, 0x7eu);
+}
+
+// Largest of a value over the 16 lanes that hold a state block (rotations inside a DPP row).
+__device__ __forceinline__ float mt_max16(float v) {
+  v = fmaxf(v, DPC_DPP(v, 0x128, 0xf, 0xf));
+  v = fmaxf(v, DPC_DPP(v, 0x124, 0xf, 0xf));
+  v = fmaxf(v, DPC_DPP(v, 0x122, 0xf, 0xf));
+  return fmaxf(v, DPC_DPP(v, 0x121, 0xf, 0xf));
+}
+
+__device__ __forceinline__ f32x8 mt_load8(const void* base, int64_t i, bool whole, int left, float scale) {
+  u32x2 q = {0u, 0u};
+  if (whole) {
+    q = *reinterpret_cast<const u32x2*>((const uint8_t*)base + i);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < left) q[e >> 2] |= (uint32_t)((const uint8_t*)base)[i + e] << (8 * (e & 3));
+  }
+  const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(q.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(q.x, true);
+  const f32x2 c = __builtin_amdgcn_cvt_pk_f32_fp8(q.y, false), d = __builtin_amdgcn_cvt_pk_f32_fp8(q.y, true);
+  return f32x8{a.x * scale, a.y * scale, b.x * scale, b.y * scale, c.x * scale, c.y * scale, d.x * scale, d.y * scale};
+}
+
+// Hold the 8 values x of this lane, part of a 128-element block, in 8 bits.  The block's largest finite value goes on
+// 448, the largest e4m3 number; what is not finite is held as NaN.  `up`: a value that is not 0 is not held as 0
+// (a root held as 0 would divide its moment by eps alone).
+__device__ __forceinline__ void mt_hold8(void* base, float* scales, int64_t i, bool whole, int left, f32x8 x, const uint32_t d[8], bool up) {
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float ax = fabsf(x[e]);
+    top = fmaxf(top, ax <= 3.402823466e38f ? ax : 0.f);
+  }
+  const float s = fmaxf(mt_max16(top), 7.88860905e-31f) / 448.f;      // at least 2^-100 / 448: 1 / s stays finite
+  const float inv = 1.f / s;
+  uint32_t q[2] = {0u, 0u};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float xe = x[e], ax = fabsf(xe);
+    uint32_t c = mt_code8(fminf(ax * inv, 448.f), d[e]);
+    if (up && ax > 0.f && c == 0u) c = 1u;
+    if (!(ax <= 3.402823466e38f)) c = 0x7fu;
+    c |= (__builtin_bit_cast(uint32_t, xe) >> 24) & 0x80u;
+    q[e >> 2] |= c << (8 * (e & 3));
+  }
+  if (whole) {
+    *reinterpret_cast<u32x2*>((uint8_t*)base + i) = u32x2{q[0], q[1]};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < left) ((uint8_t*)base)[i + e] = (uint8_t)(q[e >> 2] >> (8 * (e & 3)));
+  }
+  if ((threadIdx.x & 15) == 0 && left > 0) scales[i / MT_BLOCK8] = s;
+}
+
+template <bool S8>
+__global__ __launch_bounds__(256) void adamw_kernel(AdamwArgs a) {
+  __shared__ float bc[2];
+  const float coef = a.coef ? a.coef[0] : 1.f;
+  if (a.coef && coef == 0.f) return;            // the clip factor of a gradient that is not finite
+  const MtChunk ch = a.pl.chunk[blockIdx.x];
+  const MtRec r = a.pl.rec[ch.t];
+  float step_size = a.step_size, inv_bc2s = a.inv_bc2s;
+  if (a.t_dev) {                                // beta^t by repeated squaring, as dpc_adam_step's kernel
+    if (threadIdx.x == 0) {
+      double p1 = 1.0, p2 = 1.0, x1 = a.b1d, x2 = a.b2d;
+      for (int e = a.t_dev[0] + a.t_host; e > 0; e >>= 1) {
+        if (e & 1) { p1 *= x1; p2 *= x2; }
+        x1 *= x1; x2 *= x2;
+      }
+      bc[0] = (float)((double)a.lr / (1.0 - p1));
+      bc[1] = (float)(1.0 / sqrt(1.0 - p2));
+    }
+    __syncthreads();
+    step_size = bc[0];
+    inv_bc2s = bc[1];
+  }
+  const float gs = a.gscale * coef, keep = 1.f - a.lr * r.wd;
+  const int64_t end = min(ch.start + (int64_t)a.pl.chunk_len, r.n);
+  // (whole passes of the block, also where the tensor ends inside: the 16 lanes of a state block stay together)
+  for (int64_t i = ch.start + 8 * threadIdx.x; i - 8 * (int64_t)threadIdx.x < end; i += MT_SUB) {
+    const int left = (int)max((int64_t)0, min((int64_t)8, end - i));
+    const bool whole = r.vec && left == 8;
+    f32x8 g = mt_load(r.g, i, r.g_t, whole, left), p = mt_load(r.p, i, r.p_t, whole, left);
+    f32x8 m, v, rt;
+    if (S8) {
+      const float ms = left > 0 ? r.ms[i / MT_BLOCK8] : 0.f, vs = left > 0 ? r.vs[i / MT_BLOCK8] : 0.f;
+      m = mt_load8(r.m, i, whole, left, ms);
+      v = mt_load8(r.v, i, whole, left, vs);
+      v *= v;
+    } else {
+      m = mt_load(r.m, i, DPC_F32, whole, left);
+      v = mt_load(r.v, i, DPC_F32, whole, left);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float me = m[e], ve = v[e], re;
+      p[e] = adamw_one(a, g[e] * gs, p[e], me, ve, re, keep, step_size, inv_bc2s);
+      m[e] = me; v[e] = ve; rt[e] = re;
+    }
+    if (S8) {
+      uint32_t d[8];
+      if (r.dith) {
+        if (whole) {
+          const u32x4 q = *reinterpret_cast<const u32x4*>(r.dith + i);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[e] = (q[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[e] = e < left ? r.dith[i + e] : 0u;
+        }
+      } else {
+        const DpcPhilox4 ph = dpc_philox(a.rng[0], a.rng[1], a.site, (uint64_t)(r.draw8 + (i >> 3)));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] = (ph.v[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+      }
+      mt_hold8(r.m, r.ms, i, whole, left, m, d, false);
+      mt_hold8(r.v, r.vs, i, whole, left, rt, d, true);
+    } else {
+      mt_store(r.m, i, DPC_F32, whole, left, m);
+      mt_store(r.v, i, DPC_F32, whole, left, v);
+    }
+    mt_store(r.p, i, r.p_t, whole, left, p);
+    if (r.cp) mt_store(r.cp, i, r.c_t, whole, left, p);
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------
+static int mt_size(int type) { return type == DPC_F32 ? 4 : 2; }
+static bool mt_type_ok(int type) { return type == DPC_F32 || type == DPC_BF16 || type == DPC_F16; }
+static bool mt_al(const void* p, int bytes) { return ((uintptr_t)p % (uintptr_t)bytes) == 0; }
+#define MT_PARTS 2048            // partial sums of the global norm (blocks of its first launch)
+
+static int mt_check(const dpc_multi_tensor* t, int count, dpc_multi_info* info) {
+  DPC_CHECK_ARG(count >= 0 && (t || count == 0) && info, "multi_plan: null pointer or negative count");
+  int64_t total = 0;
+  int kinds = 0;
+  for (int k = 0; k < count; ++k) {
+    const dpc_multi_tensor& x = t[k];
+    DPC_CHECK_ARG(x.n >= 0 && x.n < (1ll << 46), "multi_plan: bad tensor size");
+    DPC_CHECK_ARG(mt_type_ok(x.g_type) && mt_type_ok(x.p_type) && mt_type_ok(x.copy_type), "multi_plan: unknown element type");
+    if (x.n == 0) continue;
+    DPC_CHECK_ARG(x.g && mt_al(x.g, mt_size(x.g_type)), "multi_plan: null or misaligned gradient");
+    if (x.p) {
+      DPC_CHECK_ARG(x.m && x.v, "multi_plan: a parameter needs both moments");
+      DPC_CHECK_ARG(mt_al(x.p, mt_size(x.p_type)) && (!x.copy || mt_al(x.copy, mt_size(x.copy_type))), "multi_plan: misaligned tensor");
+      DPC_CHECK_ARG(!x.m_scale == !x.v_scale, "multi_plan: both 8-bit states need their scales");
+      DPC_CHECK_ARG(x.m_scale ? (mt_al(x.m_scale, 4) && mt_al(x.v_scale, 4)) : (mt_al(x.m, 4) && mt_al(x.v, 4)), "multi_plan: misaligned state");
+      DPC_CHECK_ARG(!x.dither || (x.m_scale && mt_al(x.dither, 2)), "multi_plan: random bits go with 8-bit states");
+      DPC_CHECK_ARG(x.wd >= 0.f && x.wd <= 3.402823466e38f, "multi_plan: weight decay must be finite and not negative");
+      kinds |= x.m_scale ? (x.dither ? 4 : 2) : 1;
+    } else {
+      DPC_CHECK_ARG(!x.m && !x.v && !x.copy && !x.m_scale && !x.v_scale, "multi_plan: states without a parameter");
+      kinds |= 8;
+    }
+    total += x.n;
+  }
+  DPC_CHECK_ARG(kinds == 0 || kinds == 1 || kinds == 2 || kinds == 4 || kinds == 8,
+                "multi_plan: the tensors of a plan are of one kind (gradients only, 32-bit states, or 8-bit states with or without given random bits)");
+  // A chunk is one pass of a block while that gives a round of blocks or two (256 CUs x 8 blocks); beyond, four passes
+  // halve the blocks' own cost (record, step size) against the bytes they move.
+  info->chunk_len = total <= (int64_t)MT_SUB * 8192 ? MT_SUB : 4 * MT_SUB;
+  int64_t blocks = 0;
+  for (int k = 0; k < count; ++k) blocks += dpc_cdiv(t[k].n, info->chunk_len);
+  DPC_CHECK_ARG(blocks < (1ll << 31), "multi_plan: too many elements");
+  info->kind = kinds;
+  info->count = count;
+  info->blocks = (int)blocks;
+  info->rec_off = 0;
+  info->chunk_off = mt_align((int64_t)count * sizeof(MtRec));
+  info->part_off = info->chunk_off + mt_align(blocks * (int64_t)sizeof(MtChunk));
+  info->bytes = info->part_off + MT_PARTS * sizeof(double);
+  return DPC_OK;
+}
+
+extern "C" int dpc_multi_plan_size(const dpc_multi_tensor* t, int count, dpc_multi_info* info) { return mt_check(t, count, info); }
+
+extern "C" int dpc_multi_plan(const dpc_multi_tensor* t, int count, const dpc_multi_info* info, void* plan, int64_t bytes) {
+  DPC_CHECK_ARG(info && plan, "multi_plan: null pointer");
+  dpc_multi_info in;
+  const int rc = mt_check(t, count, &in);
+  if (rc != DPC_OK) return rc;
+  DPC_CHECK_ARG(in.bytes == info->bytes && in.blocks == info->blocks && in.kind == info->kind && bytes >= in.bytes,
+                "multi_plan: the buffer or the sizes are not those of dpc_multi_plan_size");
+  memset(plan, 0, (size_t)in.bytes);
+  MtRec* rec = (MtRec*)((char*)plan + in.rec_off);
+  MtChunk* chunk = (MtChunk*)((char*)plan + in.chunk_off);
+  int64_t draw = 0, b = 0;
+  for (int k = 0; k < count; ++k) {
+    const dpc_multi_tensor& x = t[k];
+    MtRec& r = rec[k];
+    r.p = x.p; r.g = x.g; r.m = x.m; r.v = x.v; r.ms = x.m_scale; r.vs = x.v_scale; r.cp = x.copy; r.dith = x.dither;
+    r.n = x.n; r.draw8 = draw; r.p_t = x.p_type; r.g_t = x.g_type; r.c_t = x.copy_type; r.wd = x.wd;
+    r.vec = mt_al(x.g, 16) && (!x.p || (mt_al(x.p, 16) && mt_al(x.m, x.m_scale ? 8 : 16) && mt_al(x.v, x.m_scale ? 8 : 16) &&
+                                        mt_al(x.copy, 16) && mt_al(x.dither, 16)));
+    draw += dpc_cdiv(x.n, 8);
+    for (int64_t s = 0; s < x.n; s += in.chunk_len) { chunk[b].t = k; chunk[b].start = s; ++b; }
+  }
+  return DPC_OK;
+}
+
+static MtPlan mt_view(const dpc_multi_info* info, const void* plan) {
+  MtPlan pl;
+  pl.rec = (const MtRec*)((const char*)plan + info->rec_off);
+  pl.chunk = (const MtChunk*)((const char*)plan + info->chunk_off);
+  pl.blocks = info->blocks;
+  pl.chunk_len = info->chunk_len;
+  return pl;
+}
+
+extern "C" int dpc_grad_clip(const dpc_multi_info* info, void* plan, double max_norm, double gscale, float* out, int32_t* t_dev, void* stream) {
+  DPC_CHECK_ARG(info && plan && out, "grad_clip: null pointer");
+  DPC_CHECK_ARG(max_norm > 0.0 && gscale > 0.0 && gscale <= 3.402823466e38, "grad_clip: max_norm and gscale must be positive");
+  double* part = (double*)((char*)plan + info->part_off);
+  const int nb = info->blocks < MT_PARTS ? info->blocks : MT_PARTS;
+  if (nb > 0) hipLaunchKernelGGL(grad_sumsq_kernel, dim3(nb), dim3(256), 0, (hipStream_t)stream, mt_view(info, plan), part);
+  hipLaunchKernelGGL(grad_clip_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, part, nb, max_norm, gscale, out, t_dev);
+  DPC_LAUNCH_CHECK();
+  return DPC_OK;
+}
+
+extern "C" int dpc_adamw_step(const dpc_multi_info* info, const void* plan, double lr, double b1, double b2, double eps,
+                              const float* coef, float gscale, const int32_t* t_dev, int t_host, const uint64_t* rng,
+                              uint32_t site, void* stream) {
+  DPC_CHECK_ARG(info && plan, "adamw: null pointer");
+  DPC_CHECK_ARG(info->kind != 8, "adamw: the plan lists gradients only");
+  DPC_CHECK_ARG(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0 && eps >= 0.0 && lr >= 0.0 && lr <= 3.402823466e38, "adamw: betas must lie in [0, 1), lr and eps must not be negative");
+  DPC_CHECK_ARG(t_host >= 1 || (t_host == 0 && t_dev), "adamw: the step count starts at 1 (t_host 0 goes with a device counter)");
+  DPC_CHECK_ARG(info->kind != 2 || rng, "adamw: 8-bit states need random bits (rng, or dither in the plan)");
+  if (info->blocks == 0) return DPC_OK;
+  AdamwArgs a;
+  a.pl = mt_view(info, plan);
+  a.lr = (float)lr; a.b1 = (float)b1; a.b2 = (float)b2; a.c1 = (float)(1.0 - b1); a.c2 = (float)(1.0 - b2); a.eps = (float)eps;
+  a.b1d = b1; a.b2d = b2;
+  a.step_size = a.inv_bc2s = 0.f;
+  if (!t_dev) {
+    a.step_size = (float)(lr / (1.0 - pow(b1, t_host)));
+    a.inv_bc2s = (float)(1.0 / sqrt(1.0 - pow(b2, t_host)));
+  }
+  a.coef = coef; a.gscale = gscale; a.t_dev = t_dev; a.t_host = t_host; a.rng = rng; a.site = site;
+  if (info->kind == 1) hipLaunchKernelGGL(adamw_kernel<false>, dim3(info->blocks), dim3(256), 0, (hipStream_t)stream, a);
+  else hipLaunchKernelGGL(adamw_kernel<true>, dim3(info->blocks), dim3(256), 0, (hipStream_t)stream, a);
+  DPC_LAUNCH_CHECK();
+  return DPC_OK;
+}

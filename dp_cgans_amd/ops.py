@@ -14,7 +14,7 @@ FILL_U32, FILL_NORMAL, FILL_EXP, FILL_UNIFORM, FILL_UNIFORM64, FILL_KEEP = 0, 1,
 
 # call-site ids of the Philox streams (one independent stream per site and step)
 SITE_Z, SITE_GUMBEL, SITE_DROP0, SITE_ALPHA, SITE_CONDVEC, SITE_ROWPICK, SITE_PERM = 1, 2, 16, 3, 4, 5, 6
-SITE_NOISE_D, SITE_HOOK, SITE_ENCODE = 7, 8, 9
+SITE_NOISE_D, SITE_HOOK, SITE_ENCODE, SITE_DITHER = 7, 8, 9, 10
 
 
 _dev_index = None        # GPU of the tensors of the call being assembled (see _stream)
@@ -662,6 +662,155 @@ def adam_step_slices(p, g, m, v, lr, wd, mats, slices, b1=0.5, b2=0.9, eps=1e-8,
                I64s(*[(_ld(gT) if gT is not None else 0) for _, _, _, gT, _ in slices]),
                Ps(*[(pT.data_ptr() if pT is not None else None) for _, _, _, _, pT in slices]),
                I64s(*[(_ld(pT) if pT is not None else 0) for _, _, _, _, pT in slices]), _stream())
+
+
+# ---- optimiser over many tensors ---------------------------------------------------------------------------------
+_MULTI_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class MultiTensor(ctypes.Structure):
+    """dpc_multi_tensor of include/dpcgan_hip.h."""
+    _fields_ = [('p', ctypes.c_void_p), ('g', ctypes.c_void_p), ('m', ctypes.c_void_p), ('v', ctypes.c_void_p),
+                ('m_scale', ctypes.c_void_p), ('v_scale', ctypes.c_void_p), ('copy', ctypes.c_void_p),
+                ('dither', ctypes.c_void_p), ('n', ctypes.c_int64), ('p_type', ctypes.c_int32),
+                ('g_type', ctypes.c_int32), ('copy_type', ctypes.c_int32), ('wd', ctypes.c_float)]
+
+
+class MultiInfo(ctypes.Structure):
+    """dpc_multi_info of include/dpcgan_hip.h."""
+    _fields_ = [('bytes', ctypes.c_int64), ('rec_off', ctypes.c_int64), ('chunk_off', ctypes.c_int64),
+                ('part_off', ctypes.c_int64), ('count', ctypes.c_int32), ('blocks', ctypes.c_int32),
+                ('chunk_len', ctypes.c_int32), ('kind', ctypes.c_int32)]
+
+
+class MultiPlan(object):
+    """The tensors of grad_clip / adamw_step, laid out once (grad_plan, adamw_plan).  It keeps the tensors alive and
+    serves every step while they stay where they are; calls on one plan must follow one another (they share the
+    partial sums of the norm, and the parameters)."""
+
+    def __init__(self, info, table, keep):
+        self.info, self.table, self._keep = info, table, keep
+        self._info = ctypes.byref(info)
+
+
+def _multi_list(ts, n, types, what):
+    if ts is None:
+        return [None] * n
+    ts = list(ts)
+    if len(ts) != n:
+        raise ValueError('%s: %d tensors for %d gradients' % (what, len(ts), n))
+    for t in ts:
+        if not t.is_cuda:
+            raise ValueError('%s must live on the GPU' % what)
+        if t.dtype not in types:
+            raise TypeError('%s must be %s, got %s' % (what, ' or '.join(str(x) for x in types), t.dtype))
+        if not t.is_contiguous():
+            raise ValueError('%s must be contiguous' % what)
+    return ts
+
+
+def _multi_plan(lists, wd):
+    n = len(lists['g'])
+    rec = (MultiTensor * max(n, 1))()
+    spans, devs = [], set()
+    for k in range(n):
+        r, size = rec[k], lists['g'][k].numel()
+        for name in ('p', 'g', 'm', 'v', 'm_scale', 'v_scale', 'copy', 'dither'):
+            t = lists[name][k]
+            if t is None:
+                continue
+            if t.numel() != (-(-size // 128) if name.endswith('_scale') else size):
+                raise ValueError('multi-tensor plan: %s %d has %d elements, its gradient %d' % (name, k, t.numel(), size))
+            setattr(r, name, t.data_ptr())
+            devs.add(t.device)
+            if size:
+                spans.append((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), name in ('g', 'dither')))
+        r.n, r.wd = size, wd[k]
+        r.g_type = _MULTI_TYPES[lists['g'][k].dtype]
+        r.p_type = _MULTI_TYPES[lists['p'][k].dtype] if lists['p'][k] is not None else 0
+        r.copy_type = _MULTI_TYPES[lists['copy'][k].dtype] if lists['copy'][k] is not None else 0
+    if len(devs) > 1:
+        raise ValueError('multi-tensor plan: tensors on %s; a plan serves one GPU' % ', '.join(sorted(str(d) for d in devs)))
+    spans.sort()
+    end_read = end_written = 0              # furthest ends of the buffers so far, by whether a step writes them
+    for a, b, read in spans:
+        if a < end_written or (not read and a < end_read):
+            raise ValueError('multi-tensor plan: tensors that a step writes overlap another one')
+        if read:
+            end_read = max(end_read, b)
+        else:
+            end_written = max(end_written, b)
+    info = MultiInfo()
+    L = lib()
+    L.call('dpc_multi_plan_size', rec, n, ctypes.byref(info))
+    host = (ctypes.c_uint8 * info.bytes)()
+    L.call('dpc_multi_plan', rec, n, ctypes.byref(info), host, info.bytes)
+    dev = devs.pop() if devs else torch.device('cuda', torch.cuda.current_device())
+    table = torch.frombuffer(bytearray(host), dtype=torch.uint8).to(dev)
+    return MultiPlan(info, table, lists)
+
+
+def grad_plan(grads):
+    """Plan over gradients alone, for grad_clip: a list of contiguous fp32 / bf16 / fp16 tensors of one GPU."""
+    grads = list(grads)
+    lists = {k: [None] * len(grads) for k in ('p', 'm', 'v', 'm_scale', 'v_scale', 'copy', 'dither')}
+    lists['g'] = _multi_list(grads, len(grads), list(_MULTI_TYPES), 'grads')
+    return _multi_plan(lists, [0.0] * len(grads))
+
+
+def adamw_plan(params, grads, exp_avg, exp_avg_sq, wd=0.0, copies=None, m_scale=None, v_scale=None, dither=None):
+    """Plan of an adamw_step (and of the grad_clip before it) over lists of contiguous tensors: params and grads fp32 /
+    bf16 / fp16, states fp32 - or float8_e4m3fn with fp32 scales, one per 128 elements (adamw_state8 makes them;
+    v then holds square roots).  wd: one weight decay or one per tensor; copies: bf16 / fp16 tensors that take the updated
+    parameters as well; dither: int16 tensors of random bits for the 8-bit states instead of Philox draws."""
+    grads = list(grads)
+    n = len(grads)
+    any16 = list(_MULTI_TYPES)
+    eight = m_scale is not None or v_scale is not None
+    st = [torch.float8_e4m3fn] if eight else [torch.float32]
+    if eight and (m_scale is None or v_scale is None):
+        raise ValueError('adamw_plan: 8-bit states need m_scale and v_scale')
+    if dither is not None and not eight:
+        raise ValueError('adamw_plan: dither goes with 8-bit states')
+    lists = dict(g=_multi_list(grads, n, any16, 'grads'), p=_multi_list(list(params), n, any16, 'params'),
+                 m=_multi_list(list(exp_avg), n, st, 'exp_avg'), v=_multi_list(list(exp_avg_sq), n, st, 'exp_avg_sq'),
+                 m_scale=_multi_list(m_scale, n, [torch.float32], 'm_scale'),
+                 v_scale=_multi_list(v_scale, n, [torch.float32], 'v_scale'),
+                 copy=_multi_list(copies, n, [torch.bfloat16, torch.float16], 'copies'),
+                 dither=_multi_list(dither, n, [torch.int16], 'dither'))
+    wd = [float(wd)] * n if isinstance(wd, (int, float)) else [float(x) for x in wd]
+    if len(wd) != n:
+        raise ValueError('adamw_plan: %d weight decays for %d tensors' % (len(wd), n))
+    return _multi_plan(lists, wd)
+
+
+def adamw_state8(like):
+    """A fresh 8-bit state for adamw_plan: (codes float8_e4m3fn shaped as ``like``, scales fp32), all zero."""
+    return (torch.zeros_like(like, dtype=torch.uint8, memory_format=torch.contiguous_format).view(torch.float8_e4m3fn),
+            torch.zeros(-(-like.numel() // 128), device=like.device))
+
+
+def grad_clip(plan, max_norm, out, gscale=1.0, t_dev=None):
+    """out [2] <- (norm, coef): the norm of gscale times all gradients of ``plan`` and the factor that brings them to at
+    most ``max_norm``, for adamw_step's ``coef``; nothing is read back.  A norm that is not finite gives coef 0 (the
+    step is skipped); otherwise the device step count ``t_dev`` (int32 [1], optional) goes up by one."""
+    _chk(out, torch.float32, 'out')
+    _chk(t_dev, torch.int32, 't_dev')
+    if out.numel() < 2 or not out.is_contiguous():
+        raise ValueError('grad_clip: out must be a contiguous fp32 [2]')
+    lib().call('dpc_grad_clip', plan._info, _p(plan.table), float(max_norm), float(gscale), _p(out), _p(t_dev), _stream())
+    return out
+
+
+def adamw_step(plan, lr, b1=0.9, b2=0.999, eps=1e-8, coef=None, gscale=1.0, t_dev=None, t_host=1, rng=None,
+               site=SITE_DITHER):
+    """One AdamW step over the tensors of ``plan`` in one launch.  coef: fp32 device factor of the gradients (grad_clip's
+    out[1:]; 0 skips the step).  Step count (t_dev's value + t_host) >= 1; rng: required by 8-bit states without dither."""
+    _chk(coef, torch.float32, 'coef')
+    _chk(t_dev, torch.int32, 't_dev')
+    _chk(rng, torch.int64, 'rng')
+    lib().call('dpc_adamw_step', plan._info, _p(plan.table), float(lr), float(b1), float(b2), float(eps), _p(coef),
+               float(gscale), _p(t_dev), int(t_host), _p(rng), site, _stream())
 
 
 def noise_add_clamp(x, scale, noise_inj=None, rng=None, site=SITE_NOISE_D, clamp=0.0):

@@ -446,6 +446,53 @@ int dpc_adam_step_slices(float* p, float* g, float* m, float* v, int64_t n, floa
 int dpc_noise_add_clamp(float* x, int64_t n, float scale, const float* noise_inj, const uint64_t* rng,
                         uint32_t site, float clamp, void* stream);
 
+/* ---- optimiser over many tensors (no counterpart in the reference, whose torch.optim.Adam, dp_cgan.py:510-518, walks
+ * its fp32 tensors one by one; dpc_adam_step covers that over one flat buffer) ------------------------------------ */
+#define DPC_F32 0
+#define DPC_BF16 1
+#define DPC_F16 2
+/* One tensor of n contiguous elements.  p (nullable: the gradients of grad_clip alone), g, and the two moments:
+ *   32-bit states   m, v fp32 [n]: first and second moment;
+ *   8-bit states    m, v e4m3 (OCP, no infinities) codes [n], m_scale, v_scale fp32 [ceil(n/128)]: code * scale of its
+ *                   128-element block is the first moment / the square ROOT of the second (all zero = a fresh state).
+ * copy (nullable): the updated parameters once more, in copy_type (the half-precision copy a product reads).
+ * dither (nullable, 8-bit states): uint16 [n] random bits instead of Philox draws.  wd: this tensor's weight decay.
+ * Any element alignment; 16 bytes in all buffers (8 for e4m3 codes) take the wide accesses. */
+typedef struct dpc_multi_tensor {
+  void* p; const void* g; void* m; void* v;
+  float* m_scale; float* v_scale;
+  void* copy; const uint16_t* dither;
+  int64_t n;
+  int32_t p_type, g_type, copy_type;
+  float wd;
+} dpc_multi_tensor;
+/* Sizes of a plan (host struct, filled by dpc_multi_plan_size; the caller only reads `bytes`). */
+typedef struct dpc_multi_info {
+  int64_t bytes, rec_off, chunk_off, part_off;
+  int32_t count, blocks, chunk_len, kind;
+} dpc_multi_info;
+/* A plan is built in host memory (t, info, plan: HOST pointers; nothing is launched) and copied by the caller into
+ * `bytes` of 256-byte aligned device memory; it holds addresses, so it serves every step while the tensors stay where
+ * they are.  The tensors of a plan are all of one kind (gradients only; 32-bit; 8-bit; 8-bit with dither) and none
+ * may overlap.  A plan holds grad_clip's partial sums: calls on one plan follow one another. */
+int dpc_multi_plan_size(const dpc_multi_tensor* t, int count, dpc_multi_info* info);
+int dpc_multi_plan(const dpc_multi_tensor* t, int count, const dpc_multi_info* info, void* plan, int64_t bytes);
+/* out fp32 [2] = {norm, coef}: norm = gscale * sqrt(sum of g^2 over all tensors) (fp64 sums, fixed order), coef =
+ * gscale * min(1, max_norm / norm).  A norm that is not finite gives coef 0 - dpc_adamw_step then writes nothing - and
+ * is the only case in which *t_dev (nullable, device step count) does not go up by 1. */
+int dpc_grad_clip(const dpc_multi_info* info, void* plan, double max_norm, double gscale, float* out, int32_t* t_dev,
+                  void* stream);
+/* One launch: g' = gscale * coef * g (coef: device fp32, nullable = 1; exactly 0 skips the whole step);
+ * m = b1 m + (1 - b1) g', v = b2 v + (1 - b2) g'^2, p = p (1 - lr wd) - lr/(1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps),
+ * t = (t_dev ? *t_dev : 0) + t_host >= 1.  The step uses the new moments before they are held in 8 bits; those are
+ * rounded up or down at random in proportion (16 random bits, shared by the two moments of an element): rounding to
+ * the nearest would freeze v, which moves by less than half a step of the code at b2 = 0.999.  Element i of tensor k
+ * takes half i % 2 of word (i % 8) / 2 of Philox block D + i/8 of (rng, site), D = sum of ceil(n/8) over the
+ * tensors before k.  The largest finite value of a block is held on 448; what is not finite, as NaN. */
+int dpc_adamw_step(const dpc_multi_info* info, const void* plan, double lr, double b1, double b2, double eps,
+                   const float* coef, float gscale, const int32_t* t_dev, int t_host, const uint64_t* rng, uint32_t site,
+                   void* stream);
+
 /* ---- DP-SGD mode (north_star; the reference has no per-example clipping: SURVEY F2) ------------- */
 /* An example is one pac group i = rows i, n+i, 2n+i (fake, real, penalty) of the stacked
  * discriminator batch.  norm2[i] (+)= ||gradient of example i w.r.t. one Linear layer||_F^2 computed
