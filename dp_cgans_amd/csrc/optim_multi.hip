@@ -37,35 +37,46 @@ struct MtPlan { const MtRec* rec; const MtChunk* chunk; int blocks; int chunk_le
 
 static int64_t mt_align(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
-// 8 consecutive elements as floats; elements past `left` come back 0.
-__device__ __forceinline__ f32x8 mt_load(const void* base, int64_t i, int type, bool whole, int left) {
-  f32x8 o;
-  if (whole) {
-    if (type == DPC_F32) {
-      const f32x4* q = reinterpret_cast<const f32x4*>((const float*)base + i);
-      const f32x4 a = q[0], b = q[1];
-      o = f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    } else if (type == DPC_BF16) {
-      o = __builtin_convertvector(*reinterpret_cast<const bf16x8*>((const uint16_t*)base + i), f32x8);
+// 8 consecutive elements, as loaded: two halves of fp32, one of 16 bits.  Loading and converting are apart so that a
+// block has all its loads in flight before the first wait (the element types are branches the whole block takes).
+struct Raw8 { u32x4 a, b; };
+template <bool FULL>
+__device__ __forceinline__ Raw8 mt_load(const void* base, int64_t i, int type, int left) {
+  Raw8 o = {u32x4{0u, 0u, 0u, 0u}, u32x4{0u, 0u, 0u, 0u}};
+  if (type == DPC_F32) {
+    const uint32_t* q = (const uint32_t*)base + i;
+    if (FULL) {
+      o.a = reinterpret_cast<const u32x4*>(q)[0];
+      o.b = reinterpret_cast<const u32x4*>(q)[1];
     } else {
-      o = __builtin_convertvector(*reinterpret_cast<const f16x8*>((const uint16_t*)base + i), f32x8);
-    }
-    return o;
-  }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    o[e] = 0.f;
-    if (e < left) {
-      if (type == DPC_F32) o[e] = ((const float*)base)[i + e];
-      else if (type == DPC_BF16) o[e] = (float)((const __bf16*)base)[i + e];
-      else o[e] = (float)((const _Float16*)base)[i + e];
+      for (int e = 0; e < 8; ++e)
+        if (e < left) { if (e < 4) o.a[e] = q[e]; else o.b[e - 4] = q[e]; }
+    }
+  } else {
+    const uint16_t* q = (const uint16_t*)base + i;
+    if (FULL) {
+      o.a = *reinterpret_cast<const u32x4*>(q);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < left) o.a[e >> 1] |= (uint32_t)q[e] << (16 * (e & 1));
     }
   }
   return o;
 }
+__device__ __forceinline__ f32x8 mt_float(const Raw8& r, int type) {
+  if (type == DPC_F32) {
+    const f32x4 a = __builtin_bit_cast(f32x4, r.a), b = __builtin_bit_cast(f32x4, r.b);
+    return f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  }
+  if (type == DPC_BF16) return __builtin_convertvector(__builtin_bit_cast(bf16x8, r.a), f32x8);
+  return __builtin_convertvector(__builtin_bit_cast(f16x8, r.a), f32x8);
+}
 
-__device__ __forceinline__ void mt_store(void* base, int64_t i, int type, bool whole, int left, f32x8 x) {
-  if (whole) {
+template <bool FULL>
+__device__ __forceinline__ void mt_store(void* base, int64_t i, int type, int left, f32x8 x) {
+  if (FULL) {
     if (type == DPC_F32) {
       f32x4* q = reinterpret_cast<f32x4*>((float*)base + i);
       q[0] = f32x4{x[0], x[1], x[2], x[3]};
@@ -97,9 +108,11 @@ __global__ __launch_bounds__(256) void grad_sumsq_kernel(MtPlan pl, double* part
     const MtChunk ch = pl.chunk[c];
     const MtRec r = pl.rec[ch.t];
     const int64_t end = min(ch.start + (int64_t)pl.chunk_len, r.n);
-    for (int64_t i = ch.start + 8 * threadIdx.x; i < end; i += MT_SUB) {
-      const int left = (int)min((int64_t)8, end - i);
-      const f32x8 g = mt_load(r.g, i, r.g_t, r.vec && left == 8, left);
+    for (int64_t at = ch.start; at < end; at += MT_SUB) {
+      const int64_t i = at + 8 * threadIdx.x;
+      const int left = (int)max((int64_t)0, min((int64_t)8, end - i));
+      const bool full = r.vec && end - at >= MT_SUB;
+      const f32x8 g = mt_float(full ? mt_load<true>(r.g, i, r.g_t, 8) : mt_load<false>(r.g, i, r.g_t, left), r.g_t);
 #pragma unroll
       for (int e = 0; e < 8; ++e) s = fma((double)g[e], (double)g[e], s);
     }
@@ -127,84 +140,165 @@ __global__ __launch_bounds__(256) void grad_clip_kernel(const double* part, int 
 struct AdamwArgs {
   MtPlan pl;
   float lr, b1, b2, c1, c2, eps;        // c = 1 - b, taken in fp64
-  double b1d, b2d;
+  double b1d, b2d, c1d, c2d;
   float step_size, inv_bc2s;            // lr / (1 - b1^t), 1 / sqrt(1 - b2^t) where the step count is the host's
   const float* coef; float gscale;
   const int32_t* t_dev; int t_host;
   const uint64_t* rng; uint32_t site;
 };
 
-// One element in full precision: the new moment, root and parameter.  Contraction off: the vector and the element-wise
+// The parameter's step from the new moment and root.  Contraction off here and below: the vector and the element-wise
 // paths give the same bits.
-__device__ __forceinline__ float adamw_one(const AdamwArgs& a, float g, float p, float& m, float& v, float& r, float keep,
-                                           float step_size, float inv_bc2s) {
+__device__ __forceinline__ float adamw_param(const AdamwArgs& a, float p, float m, float r, float keep, float step_size, float inv_bc2s) {
 #pragma clang fp contract(off)
-  m = a.b1 * m + a.c1 * g;
-  v = a.b2 * v + a.c2 * g * g;
-  r = sqrtf(v);
   return p * keep - step_size * (m / (r * inv_bc2s + a.eps));
 }
 
-// x in [0, 448] to the e4m3 code below or above it, above where the fraction between them plus d / 65536 reaches 1.
-// Normal values: d is added to the 20 mantissa bits that go; below 2^-6 the grid is 2^-9.
-__device__ __forceinline__ uint32_t mt_code8(float x, uint32_t d) {
-  const uint32_t big = ((__builtin_bit_cast(uint32_t, x) + (d << 4)) >> 20) - (120u << 3);
-  const uint32_t small = (uint32_t)(x * 512.f + (float)d * (1.f / 65536.f));
-  return min(x >= 0.015625f ? big : small, 0x7eu);
+// ---- 8-bit states.  The moments are updated in fp64 from what is held and rounded ONCE, to 4 significant bits, so what
+// is held is the exact rounding for the given random bits (an update in fp32 lands on the other side of a border for one
+// element in 10^6).
+struct Hold8 { double x[8]; };
+
+// y in [0, 448] to the e4m3 code below or above it, above where the fraction between them plus d / 65536 reaches 1: d is
+// added to the bits of the mantissa that go, its top bit on the highest of them.  Below 2^-6 the grid keeps its step of
+// 2^-9, as a mantissa does when 2^-6 (code 8) is added.
+__device__ __forceinline__ uint32_t mt_code8(double y, uint32_t d) {
+  const bool small = y < 0.015625;
+  const double z = small ? y + 0.015625 : y;
+  const uint32_t hi = (uint32_t)(__builtin_bit_cast(uint64_t, z) >> 32);
+  return ((hi + (d << 1)) >> 17) - (small ? ((1023u - 7u) << 3) + 8u : (1023u - 7u) << 3);
+}
+
+// sqrt(v) to 2^-45: the 1-ulp fp32 root and one Newton step in fp64.  v == 0 and the ends of the fp32 range (also
+// infinities and NaN) take the full routine.
+__device__ __forceinline__ double mt_root(double v) {
+  if (!(v > 1e-30 && v < 1e30)) return sqrt(v);
+  const float r = __builtin_amdgcn_sqrtf((float)v);
+  const double rd = (double)r;
+  return fma(fma(-rd, rd, v), (double)(0.5f * __builtin_amdgcn_rcpf(r)), rd);
 }
 
 // Largest of a value over the 16 lanes that hold a state block (rotations inside a DPP row).
-__device__ __forceinline__ float mt_max16(float v) {
-  v = fmaxf(v, DPC_DPP(v, 0x128, 0xf, 0xf));
-  v = fmaxf(v, DPC_DPP(v, 0x124, 0xf, 0xf));
-  v = fmaxf(v, DPC_DPP(v, 0x122, 0xf, 0xf));
-  return fmaxf(v, DPC_DPP(v, 0x121, 0xf, 0xf));
+template <int CTRL>
+__device__ __forceinline__ double mt_ror(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double mt_max16(double v) {
+  v = fmax(v, mt_ror<0x128>(v));
+  v = fmax(v, mt_ror<0x124>(v));
+  v = fmax(v, mt_ror<0x122>(v));
+  return fmax(v, mt_ror<0x121>(v));
 }
 
-__device__ __forceinline__ f32x8 mt_load8(const void* base, int64_t i, bool whole, int left, float scale) {
+template <bool FULL>
+__device__ __forceinline__ u32x2 mt_load8(const void* base, int64_t i, int left) {
+  if (FULL) return *reinterpret_cast<const u32x2*>((const uint8_t*)base + i);
   u32x2 q = {0u, 0u};
-  if (whole) {
-    q = *reinterpret_cast<const u32x2*>((const uint8_t*)base + i);
-  } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < left) q[e >> 2] |= (uint32_t)((const uint8_t*)base)[i + e] << (8 * (e & 3));
-  }
+  for (int e = 0; e < 8; ++e)
+    if (e < left) q[e >> 2] |= (uint32_t)((const uint8_t*)base)[i + e] << (8 * (e & 3));
+  return q;
+}
+__device__ __forceinline__ f32x8 mt_float8(u32x2 q) {
   const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(q.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(q.x, true);
   const f32x2 c = __builtin_amdgcn_cvt_pk_f32_fp8(q.y, false), d = __builtin_amdgcn_cvt_pk_f32_fp8(q.y, true);
-  return f32x8{a.x * scale, a.y * scale, b.x * scale, b.y * scale, c.x * scale, c.y * scale, d.x * scale, d.y * scale};
+  return f32x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
-// Hold the 8 values x of this lane, part of a 128-element block, in 8 bits.  The block's largest finite value goes on
-// 448, the largest e4m3 number; what is not finite is held as NaN.  `up`: a value that is not 0 is not held as 0
-// (a root held as 0 would divide its moment by eps alone).
-__device__ __forceinline__ void mt_hold8(void* base, float* scales, int64_t i, bool whole, int left, f32x8 x, const uint32_t d[8], bool up) {
-  float top = 0.f;
+// Hold the 8 values x of this lane, part of a 128-element block, in 8 bits.  The block's largest finite value is held as
+// 448, the largest e4m3 number; what is not finite (ODD: the wave has such a value), as NaN.  UP: a value that is not 0
+// is not held as 0 (a root held as 0 would divide its moment by eps alone).
+template <bool FULL, bool UP, bool ODD>
+__device__ __forceinline__ void mt_hold8(void* base, float* scales, int64_t i, int left, const Hold8& h, const uint32_t d[8]) {
+  const double most = 3.4028234663852886e38;
+  double top = 0.0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float ax = fabsf(x[e]);
-    top = fmaxf(top, ax <= 3.402823466e38f ? ax : 0.f);
+    const double ax = fabs(h.x[e]);
+    top = fmax(top, ODD ? (ax <= most ? ax : 0.0) : ax);
   }
-  const float s = fmaxf(mt_max16(top), 7.88860905e-31f) / 448.f;      // at least 2^-100 / 448: 1 / s stays finite
-  const float inv = 1.f / s;
+  top = fmax(mt_max16(top), 7.888609052210118e-31);                     // at least 2^-100: the fp32 scale stays normal
+  const double inv = 448.0 / top;
   uint32_t q[2] = {0u, 0u};
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float xe = x[e], ax = fabsf(xe);
-    uint32_t c = mt_code8(fminf(ax * inv, 448.f), d[e]);
-    if (up && ax > 0.f && c == 0u) c = 1u;
-    if (!(ax <= 3.402823466e38f)) c = 0x7fu;
-    c |= (__builtin_bit_cast(uint32_t, xe) >> 24) & 0x80u;
+    const double ax = fabs(h.x[e]);
+    uint32_t c = mt_code8(ax * inv, d[e]);
+    c = ax == top ? 0x7eu : min(c, 0x7eu);
+    if (UP) c = max(c, ax > 0.0 ? 1u : 0u);
+    if (ODD) c = ax <= most ? c : 0x7fu;
+    c |= (uint32_t)(__builtin_bit_cast(uint64_t, h.x[e]) >> 56) & 0x80u;
     q[e >> 2] |= c << (8 * (e & 3));
   }
-  if (whole) {
+  if (FULL) {
     *reinterpret_cast<u32x2*>((uint8_t*)base + i) = u32x2{q[0], q[1]};
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (e < left) ((uint8_t*)base)[i + e] = (uint8_t)(q[e >> 2] >> (8 * (e & 3)));
   }
-  if ((threadIdx.x & 15) == 0 && left > 0) scales[i / MT_BLOCK8] = s;
+  if ((threadIdx.x & 15) == 0 && left > 0) scales[i / MT_BLOCK8] = (float)(top * (1.0 / 448.0));
+}
+
+// One pass of a block: 8 elements of each thread from i.  FULL: all of them exist and every buffer is aligned.
+template <bool S8, bool FULL>
+__device__ __forceinline__ void adamw_pass(const AdamwArgs& a, const MtRec& r, int64_t i, int left, double gs, float keep,
+                                           float step_size, float inv_bc2s) {
+#pragma clang fp contract(off)
+  const Raw8 graw = mt_load<FULL>(r.g, i, r.g_t, left), praw = mt_load<FULL>(r.p, i, r.p_t, left);
+  f32x8 p;
+  if (S8) {
+    const u32x2 mc = mt_load8<FULL>(r.m, i, left), rc = mt_load8<FULL>(r.v, i, left);
+    const double ms = FULL || left > 0 ? r.ms[i / MT_BLOCK8] : 0.f, vs = FULL || left > 0 ? r.vs[i / MT_BLOCK8] : 0.f;
+    u32x4 dw;
+    if (r.dith) {
+      dw = mt_load<FULL>(r.dith, i, DPC_F16, left).a;
+    } else {
+      const DpcPhilox4 ph = dpc_philox(a.rng[0], a.rng[1], a.site, (uint64_t)(r.draw8 + (i >> 3)));
+      dw = u32x4{ph.v[0], ph.v[1], ph.v[2], ph.v[3]};
+    }
+    const f32x8 g = mt_float(graw, r.g_t), mf = mt_float8(mc), rf = mt_float8(rc);
+    p = mt_float(praw, r.p_t);
+    uint32_t d[8];
+    Hold8 m, rt;
+    float odd = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      d[e] = (dw[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+      const double ge = (double)g[e] * gs, re = (double)rf[e] * vs;
+      m.x[e] = a.b1d * ((double)mf[e] * ms) + a.c1d * ge;
+      rt.x[e] = mt_root(a.b2d * (re * re) + a.c2d * ge * ge);
+      const float m32 = (float)m.x[e], r32 = (float)rt.x[e];
+      odd += 0.f * m32 + 0.f * r32;                                    // NaN once a value is not finite
+      p[e] = adamw_param(a, p[e], m32, r32, keep, step_size, inv_bc2s);
+    }
+    if (__any(odd != 0.f)) {
+      mt_hold8<FULL, false, true>(r.m, r.ms, i, left, m, d);
+      mt_hold8<FULL, true, true>(r.v, r.vs, i, left, rt, d);
+    } else {
+      mt_hold8<FULL, false, false>(r.m, r.ms, i, left, m, d);
+      mt_hold8<FULL, true, false>(r.v, r.vs, i, left, rt, d);
+    }
+  } else {
+    const Raw8 mraw = mt_load<FULL>(r.m, i, DPC_F32, left), vraw = mt_load<FULL>(r.v, i, DPC_F32, left);
+    const f32x8 g = mt_float(graw, r.g_t);
+    f32x8 m = mt_float(mraw, DPC_F32), v = mt_float(vraw, DPC_F32);
+    p = mt_float(praw, r.p_t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float ge = g[e] * (float)gs;
+      m[e] = a.b1 * m[e] + a.c1 * ge;
+      v[e] = a.b2 * v[e] + a.c2 * ge * ge;
+      p[e] = adamw_param(a, p[e], m[e], sqrtf(v[e]), keep, step_size, inv_bc2s);
+    }
+    mt_store<FULL>(r.m, i, DPC_F32, left, m);
+    mt_store<FULL>(r.v, i, DPC_F32, left, v);
+  }
+  mt_store<FULL>(r.p, i, r.p_t, left, p);
+  if (r.cp) mt_store<FULL>(r.cp, i, r.c_t, left, p);
 }
 
 template <bool S8>
@@ -229,53 +323,16 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwArgs a) {
     step_size = bc[0];
     inv_bc2s = bc[1];
   }
-  const float gs = a.gscale * coef, keep = 1.f - a.lr * r.wd;
+  const double gs = (double)a.gscale * coef;
+  const float keep = 1.f - a.lr * r.wd;
   const int64_t end = min(ch.start + (int64_t)a.pl.chunk_len, r.n);
   // (whole passes of the block, also where the tensor ends inside: the 16 lanes of a state block stay together)
-  for (int64_t i = ch.start + 8 * threadIdx.x; i - 8 * (int64_t)threadIdx.x < end; i += MT_SUB) {
-    const int left = (int)max((int64_t)0, min((int64_t)8, end - i));
-    const bool whole = r.vec && left == 8;
-    f32x8 g = mt_load(r.g, i, r.g_t, whole, left), p = mt_load(r.p, i, r.p_t, whole, left);
-    f32x8 m, v, rt;
-    if (S8) {
-      const float ms = left > 0 ? r.ms[i / MT_BLOCK8] : 0.f, vs = left > 0 ? r.vs[i / MT_BLOCK8] : 0.f;
-      m = mt_load8(r.m, i, whole, left, ms);
-      v = mt_load8(r.v, i, whole, left, vs);
-      v *= v;
-    } else {
-      m = mt_load(r.m, i, DPC_F32, whole, left);
-      v = mt_load(r.v, i, DPC_F32, whole, left);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float me = m[e], ve = v[e], re;
-      p[e] = adamw_one(a, g[e] * gs, p[e], me, ve, re, keep, step_size, inv_bc2s);
-      m[e] = me; v[e] = ve; rt[e] = re;
-    }
-    if (S8) {
-      uint32_t d[8];
-      if (r.dith) {
-        if (whole) {
-          const u32x4 q = *reinterpret_cast<const u32x4*>(r.dith + i);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) d[e] = (q[e >> 1] >> (16 * (e & 1))) & 0xffffu;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) d[e] = e < left ? r.dith[i + e] : 0u;
-        }
-      } else {
-        const DpcPhilox4 ph = dpc_philox(a.rng[0], a.rng[1], a.site, (uint64_t)(r.draw8 + (i >> 3)));
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = (ph.v[e >> 1] >> (16 * (e & 1))) & 0xffffu;
-      }
-      mt_hold8(r.m, r.ms, i, whole, left, m, d, false);
-      mt_hold8(r.v, r.vs, i, whole, left, rt, d, true);
-    } else {
-      mt_store(r.m, i, DPC_F32, whole, left, m);
-      mt_store(r.v, i, DPC_F32, whole, left, v);
-    }
-    mt_store(r.p, i, r.p_t, whole, left, p);
-    if (r.cp) mt_store(r.cp, i, r.c_t, whole, left, p);
+  for (int64_t at = ch.start; at < end; at += MT_SUB) {
+    const int64_t i = at + 8 * threadIdx.x;
+    if (r.vec && end - at >= MT_SUB)
+      adamw_pass<S8, true>(a, r, i, 8, gs, keep, step_size, inv_bc2s);
+    else
+      adamw_pass<S8, false>(a, r, i, (int)max((int64_t)0, min((int64_t)8, end - i)), gs, keep, step_size, inv_bc2s);
   }
 }
 
@@ -385,7 +442,7 @@ extern "C" int dpc_adamw_step(const dpc_multi_info* info, const void* plan, doub
   AdamwArgs a;
   a.pl = mt_view(info, plan);
   a.lr = (float)lr; a.b1 = (float)b1; a.b2 = (float)b2; a.c1 = (float)(1.0 - b1); a.c2 = (float)(1.0 - b2); a.eps = (float)eps;
-  a.b1d = b1; a.b2d = b2;
+  a.b1d = b1; a.b2d = b2; a.c1d = 1.0 - b1; a.c2d = 1.0 - b2;
   a.step_size = a.inv_bc2s = 0.f;
   if (!t_dev) {
     a.step_size = (float)(lr / (1.0 - pow(b1, t_host)));
