@@ -1,0 +1,749 @@
+// Softmax cross entropy of a Linear layer over a large vocabulary, with its gradients, logits never whole in memory.
+//
+//   l = h W^T,  lse_r = log sum_v e^(l_rv),  loss_r = lse_r - l_(r, t_r),
+//   d_rv = e^(l_rv - lse_r) - [v = t_r],  dh = alpha d W,  dW = alpha d^T h,  alpha = gscale / rows that count.
+//
+// Half-precision operands (bf16, fp16), per piece of rows:
+//   1. logits tiles on the matrix cores, fp32 accumulators.  A wave reduces its 128 vocabulary entries of a row to
+//      (max, sum of e^(l - max)) in fp32 and, for training, leaves e^(l - max) in fp16 (values in (0, 1]: 11 bits where a
+//      later bf16 holds 8, so what reaches the gradients is rounded once) in P.
+//   2. per row: lse from the (max, sum) pairs, the loss, p_t - 1 by expm1 (no cancellation for sure rows).
+//   3. P becomes d in the operands' type: e^(max - lse) times what is there, p_t - 1 in the target's place, exactly 0 in
+//      rows that are ignored.
+//   4. dh and dW as products over d.  dW of several pieces adds up in fp32.
+// That is 6 T V D flops, the least there is without keeping the logits; they bound it: d costs 4 bytes of traffic per
+// logit against 6 D flops.
+//
+// P's layout [vocabulary / 8][row][8 entries] serves all three products: 16-byte chunks of 8 vocabulary entries are k-runs
+// of the dh product's operand and, transposed on the way out of LDS, m-runs of dW's; step 1 and 3 touch it in runs of
+// consecutive rows.
+//
+// fp32 operands: the products are dpc_gemm_f32_ex's (fp32 matrix cores), the logits of a piece in fp32.
+#include "dpc_common.h"
+#include "../../include/dpcgan_hip.h"
+#include <math.h>
+#include <string.h>
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+#define LCE_BK 64
+#define LCE_SLAB 128            // vocabulary entries of one (max, sum) pair
+#define LCE_LOG2E 1.4426950408889634f
+#define LCE_LN2 0.6931471805599453f
+
+enum { LCE_LOGITS = 0, LCE_DH = 1, LCE_DW = 2 };
+
+// 16-bit element types: the matrix instruction, and the conversion of 8 results
+template <typename E> struct Half;
+template <> struct Half<__bf16> {
+  typedef bf16x8 v8;
+  static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  static constexpr float kUp = 1.f;         // d as it is: bf16 has fp32's range
+};
+template <> struct Half<_Float16> {
+  typedef f16x8 v8;
+  static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+  static constexpr float kUp = 16384.f;     // |d| <= 1 lifted by 2^14: probabilities stay normal numbers down to 2^-28
+};
+
+// What a product reads and writes.  The result is C[n][m]: m is the contiguous axis of the output.
+struct LceArgs {
+  const char* A; int64_t lda;     // LOGITS: W [V][D]; DH: W [V][D] (k = row); DW: masked h [rows][D] (k = row); bytes per row
+  const char* B; int64_t ldb;     // LOGITS: h [rows][D]
+  char* P; int64_t prow;          // P, rows of one chunk column
+  int M, N, K;
+  int tiles_m, tiles_n;
+  const char* zero;               // 16 zero bytes
+  // LOGITS
+  f32x2* stat;                    // [slab][prow] (max * log2 e, sum)
+  float* lt;                      // [row] logit of the target
+  const int64_t* target;
+  int grads;
+  // DH / DW
+  const float* alpha;
+  void* C; int64_t ldc;           // elements
+  int c_f32;                      // C is fp32 (a slab of a split product, or the gradient itself)
+  const float* add;               // fp32 [n][ldadd] added to the result (accumulation over pieces, or into dW)
+  int64_t ldadd;
+  int splits; int kchunk; int64_t slab;   // K ranges, each into its own fp32 slab (elements)
+};
+
+// Runs of neighbouring tiles per XCD: blocks go to the 8 XCDs in turn; each XCD takes a contiguous run of tile numbers
+// (the tail that does not divide by 8 stays in place).
+__device__ __forceinline__ int lce_xcd(int b, int total) {
+  const int per = total >> 3, even = per << 3;
+  return b < even ? (b & 7) * per + (b >> 3) : b;
+}
+
+__device__ __forceinline__ void lce_dma(const char* src, char* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+__device__ __forceinline__ u32x2 lce_tr(const char* lds) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lds));
+}
+
+// One BM x BN tile of a product, WM x WN waves.  A tile of an operand is 64 k; it goes from memory straight into LDS, 16
+// bytes per lane, in one of two images:
+//   k-runs  (W and h of LOGITS, P of DH): [row][8 chunks of 8 k], chunk c of row r at c ^ (r & 7)  - read 16 bytes a lane
+//   m-runs  (W of DH, h of DW): [k][chunks of 8 m], chunk c of row k at c ^ 2 (k & 3)              - read transposed
+//           (P of DW): [chunk of 8 m][k], k at k ^ 4 (chunk & 1)                                     - read transposed
+// The transposing read gives lane i of 16 the column i of a 4 x 16 block whose row r comes from lanes 4r .. 4r+3; the
+// swizzles put what 16 lanes read on 32 different banks.
+template <typename E, int MODE, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
+  using H = Half<E>;
+  constexpr int NT = WM * WN * 64;
+  constexpr int SM = BM / WM / 32, SN = BN / WN / 32;
+  constexpr int NA = BM * 8 / NT, NB = BN * 8 / NT;
+  constexpr bool A_K = MODE == LCE_LOGITS, B_K = MODE != LCE_DW;
+  __shared__ __attribute__((aligned(1024))) char lds[2][(BM + BN) * 128];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  // tile: groups of 8 m-tiles run through all n-tiles, so that the tiles an XCD works on at a time share rows of both operands
+  const int tiles = g.tiles_m * g.tiles_n;
+  const int slot = lce_xcd(blockIdx.x, gridDim.x);
+  const int split = slot / tiles, tl = slot - split * tiles;
+  const int per = 8 * g.tiles_n, grp = tl / per, gm = min(8, g.tiles_m - grp * 8);
+  const int m0 = (grp * 8 + (tl - grp * per) % gm) * BM, n0 = ((tl - grp * per) / gm) * BN;
+  const int k_begin = split * g.kchunk, k_end = min(g.K, k_begin + g.kchunk);
+  const int nk = (k_end - k_begin + LCE_BK - 1) / LCE_BK;
+
+  // sources of this thread's chunks of a K-tile (the tile's own offset is added as it goes)
+  const char* sa[NA];
+  const char* sb[NB];
+  int64_t step_a, step_b;
+  if (A_K) {
+    const int c = (tid & 7) ^ ((tid >> 3) & 7);
+#pragma unroll
+    for (int i = 0; i < NA; ++i) sa[i] = g.A + (int64_t)min(m0 + i * (NT / 8) + (tid >> 3), g.M - 1) * g.lda + c * 16;
+    step_a = LCE_BK * 2;
+  } else {
+    constexpr int CR = BM / 8;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      const int k = i * (NT / CR) + tid / CR, c = (tid % CR) ^ (2 * (k & 3));
+      sa[i] = g.A + (int64_t)(k_begin + k) * g.lda + min(m0 / 8 + c, g.M / 8 - 1) * 16;
+    }
+    step_a = LCE_BK * g.lda;
+  }
+  if (MODE == LCE_LOGITS) {
+    const int c = (tid & 7) ^ ((tid >> 3) & 7);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) sb[i] = g.B + (int64_t)min(n0 + i * (NT / 8) + (tid >> 3), g.N - 1) * g.ldb + c * 16;
+    step_b = LCE_BK * 2;
+  } else if (MODE == LCE_DH) {
+    const int c = (tid & 7) ^ ((tid >> 3) & 7);
+#pragma unroll
+    for (int i = 0; i < NB; ++i) sb[i] = g.P + ((int64_t)(k_begin / 8 + c) * g.prow + n0 + i * (NT / 8) + (tid >> 3)) * 16;
+    step_b = 8 * g.prow * 16;
+  } else {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int n8 = i * (NT / 64) + (tid >> 6), k = (tid & 63) ^ (4 * (n8 & 1));
+      sb[i] = g.P + ((int64_t)(n0 / 8 + n8) * g.prow + k_begin + k) * 16;
+    }
+    step_b = LCE_BK * 16;
+  }
+  const auto issue = [&](int kt, char* buf) {
+    const int k0 = k_begin + kt * LCE_BK;
+    const bool tail = k0 + LCE_BK > g.K;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      const char* s = sa[i] + kt * step_a;
+      if (tail) {
+        if (A_K) {
+          if (k0 / 8 + ((tid & 7) ^ ((tid >> 3) & 7)) >= g.K / 8) s = g.zero;
+        } else if (MODE == LCE_DH) {            // (rows of W past the vocabulary: any finite row, P holds 0 there)
+          const int k = k0 + i * (NT / (BM / 8)) + tid / (BM / 8);
+          s -= (int64_t)max(0, k - (g.K - 1)) * g.lda;
+        }
+      }
+      lce_dma(s, buf + (i * NT + wave * 64) * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const char* s = sb[i] + kt * step_b;
+      if (tail && MODE == LCE_LOGITS && k0 / 8 + ((tid & 7) ^ ((tid >> 3) & 7)) >= g.K / 8) s = g.zero;
+      lce_dma(s, buf + BM * 128 + (i * NT + wave * 64) * 16);
+    }
+  };
+
+  f32x16 acc[SM][SN];
+#pragma unroll
+  for (int i = 0; i < SM; ++i)
+#pragma unroll
+    for (int j = 0; j < SN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+  // lane addresses inside an image
+  const int l16 = lane & 15, G = lane >> 4;
+  const int krow = (lane & 31) * 128;                                  // k-runs: row of this lane
+  const int mk = (8 * (G >> 1) + (l16 >> 2)) * (BM * 2);                // m-runs [k][chunk]: k of this lane
+  const int mc = 2 * (G & 1) + ((l16 & 3) >> 1), mx = 2 * (l16 >> 2), mh = (l16 & 1) * 8;
+  const int pb = ((l16 >> 1) & 1) * 4;                                  // m-runs [chunk][k]
+  const auto frag_a = [&](const char* buf, int s, int i) -> typename H::v8 {
+    const int r0 = (wm * SM + i) * 32;
+    if (A_K) return *reinterpret_cast<const typename H::v8*>(buf + r0 * 128 + krow + (((2 * s + (lane >> 5)) ^ (lane & 7)) * 16));
+    const char* q = buf + mk + s * 16 * (BM * 2) + (((r0 / 8 + mc) ^ mx) * 16) + mh;
+    const u32x2 lo = lce_tr(q), hi = lce_tr(q + 4 * (BM * 2));
+    return __builtin_bit_cast(typename H::v8, u32x4{lo.x, lo.y, hi.x, hi.y});
+  };
+  const auto frag_b = [&](const char* buf, int s, int j) -> typename H::v8 {
+    const int r0 = (wn * SN + j) * 32;
+    if (B_K) return *reinterpret_cast<const typename H::v8*>(buf + r0 * 128 + krow + (((2 * s + (lane >> 5)) ^ (lane & 7)) * 16));
+    const char* q = buf + (r0 / 8 + mc) * 1024 + (s * 16 + 8 * (G >> 1) + (l16 >> 2)) * 16 + mh;
+    const u32x2 lo = lce_tr(q + pb * 16), hi = lce_tr(q + (4 - pb) * 16);
+    return __builtin_bit_cast(typename H::v8, u32x4{lo.x, lo.y, hi.x, hi.y});
+  };
+
+  if (nk > 0) issue(0, lds[0]);
+  for (int kt = 0; kt < nk; ++kt) {
+    const char* buf = lds[kt & 1];
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                    // this wave's share of tile kt has landed ...
+    __syncthreads();                                                    // ... every wave's; and tile kt - 1 has been read
+    if (kt + 1 < nk) issue(kt + 1, lds[(kt + 1) & 1]);
+#pragma unroll
+    for (int s = 0; s < LCE_BK / 16; ++s) {
+      typename H::v8 a[SM], b[SN];
+#pragma unroll
+      for (int i = 0; i < SM; ++i) a[i] = frag_a(buf, s, i);
+#pragma unroll
+      for (int j = 0; j < SN; ++j) b[j] = frag_b(buf + BM * 128, s, j);
+#pragma unroll
+      for (int i = 0; i < SM; ++i)
+#pragma unroll
+        for (int j = 0; j < SN; ++j) acc[i][j] = H::mfma(a[i], b[j], acc[i][j]);
+    }
+  }
+
+  // C layout of a 32 x 32 block: n = lane & 31, m = (e & 3) + 8 (e >> 2) + 4 (lane >> 5)
+  const int half = lane >> 5;
+  const int mw = m0 + wm * SM * 32, nw = n0 + wn * SN * 32 + (lane & 31);
+  if (MODE == LCE_LOGITS) {
+    if (mw + SM * 32 > g.M) {
+#pragma unroll
+      for (int i = 0; i < SM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (mw + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * half >= g.M)
+#pragma unroll
+            for (int j = 0; j < SN; ++j) acc[i][j][e] = -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < SN; ++j) {
+      const int n = nw + j * 32;
+      const bool row = n < g.N;
+      const int64_t t = row ? g.target[n] : -1;
+      if (__any(t >= mw && t < mw + SM * 32)) {
+        const int at = (int)(t - mw);
+#pragma unroll
+        for (int i = 0; i < SM; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (t >= mw && at == i * 32 + (e & 3) + 8 * (e >> 2) + 4 * half) g.lt[n] = acc[i][j][e];
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < SM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, acc[i][j][e]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64)) * LCE_LOG2E;
+      const float ref = top == -INFINITY ? 0.f : top;                  // (all -inf: e^(l - 0) = 0, not NaN)
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < SM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], LCE_LOG2E, -ref));
+          sum += acc[i][j][e];
+        }
+      sum += __shfl_xor(sum, 32, 64);
+      if (half == 0 && mw < g.M) g.stat[(int64_t)(mw / LCE_SLAB) * g.prow + n] = f32x2{top, sum};
+      if (g.grads) {
+#pragma unroll
+        for (int i = 0; i < SM; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; q += 2) {
+            u32x2 x[2];
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const f16x2 v = {(_Float16)acc[i][j][4 * (q + w) + 2 * c], (_Float16)acc[i][j][4 * (q + w) + 2 * c + 1]};
+                x[w][c] = __builtin_bit_cast(uint32_t, v);
+              }
+            // lanes below 32 come to hold chunk q of their row, the others chunk q + 1 of the same rows
+            const auto s0 = __builtin_amdgcn_permlane32_swap(x[0].x, x[1].x, false, false);
+            const auto s1 = __builtin_amdgcn_permlane32_swap(x[0].y, x[1].y, false, false);
+            const int64_t chunk = (mw + i * 32) / 8 + q + half;
+            *reinterpret_cast<u32x4*>(g.P + (chunk * g.prow + n) * 16) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+          }
+      }
+    }
+  } else {
+    const float alpha = g.splits > 1 ? 1.f : g.alpha[0];
+#pragma unroll
+    for (int j = 0; j < SN; ++j) {
+      const int n = nw + j * 32;
+      if (n >= g.N) continue;
+#pragma unroll
+      for (int i = 0; i < SM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int m = mw + i * 32 + 8 * q + 4 * half;
+          if (m >= g.M) continue;
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = alpha * acc[i][j][4 * q + e];
+          if (g.add) v += *reinterpret_cast<const f32x4*>(g.add + (int64_t)n * g.ldadd + m);
+          const int64_t o = (int64_t)n * g.ldc + m + split * g.slab;
+          if (g.c_f32) *reinterpret_cast<f32x4*>((float*)g.C + o) = v;
+          else {
+            typedef E e4 __attribute__((ext_vector_type(4)));
+            *reinterpret_cast<e4*>((E*)g.C + o) = __builtin_convertvector(v, e4);
+          }
+        }
+    }
+  }
+}
+
+// ---- the passes between the products --------------------------------------------------------------------------------
+// alpha = gscale / (rows that count, or 1) / lift; zero: 16 zero bytes; count as a float for the mean of the losses
+__global__ __launch_bounds__(1024) void lce_begin_kernel(const int64_t* target, int64_t T, int64_t ignore, int V, int mean, float gscale,
+                                                         float lift, float* head) {
+  __shared__ int red[16];
+  int c = 0;
+  if (mean)
+    for (int64_t i = threadIdx.x; i < T; i += 1024) c += target[i] != ignore;
+  c = dpc_block_sum(c, red);
+  if (threadIdx.x == 0) {
+    const float n = mean ? (float)max(c, 1) : 1.f;
+    head[0] = gscale / n / lift;
+    head[1] = n;
+    head[2] = 1.f;
+  }
+  if (threadIdx.x < 4) head[4 + threadIdx.x] = 0.f;
+}
+
+// Per row: lse from the slabs' (max, sum) pairs.  32 rows x 8 lanes of slabs per block.
+struct LceRowArgs {
+  const f32x2* stat; int64_t prow; int slabs; int rows; int V;
+  const float* lt; const int64_t* target; int64_t ignore;
+  float* loss; float* lse;      // lse nullable
+  float* glse;                  // lse * log2 e, +inf in rows that take no part in the gradient
+  float* pm1;                   // p_t - 1
+};
+__device__ __forceinline__ void lce_row_end(const LceRowArgs& a, int n, float lse, float lt) {
+  const int64_t t = a.target[n];
+  const bool off = t == a.ignore, bad = !off && (t < 0 || t >= a.V);
+  const float loss = off ? 0.f : (bad ? NAN : lse - lt);
+  a.loss[n] = loss;
+  if (a.lse) a.lse[n] = lse;
+  if (a.glse) {
+    a.glse[n] = off || bad ? INFINITY : lse * LCE_LOG2E;
+    a.pm1[n] = off || bad ? 0.f : expm1f(-loss);
+  }
+}
+__global__ __launch_bounds__(256) void lce_rows_kernel(LceRowArgs a) {
+  __shared__ f32x2 red[8][32];
+  const int r = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int n = blockIdx.x * 32 + r;
+  float top = -INFINITY, sum = 0.f;
+  if (n < a.rows) {
+    for (int s = w; s < a.slabs; s += 8) {
+      const f32x2 x = a.stat[(int64_t)s * a.prow + n];
+      const float m = fmaxf(top, x.x);
+      const float ref = m == -INFINITY ? 0.f : m;
+      sum = sum * __builtin_amdgcn_exp2f(top - ref) + x.y * __builtin_amdgcn_exp2f(x.x - ref);
+      top = m;
+    }
+  }
+  red[w][r] = f32x2{top, sum};
+  __syncthreads();
+  if (w == 0 && n < a.rows) {
+    float m = top;
+    for (int k = 1; k < 8; ++k) m = fmaxf(m, red[k][r].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
+    for (int k = 0; k < 8; ++k) s += red[k][r].y * __builtin_amdgcn_exp2f(red[k][r].x - ref);
+    lce_row_end(a, n, (ref + __builtin_amdgcn_logf(s)) * LCE_LN2, a.lt[n]);
+  }
+}
+
+// P from e^(l - slab max) in fp16 to d in the operands' type, in place.  One thread per row and slab.
+template <typename E>
+__global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, const f32x2* stat, int rows, int V, int chunks, const float* glse,
+                                                        const float* pm1, const int64_t* target) {
+  const int n = blockIdx.x * 256 + threadIdx.x, slab = blockIdx.y;
+  const float gl = n < rows ? glse[n] : INFINITY;
+  const bool live = gl != INFINITY;
+  const float f = live ? __builtin_amdgcn_exp2f(stat[(int64_t)slab * prow + n].x - gl) * Half<E>::kUp : 0.f;
+  int at = -1;
+  float pt = 0.f;
+  if (live) {
+    const int64_t t = target[n] - (int64_t)slab * LCE_SLAB;
+    if (t >= 0 && t < LCE_SLAB) { at = (int)t; pt = pm1[n] * Half<E>::kUp; }
+  }
+#pragma unroll 4
+  for (int c = 0; c < LCE_SLAB / 8; ++c) {
+    if (slab * (LCE_SLAB / 8) + c >= chunks) break;
+    u32x4* q = reinterpret_cast<u32x4*>(P + ((int64_t)(slab * (LCE_SLAB / 8) + c) * prow + n) * 16);
+    const f16x8 x = __builtin_bit_cast(f16x8, *q);
+    typename Half<E>::v8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (E)(live ? (c * 8 + e == at ? pt : (float)x[e] * f) : 0.f);
+    *q = __builtin_bit_cast(u32x4, y);
+  }
+}
+
+// h with its ignored rows, and the rows up to the end of the piece's last tile, set to 0: what such a row holds must
+// not reach dW (0 x NaN)
+__global__ __launch_bounds__(256) void lce_mask_rows_kernel(const char* h, int64_t ldh, int rows, int64_t total16, int row16, const float* glse, char* out) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total16; i += (int64_t)gridDim.x * 256) {
+    const int n = (int)(i / row16), c = (int)(i - (int64_t)n * row16);
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (n < rows && glse[n] != INFINITY) v = *reinterpret_cast<const u32x4*>(h + (int64_t)n * ldh + c * 16);
+    *reinterpret_cast<u32x4*>(out + i * 16) = v;
+  }
+}
+
+// out[n][m] = alpha * sum of the split product's slabs, in their order
+template <typename E>
+__global__ __launch_bounds__(256) void lce_fold_kernel(const float* slabs, int64_t slab, int splits, int N, int M, const float* alpha,
+                                                       const float* add, int64_t ldadd, void* out, int64_t ldo, int out_f32) {
+  const int m4 = M / 4;
+  const float al = alpha[0];
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)N * m4; i += (int64_t)gridDim.x * 256) {
+    const int n = (int)(i / m4), m = (int)(i - (int64_t)n * m4) * 4;
+    f32x4 v = *reinterpret_cast<const f32x4*>(slabs + i * 4);
+    for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(slabs + s * slab + i * 4);
+    v *= al;
+    if (add) v += *reinterpret_cast<const f32x4*>(add + (int64_t)n * ldadd + m);
+    if (out_f32) *reinterpret_cast<f32x4*>((float*)out + (int64_t)n * ldo + m) = v;
+    else {
+      typedef E e4 __attribute__((ext_vector_type(4)));
+      *reinterpret_cast<e4*>((E*)out + (int64_t)n * ldo + m) = __builtin_convertvector(v, e4);
+    }
+  }
+}
+
+// fp32: a row of logits to its loss and, in place, to alpha d; and h with its ignored rows set to 0.  One block per row.
+__global__ __launch_bounds__(256) void lce_rows_f32_kernel(float* logits, int64_t ld, LceRowArgs a, const float* alpha, const float* h, int64_t ldh,
+                                                           float* hm, int D) {
+  __shared__ float red[16];
+  const int n = blockIdx.x;
+  float* x = logits + (int64_t)n * ld;
+  const int64_t t = a.target[n];
+  const bool live = t != a.ignore && t >= 0 && t < a.V;
+  float top = -INFINITY;
+  for (int v = threadIdx.x; v < a.V; v += 256) top = fmaxf(top, x[v]);
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float ref = top == -INFINITY ? 0.f : top * LCE_LOG2E;
+  float sum = 0.f;
+  for (int v = threadIdx.x; v < a.V; v += 256) sum += __builtin_amdgcn_exp2f(fmaf(x[v], LCE_LOG2E, -ref));
+  sum = dpc_block_sum(sum, red);
+  const float lse2 = ref + __builtin_amdgcn_logf(sum), lse = lse2 * LCE_LN2;
+  const float lt = live ? x[t] : 0.f;
+  if (threadIdx.x == 0) lce_row_end(a, n, lse, lt);
+  if (!alpha) return;
+  __syncthreads();                                                     // x[t] has been read
+  const float al = alpha[0];
+  for (int v = threadIdx.x; v < a.V; v += 256)
+    x[v] = live ? al * (v == t ? expm1f(lt - lse) : __builtin_amdgcn_exp2f(fmaf(x[v], LCE_LOG2E, -lse2))) : 0.f;
+  if (hm)
+    for (int k = threadIdx.x; k < D; k += 256) hm[(int64_t)n * D + k] = live ? h[(int64_t)n * ldh + k] : 0.f;
+}
+
+// out[n][m] = sum of the split product's fp32 slabs [n][M], in their order
+__global__ __launch_bounds__(256) void lce_fold_f32_kernel(const float* slabs, int64_t slab, int splits, int64_t N, int M, float* out, int64_t ldo) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < slab; i += (int64_t)gridDim.x * 256) {
+    float v = slabs[i];
+    for (int s = 1; s < splits; ++s) v += slabs[s * slab + i];
+    const int64_t n = i / M;
+    out[n * ldo + (i - n * M)] = v;
+  }
+}
+
+// M 16-bit words of each of N rows set to 0 (the gradient of no rows at all)
+__global__ __launch_bounds__(256) void lce_zero_kernel(uint16_t* out, int64_t ld, int64_t N, int M) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < N * M; i += (int64_t)gridDim.x * 256) {
+    const int64_t n = i / M;
+    out[n * ld + (i - n * M)] = 0;
+  }
+}
+
+// sum of the rows' losses over the rows that count (one block, fixed order)
+__global__ __launch_bounds__(1024) void lce_total_kernel(const float* loss, int64_t T, const float* head, float* total) {
+  __shared__ double red[16];
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < T; i += 1024) s += (double)loss[i];
+  s = dpc_block_sum(s, red);
+  if (threadIdx.x == 0) total[0] = (float)(s / (double)head[1]);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+static int64_t lce_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+static int lce_size(int dtype) { return dtype == DPC_F32 ? 4 : 2; }
+
+// Where things lie in the workspace for pieces of `rows` rows.
+struct LceLayout {
+  int64_t rows, prow;           // rows of a piece; padded to whole tiles
+  int64_t stat, lt, glse, pm1, P, hm, slabs, acc, bytes;   // byte offsets, and the whole
+  int splits_h, splits_w;
+  int pieces;
+};
+
+// K ranges of a product with `tiles` tiles: enough to give every CU a tile, none shorter than 512
+static int lce_splits(int64_t tiles, int64_t K) {
+  int64_t s = 256 / (tiles < 1 ? 1 : tiles);
+  if (s > K / 512) s = K / 512;
+  if (s > 32) s = 32;
+  return s < 1 ? 1 : (int)s;
+}
+
+static LceLayout lce_layout(int64_t T, int D, int V, int dtype, bool grads, bool dw16, int64_t rows) {
+  LceLayout l;
+  memset(&l, 0, sizeof(l));
+  l.rows = rows < T ? rows : T;
+  if (l.rows < 1) l.rows = 1;
+  l.pieces = (int)dpc_cdiv(T < 1 ? 1 : T, l.rows);
+  l.prow = lce_up(l.rows, 256);
+  int64_t at = 256;                                                    // head: alpha, count, 16 zero bytes
+  const auto take = [&](int64_t bytes) { const int64_t o = at; at += lce_up(bytes, 256); return o; };
+  l.lt = take(l.prow * 4);
+  l.glse = take(l.prow * 4);
+  l.pm1 = take(l.prow * 4);
+  l.splits_h = l.splits_w = 1;
+  if (dtype == DPC_F32) {
+    l.P = take(l.rows * (int64_t)V * 4);
+    if (grads) {
+      l.splits_h = lce_splits(dpc_cdiv(l.rows, 64) * dpc_cdiv(D, 64), V);
+      if (l.splits_h > 1) l.slabs = take(l.splits_h * l.rows * (int64_t)D * 4);
+      l.hm = take(l.rows * (int64_t)D * 4);
+    }
+  } else {
+    l.stat = take(dpc_cdiv(V, LCE_SLAB) * l.prow * 8);
+    if (grads) {
+      l.P = take(lce_up(V, 256) * l.prow * 2);
+      l.hm = take(l.prow * (int64_t)D * 2);
+      l.splits_h = lce_splits(dpc_cdiv(l.rows, 256) * dpc_cdiv(D, 256), V);
+      l.splits_w = lce_splits(dpc_cdiv(V, 256) * dpc_cdiv(D, 256), l.prow);
+      int64_t sl = 0;
+      if (l.splits_h > 1) sl = l.splits_h * l.rows * (int64_t)D * 4;
+      if (l.splits_w > 1 && l.splits_w * (int64_t)V * D * 4 > sl) sl = l.splits_w * (int64_t)V * D * 4;
+      if (sl) l.slabs = take(sl);
+      if (dw16 && l.pieces > 1) l.acc = take((int64_t)V * D * 4);
+    }
+  }
+  l.bytes = at;
+  return l;
+}
+
+static int lce_check(int64_t T, int D, int V, int dtype) {
+  DPC_CHECK_ARG(T >= 0 && T < (1ll << 31) && D >= 1 && V >= 1 && V <= (1 << 30), "linear_cross_entropy: bad size");
+  DPC_CHECK_ARG(dtype == DPC_F32 || dtype == DPC_BF16 || dtype == DPC_F16, "linear_cross_entropy: unknown element type");
+  DPC_CHECK_ARG(dtype == DPC_F32 || D % 8 == 0, "linear_cross_entropy: half-precision rows need a width that is a multiple of 8");
+  return DPC_OK;
+}
+
+// Rows of a piece where the caller names none: as many whole tiles as 1 GiB holds of what a row leaves (d, or the slabs'
+// pairs alone).
+static int64_t lce_rows_default(int V, int dtype, bool grads) {
+  const int64_t row = grads || dtype == DPC_F32 ? (int64_t)V * lce_size(dtype) : dpc_cdiv(V, LCE_SLAB) * 8;
+  const int64_t rows = (1ll << 30) / row / 256 * 256;
+  return rows < 256 ? 256 : rows;
+}
+
+extern "C" int64_t dpc_linear_cross_entropy_ws(int64_t T, int D, int V, int dtype, int grads, int dw_f32, int64_t piece_rows) {
+  if (lce_check(T, D, V, dtype) != DPC_OK) return -1;
+  if (piece_rows <= 0) piece_rows = lce_rows_default(V, dtype, grads != 0);
+  return lce_layout(T, D, V, dtype, grads != 0, dtype != DPC_F32 && !dw_f32, piece_rows).bytes;
+}
+
+template <typename E, int MODE>
+static void lce_launch(LceArgs& g, hipStream_t st) {
+  g.tiles_m = (int)dpc_cdiv(g.M, 256);
+  g.tiles_n = (int)dpc_cdiv(g.N, 256);
+  if (g.splits < 1) g.splits = 1;
+  g.kchunk = (int)lce_up(dpc_cdiv(g.K, g.splits), LCE_BK);
+  hipLaunchKernelGGL((lce_product_kernel<E, MODE, 256, 256, 2, 4>), dim3(g.tiles_m * g.tiles_n * g.splits), dim3(512), 0, st, g);
+}
+
+struct LceCall {
+  const char* h; int64_t ldh; const char* w; int64_t ldw;
+  int dtype; const int64_t* target; int64_t ignore; int64_t T; int D, V;
+  float* loss; float* lse; float* total;
+  char* dh; int64_t lddh; char* dw; int64_t lddw; int dw_f32, accumulate;
+  float gscale; int mean;
+  char* ws;
+};
+
+template <typename E>
+static int lce_half(const LceCall& c, const LceLayout& l, hipStream_t st) {
+  float* head = (float*)c.ws;
+  const bool grads = c.dh || c.dw;
+  const int slabs = (int)dpc_cdiv(c.V, LCE_SLAB);
+  for (int p = 0; p < l.pieces; ++p) {
+    const int64_t r0 = p * l.rows;
+    const int rows = (int)(c.T - r0 < l.rows ? c.T - r0 : l.rows);
+    const char* h = c.h + r0 * c.ldh * 2;
+    LceArgs g;
+    memset(&g, 0, sizeof(g));
+    g.P = c.ws + l.P; g.prow = l.prow; g.zero = (const char*)(head + 4); g.alpha = head; g.target = c.target + r0;
+    g.stat = (f32x2*)(c.ws + l.stat); g.lt = (float*)(c.ws + l.lt); g.grads = grads;
+    g.A = c.w; g.lda = c.ldw * 2; g.B = h; g.ldb = c.ldh * 2;
+    g.M = c.V; g.N = rows; g.K = c.D;
+    lce_launch<E, LCE_LOGITS>(g, st);
+    LceRowArgs ra;
+    ra.stat = g.stat; ra.prow = l.prow; ra.slabs = slabs; ra.rows = rows; ra.V = c.V; ra.lt = g.lt; ra.target = g.target; ra.ignore = c.ignore;
+    ra.loss = c.loss + r0; ra.lse = c.lse ? c.lse + r0 : nullptr;
+    ra.glse = grads ? (float*)(c.ws + l.glse) : nullptr; ra.pm1 = (float*)(c.ws + l.pm1);
+    hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)dpc_cdiv(rows, 32)), dim3(256), 0, st, ra);
+    if (!grads) continue;
+    const int chunks = (int)(lce_up(c.V, 256) / 8);
+    hipLaunchKernelGGL(lce_scale_kernel<E>, dim3((unsigned)(l.prow / 256), (unsigned)slabs), dim3(256), 0, st, g.P, l.prow, g.stat, rows, c.V,
+                       chunks, ra.glse, ra.pm1, g.target);
+    if (c.dh) {
+      LceArgs d = g;
+      d.A = c.w; d.lda = c.ldw * 2; d.M = c.D; d.N = rows; d.K = c.V; d.splits = l.splits_h;
+      if (l.splits_h > 1) { d.C = c.ws + l.slabs; d.ldc = c.D; d.c_f32 = 1; d.slab = (int64_t)rows * c.D; }
+      else { d.C = c.dh + r0 * c.lddh * 2; d.ldc = c.lddh; }
+      lce_launch<E, LCE_DH>(d, st);
+      if (l.splits_h > 1)
+        hipLaunchKernelGGL(lce_fold_kernel<E>, dim3(dpc_grid((int64_t)rows * c.D / 4, 256)), dim3(256), 0, st, (const float*)(c.ws + l.slabs),
+                           (int64_t)rows * c.D, l.splits_h, rows, c.D, head, nullptr, 0, c.dh + r0 * c.lddh * 2, c.lddh, 0);
+    }
+    if (c.dw) {
+      const int64_t row16 = c.D / 8;
+      char* hm = c.ws + l.hm;
+      hipLaunchKernelGGL(lce_mask_rows_kernel, dim3(dpc_grid(l.prow * row16, 256)), dim3(256), 0, st, h, c.ldh * 2, rows, l.prow * row16, (int)row16,
+                         ra.glse, hm);
+      LceArgs d = g;
+      d.A = hm; d.lda = (int64_t)c.D * 2; d.M = c.D; d.N = c.V; d.K = (int)lce_up(rows, LCE_BK); d.splits = l.splits_w;
+      // where the piece's share goes: dW itself, or the fp32 sums over the pieces until the last one
+      const bool last = p + 1 == l.pieces;
+      const bool via = !c.dw_f32 && l.pieces > 1;
+      float* acc = (float*)(c.ws + l.acc);
+      const float* add = via ? (p > 0 ? acc : nullptr) : (c.dw_f32 && (p > 0 || c.accumulate) ? (const float*)c.dw : nullptr);
+      void* out = via && !last ? (void*)acc : (void*)c.dw;
+      const int64_t ldo = via && !last ? c.D : c.lddw, ldadd = via ? c.D : c.lddw;
+      const int f32 = via ? !last : c.dw_f32;
+      if (l.splits_w > 1) { d.C = c.ws + l.slabs; d.ldc = c.D; d.c_f32 = 1; d.slab = (int64_t)c.V * c.D; }
+      else { d.C = out; d.ldc = ldo; d.c_f32 = f32; d.add = add; d.ldadd = ldadd; }
+      lce_launch<E, LCE_DW>(d, st);
+      if (l.splits_w > 1)
+        hipLaunchKernelGGL(lce_fold_kernel<E>, dim3(dpc_grid((int64_t)c.V * c.D / 4, 256)), dim3(256), 0, st, (const float*)(c.ws + l.slabs),
+                           (int64_t)c.V * c.D, l.splits_w, c.V, c.D, head, add, ldadd, out, ldo, f32);
+    }
+  }
+  return DPC_OK;
+}
+
+// fp32: the framework's own products (no split with atomics: the sums keep one order)
+static dpc_gemm_desc lce_desc(int M, int N, int K, const float* A, int64_t a_rs, int64_t a_cs, const float* B, int64_t b_rs, int64_t b_cs, float beta,
+                              float* C, int64_t ldc) {
+  dpc_gemm_desc d;
+  memset(&d, 0, sizeof(d));
+  d.M = M; d.N = N; d.K = K; d.alpha = 1.f; d.beta = beta; d.A = A; d.a_rs = a_rs; d.a_cs = a_cs; d.B = B; d.b_rs = b_rs; d.b_cs = b_cs;
+  d.C = C; d.ldc = ldc; d.splitk = 1;
+  return d;
+}
+static int lce_gemm(int M, int N, int K, const float* A, int64_t a_rs, int64_t a_cs, const float* B, int64_t b_rs, int64_t b_cs, float beta,
+                    float* C, int64_t ldc, hipStream_t st) {
+  const dpc_gemm_desc d = lce_desc(M, N, K, A, a_rs, a_cs, B, b_rs, b_cs, beta, C, ldc);
+  return dpc_gemm_f32_ex(&d, 1, st);
+}
+
+static int lce_full(const LceCall& c, const LceLayout& l, hipStream_t st) {
+  float* head = (float*)c.ws;
+  const bool grads = c.dh || c.dw;
+  for (int p = 0; p < l.pieces; ++p) {
+    const int64_t r0 = p * l.rows;
+    const int rows = (int)(c.T - r0 < l.rows ? c.T - r0 : l.rows);
+    const float* h = (const float*)c.h + r0 * c.ldh;
+    const float* w = (const float*)c.w;
+    float* P = (float*)(c.ws + l.P);
+    float* hm = (float*)(c.ws + l.hm);
+    int rc = lce_gemm(rows, c.V, c.D, h, c.ldh, 1, w, 1, c.ldw, 0.f, P, c.V, st);
+    if (rc != DPC_OK) return rc;
+    LceRowArgs ra;
+    memset(&ra, 0, sizeof(ra));
+    ra.rows = rows; ra.V = c.V; ra.target = c.target + r0; ra.ignore = c.ignore; ra.loss = c.loss + r0; ra.lse = c.lse ? c.lse + r0 : nullptr;
+    hipLaunchKernelGGL(lce_rows_f32_kernel, dim3(rows), dim3(256), 0, st, P, (int64_t)c.V, ra, grads ? head : nullptr, h, c.ldh,
+                       c.dw ? hm : nullptr, c.D);
+    if (c.dh) {
+      float* dh = (float*)c.dh + r0 * c.lddh;
+      if (l.splits_h > 1) {
+        float* slabs = (float*)(c.ws + l.slabs);
+        const int64_t slab = (int64_t)rows * c.D;
+        const int chunk = (int)lce_up(dpc_cdiv(c.V, l.splits_h), 32);
+        dpc_gemm_desc d[64];
+        int n = 0;
+        for (int k = 0; k < c.V; k += chunk, ++n)
+          d[n] = lce_desc(rows, c.D, c.V - k < chunk ? c.V - k : chunk, P + k, c.V, 1, w + k * c.ldw, c.ldw, 1, 0.f, slabs + n * slab, c.D);
+        rc = dpc_gemm_f32_group(d, n, st);
+        if (rc != DPC_OK) return rc;
+        hipLaunchKernelGGL(lce_fold_f32_kernel, dim3(dpc_grid(slab, 256)), dim3(256), 0, st, slabs, slab, n, (int64_t)rows, c.D, dh, c.lddh);
+      } else {
+        rc = lce_gemm(rows, c.D, c.V, P, c.V, 1, w, c.ldw, 1, 0.f, dh, c.lddh, st);
+        if (rc != DPC_OK) return rc;
+      }
+    }
+    if (c.dw) {
+      rc = lce_gemm(c.V, c.D, rows, P, 1, c.V, hm, c.D, 1, p > 0 || c.accumulate ? 1.f : 0.f, (float*)c.dw, c.lddw, st);
+      if (rc != DPC_OK) return rc;
+    }
+  }
+  return DPC_OK;
+}
+
+extern "C" int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, const int64_t* target,
+                                        int64_t ignore_index, int64_t T, int D, int V, float* loss, float* lse, float* total, void* dh,
+                                        int64_t lddh, void* dw, int64_t lddw, int dw_f32, int accumulate, float gscale, int mean,
+                                        int64_t piece_rows, void* ws, int64_t ws_bytes, void* stream) {
+  const int rc0 = lce_check(T, D, V, dtype);
+  if (rc0 != DPC_OK) return rc0;
+  DPC_CHECK_ARG(w && ws && (T == 0 || (h && target && loss)), "linear_cross_entropy: null pointer");
+  DPC_CHECK_ARG(ldh >= D && ldw >= D && (!dh || lddh >= D) && (!dw || lddw >= D), "linear_cross_entropy: a leading dimension is smaller than the width");
+  DPC_CHECK_ARG(!accumulate || (dw && (dw_f32 || dtype == DPC_F32)), "linear_cross_entropy: accumulation goes into an fp32 dw");
+  const bool f32 = dtype == DPC_F32;
+  if (!f32) {
+    const uintptr_t al = (uintptr_t)h | (uintptr_t)w | (uintptr_t)dh | (uintptr_t)dw | (uintptr_t)(ldh * 2) | (uintptr_t)(ldw * 2);
+    DPC_CHECK_ARG((al & 15) == 0, "linear_cross_entropy: half-precision rows must be 16-byte aligned");
+    DPC_CHECK_ARG((!dh || lddh % 8 == 0) && (!dw || lddw % (dw_f32 ? 4 : 8) == 0), "linear_cross_entropy: gradient rows must be 16-byte aligned");
+  }
+  DPC_CHECK_ARG(((uintptr_t)ws & 255) == 0, "linear_cross_entropy: the workspace must be 256-byte aligned");
+  const bool grads = dh || dw;
+  if (piece_rows <= 0) piece_rows = lce_rows_default(V, dtype, grads);
+  DPC_CHECK_ARG(dpc_cdiv(V, 256) * dpc_cdiv(piece_rows < T ? piece_rows : T, 256) * 32 < (1ll << 31), "linear_cross_entropy: the piece is too large");
+  const LceLayout l = lce_layout(T, D, V, dtype, grads, !f32 && !dw_f32, piece_rows);
+  DPC_CHECK_ARG(ws_bytes >= l.bytes, "linear_cross_entropy: the workspace is smaller than dpc_linear_cross_entropy_ws says");
+  hipStream_t st = (hipStream_t)stream;
+  LceCall c;
+  c.h = (const char*)h; c.ldh = ldh; c.w = (const char*)w; c.ldw = ldw; c.dtype = dtype; c.target = target; c.ignore = ignore_index; c.T = T;
+  c.D = D; c.V = V; c.loss = loss; c.lse = lse; c.total = total; c.dh = (char*)dh; c.lddh = lddh; c.dw = (char*)dw; c.lddw = lddw;
+  c.dw_f32 = dw_f32 || f32; c.accumulate = accumulate; c.gscale = gscale; c.mean = mean; c.ws = (char*)ws;
+  const float lift = dtype == DPC_F16 ? Half<_Float16>::kUp : 1.f;
+  hipLaunchKernelGGL(lce_begin_kernel, dim3(1), dim3(1024), 0, st, target, T, ignore_index, V, mean, gscale, lift, (float*)ws);
+  if (T == 0 && dw && !accumulate)
+    hipLaunchKernelGGL(lce_zero_kernel, dim3(dpc_grid((int64_t)V * D, 256)), dim3(256), 0, st, (uint16_t*)dw, c.dw_f32 ? 2 * lddw : lddw, (int64_t)V,
+                       c.dw_f32 ? 2 * D : D);
+  const int rc = T == 0 ? DPC_OK : f32 ? lce_full(c, l, st) : (dtype == DPC_BF16 ? lce_half<__bf16>(c, l, st) : lce_half<_Float16>(c, l, st));
+  if (rc != DPC_OK) return rc;
+  if (total) hipLaunchKernelGGL(lce_total_kernel, dim3(1), dim3(1024), 0, st, loss, T, (const float*)ws, total);
+  DPC_LAUNCH_CHECK();
+  return DPC_OK;
+}

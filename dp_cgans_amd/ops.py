@@ -17,6 +17,7 @@ SITE_Z, SITE_GUMBEL, SITE_DROP0, SITE_ALPHA, SITE_CONDVEC, SITE_ROWPICK, SITE_PE
 SITE_NOISE_D, SITE_HOOK, SITE_ENCODE, SITE_DITHER = 7, 8, 9, 10
 
 
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # DPC_F32, DPC_BF16, DPC_F16
 _dev_index = None        # GPU of the tensors of the call being assembled (see _stream)
 
 
@@ -664,8 +665,54 @@ def adam_step_slices(p, g, m, v, lr, wd, mats, slices, b1=0.5, b2=0.9, eps=1e-8,
                I64s(*[(_ld(pT) if pT is not None else 0) for _, _, _, _, pT in slices]), _stream())
 
 
+def linear_cross_entropy_ws(T, D, V, dtype, grads=True, dw_f32=False, piece_rows=0):
+    """Bytes of the workspace of linear_cross_entropy over T rows of width D (element type ``dtype``) and V classes."""
+    if dtype not in _TYPES:
+        raise TypeError('linear_cross_entropy: h and w must be fp32, bf16 or fp16, got %s' % (dtype,))
+    L = lib()
+    n = L.cdll.dpc_linear_cross_entropy_ws(int(T), int(D), int(V), _TYPES[dtype], int(bool(grads)), int(bool(dw_f32)), int(piece_rows))
+    if n < 0:
+        raise RuntimeError('dpc_linear_cross_entropy_ws: %s' % L.cdll.dpc_last_error().decode())
+    return n
+
+
+def linear_cross_entropy(h, w, target, loss, ws, dh=None, dw=None, lse=None, total=None, ignore_index=-100, mean=True,
+                         gscale=1.0, accumulate=False, piece_rows=0):
+    """Softmax cross entropy of the rows of h [T, D] against w [V, D]: loss [T] (and lse [T], total [1]) of logits h w^T that
+    never lie in memory as a whole; with dh [T, D] / dw [V, D] also the gradients of gscale * total in the same call.
+    h and w fp32, bf16 or fp16; dh of their type, dw too or fp32 (``accumulate``: added to); target int64 [T].
+    ws: uint8 workspace of linear_cross_entropy_ws(T, D, V, h.dtype, grads, dw_f32, piece_rows) bytes.  See
+    dpc_linear_cross_entropy for ignored rows, alignment and pieces."""
+    if h.dim() != 2 or w.dim() != 2 or h.shape[1] != w.shape[1]:
+        raise ValueError('linear_cross_entropy: h must be [T, D] and w [V, D], got %s and %s' % (tuple(h.shape), tuple(w.shape)))
+    T, D, V = h.shape[0], h.shape[1], w.shape[0]
+    if h.dtype not in _TYPES:
+        raise TypeError('linear_cross_entropy: h must be fp32, bf16 or fp16, got %s' % h.dtype)
+    _chk(h, h.dtype, 'h')
+    _chk(w, h.dtype, 'w')
+    _chk(target, torch.int64, 'target')
+    for t, n, name in ((loss, T, 'loss'), (lse, T, 'lse'), (total, 1, 'total')):
+        _chk(t, torch.float32, name)
+        if t is not None and (t.numel() != n or not t.is_contiguous()):
+            raise ValueError('linear_cross_entropy: %s must be contiguous with %d entries' % (name, n))
+    if target.numel() != T or not target.is_contiguous():
+        raise ValueError('linear_cross_entropy: target must be contiguous with %d entries' % T)
+    _chk(dh, h.dtype, 'dh')
+    dw_f32 = dw is not None and dw.dtype == torch.float32
+    _chk(dw, torch.float32 if dw_f32 else h.dtype, 'dw')
+    for t, like, name in ((dh, h, 'dh'), (dw, w, 'dw')):
+        if t is not None and t.shape != like.shape:
+            raise ValueError('linear_cross_entropy: %s must be %s, got %s' % (name, tuple(like.shape), tuple(t.shape)))
+    _chk(ws, torch.uint8, 'ws')
+    if not ws.is_contiguous():
+        raise ValueError('linear_cross_entropy: ws must be contiguous')
+    lib().call('dpc_linear_cross_entropy', _p(h), _ld(h), _p(w), _ld(w), _TYPES[h.dtype], _p(target), int(ignore_index), T, D, V, _p(loss),
+               _p(lse), _p(total), _p(dh), _ld(dh) if dh is not None else 0, _p(dw), _ld(dw) if dw is not None else 0, int(dw_f32),
+               int(bool(accumulate)), float(gscale), int(bool(mean)), int(piece_rows), _p(ws), ws.numel(), _stream())
+    return loss
+
+
 # ---- optimiser over many tensors ---------------------------------------------------------------------------------
-_MULTI_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 class MultiTensor(ctypes.Structure):
@@ -726,9 +773,9 @@ def _multi_plan(lists, wd):
             if size:
                 spans.append((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), name in ('g', 'dither')))
         r.n, r.wd = size, wd[k]
-        r.g_type = _MULTI_TYPES[lists['g'][k].dtype]
-        r.p_type = _MULTI_TYPES[lists['p'][k].dtype] if lists['p'][k] is not None else 0
-        r.copy_type = _MULTI_TYPES[lists['copy'][k].dtype] if lists['copy'][k] is not None else 0
+        r.g_type = _TYPES[lists['g'][k].dtype]
+        r.p_type = _TYPES[lists['p'][k].dtype] if lists['p'][k] is not None else 0
+        r.copy_type = _TYPES[lists['copy'][k].dtype] if lists['copy'][k] is not None else 0
     if len(devs) > 1:
         raise ValueError('multi-tensor plan: tensors on %s; a plan serves one GPU' % ', '.join(sorted(str(d) for d in devs)))
     spans.sort()
@@ -754,7 +801,7 @@ def grad_plan(grads):
     """Plan over gradients alone, for grad_clip: a list of contiguous fp32 / bf16 / fp16 tensors of one GPU."""
     grads = list(grads)
     lists = {k: [None] * len(grads) for k in ('p', 'm', 'v', 'm_scale', 'v_scale', 'copy', 'dither')}
-    lists['g'] = _multi_list(grads, len(grads), list(_MULTI_TYPES), 'grads')
+    lists['g'] = _multi_list(grads, len(grads), list(_TYPES), 'grads')
     return _multi_plan(lists, [0.0] * len(grads))
 
 
@@ -765,7 +812,7 @@ def adamw_plan(params, grads, exp_avg, exp_avg_sq, wd=0.0, copies=None, m_scale=
     parameters as well; dither: int16 tensors of random bits for the 8-bit states instead of Philox draws."""
     grads = list(grads)
     n = len(grads)
-    any16 = list(_MULTI_TYPES)
+    any16 = list(_TYPES)
     eight = m_scale is not None or v_scale is not None
     st = [torch.float8_e4m3fn] if eight else [torch.float32]
     if eight and (m_scale is None or v_scale is None):

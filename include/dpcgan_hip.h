@@ -30,6 +30,11 @@ extern "C" {
 #define DPC_EINVAL (-1)
 #define DPC_EHIP (-2)
 
+/* element types of the entry points that take more than fp32 */
+#define DPC_F32 0
+#define DPC_BF16 1
+#define DPC_F16 2
+
 int dpc_version(void);
 const char* dpc_last_error(void);
 
@@ -446,11 +451,28 @@ int dpc_adam_step_slices(float* p, float* g, float* m, float* v, int64_t n, floa
 int dpc_noise_add_clamp(float* x, int64_t n, float scale, const float* noise_inj, const uint64_t* rng,
                         uint32_t site, float clamp, void* stream);
 
+/* ---- cross entropy of a Linear layer over a large vocabulary (no counterpart in the reference, whose _cond_loss_pair,
+ * dp_cgan.py:330-389, compares two-way columns: dpc_cond_loss) ------------------------------------------------------ */
+/* logits = h w^T, h [T][ldh], w [V][ldw] (D columns; dtype DPC_F32, DPC_BF16 or DPC_F16 for both), never whole in memory.
+ *   loss[r] = lse_r - logit[r][target[r]], 0 where target[r] == ignore_index, NaN for any other target outside [0, V);
+ *   lse (nullable) [T], of every row; total (nullable) [1] = sum of loss, divided by the rows not ignored if mean;
+ *   dh (nullable) [T][lddh], dw (nullable) [V][lddw] = gradients of gscale * total: of h's type, dw fp32 if dw_f32 and
+ *   then added to what dw holds if accumulate.  Rows ignored or with a bad target take no part in dw, whatever h holds
+ *   there, and their dh is 0.
+ * Sums, softmax statistics and products are in fp32; half precision rounds (softmax - onehot) once to the operands' type,
+ * fp16 with a lift of 2^14.  No atomics: the same call gives the same bits.
+ * Half precision: D a multiple of 8, every row of every matrix 16-byte aligned.  fp32: any D and row length.
+ * ws: workspace of dpc_linear_cross_entropy_ws bytes for the same arguments (-1 if they are refused), 256-byte aligned, no
+ * state between calls; calls that overlap need one each.  piece_rows: rows worked on at a time (0 = what 1 GiB holds);
+ * smaller pieces need less workspace, and read and write dw once for each. */
+int64_t dpc_linear_cross_entropy_ws(int64_t T, int D, int V, int dtype, int grads, int dw_f32, int64_t piece_rows);
+int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, const int64_t* target,
+                             int64_t ignore_index, int64_t T, int D, int V, float* loss, float* lse, float* total,
+                             void* dh, int64_t lddh, void* dw, int64_t lddw, int dw_f32, int accumulate, float gscale,
+                             int mean, int64_t piece_rows, void* ws, int64_t ws_bytes, void* stream);
+
 /* ---- optimiser over many tensors (no counterpart in the reference, whose torch.optim.Adam, dp_cgan.py:510-518, walks
  * its fp32 tensors one by one; dpc_adam_step covers that over one flat buffer) ------------------------------------ */
-#define DPC_F32 0
-#define DPC_BF16 1
-#define DPC_F16 2
 /* One tensor of n contiguous elements.  p (nullable: the gradients of grad_clip alone), g, and the two moments:
  *   32-bit states   m, v fp32 [n]: first and second moment;
  *   8-bit states    m, v e4m3 (OCP, no infinities) codes [n], m_scale, v_scale fp32 [ceil(n/128)]: code * scale of its
