@@ -34,7 +34,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-#define LCE_BK 64
+#define LCE_BK 32               // k of one tile of an operand
 #define LCE_SLAB 128            // vocabulary entries of one (max, sum) pair
 #define LCE_LOG2E 1.4426950408889634f
 #define LCE_LN2 0.6931471805599453f
@@ -61,7 +61,6 @@ struct LceArgs {
   char* P; int64_t prow;          // P, rows of one chunk column
   int M, N, K;
   int tiles_m, tiles_n;
-  const char* zero;               // 16 zero bytes
   // LOGITS
   f32x2* stat;                    // [slab][prow] (max * log2 e, sum)
   float* lt;                      // [row] logit of the target
@@ -83,28 +82,43 @@ __device__ __forceinline__ int lce_xcd(int b, int total) {
   return b < even ? (b & 7) * per + (b >> 3) : b;
 }
 
-__device__ __forceinline__ void lce_dma(const char* src, char* lds) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+// 16 bytes per lane from base + off[lane] to lds + 16 * lane.  LCE_NONE as an offset is out of range: zeros.  (Buffer
+// loads: the per-lane offset stays in its register for the whole loop and the base moves in scalar registers; and the
+// compiler keeps counting LDS reads beside them, where a global load to LDS makes it wait for every one.)
+#define LCE_NONE 0x80000000u
+__device__ __forceinline__ void lce_dma(const char* base, uint32_t off, char* lds) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)LCE_NONE, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, (int)off, 0, 0, 0);
 }
-__device__ __forceinline__ u32x2 lce_tr(const char* lds) {
+// (__restrict: a read that carries no alias information is held back by the compiler until every load to LDS has landed)
+__device__ __forceinline__ u32x2 lce_tr(const char* __restrict lds) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lds));
 }
 
-// One BM x BN tile of a product, WM x WN waves.  A tile of an operand is 64 k; it goes from memory straight into LDS, 16
-// bytes per lane, in one of two images:
-//   k-runs  (W and h of LOGITS, P of DH): [row][8 chunks of 8 k], chunk c of row r at c ^ (r & 7)  - read 16 bytes a lane
-//   m-runs  (W of DH, h of DW): [k][chunks of 8 m], chunk c of row k at c ^ 2 (k & 3)              - read transposed
-//           (P of DW): [chunk of 8 m][k], k at k ^ 4 (chunk & 1)                                     - read transposed
+// Waits until at most N of this wave's memory operations are in flight.
+template <int N>
+__device__ __forceinline__ void lce_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// One BM x BN tile of a product, WM x WN waves.  A tile of an operand is 32 k; it goes from memory straight into LDS, 16
+// bytes per lane, in one of three images:
+//   k-runs  (W and h of LOGITS, P of DH): [row][4 chunks of 8 k], chunk c of row r at c ^ (r / 2 & 3) - read 16 bytes a lane
+//   m-runs  (W of DH, h of DW): [k][chunks of 8 m], chunk c of row k at c ^ 2 (k & 3)                - read transposed
+//           (P of DW): [chunk of 8 m][k], k at k ^ 4 (chunk & 1)                                       - read transposed
 // The transposing read gives lane i of 16 the column i of a 4 x 16 block whose row r comes from lanes 4r .. 4r+3; the
-// swizzles put what 16 lanes read on 32 different banks.
-template <typename E, int MODE, int BM, int BN, int WM, int WN>
+// swizzles put what the lanes of one LDS cycle read on different banks.
+//
+// NS tiles are in flight or in use.  Iteration kt: the second half's fragments are read while the first half's products
+// run; then, once tile kt + 1 has landed for every wave and tile kt has been read by all (one barrier), tile kt + NS goes
+// on its way into the freed slot and the next tile's first fragments are read while the second half's products run.
+template <typename E, int MODE, int BM, int BN, int WM, int WN, int NS>
 __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
   using H = Half<E>;
   constexpr int NT = WM * WN * 64;
   constexpr int SM = BM / WM / 32, SN = BN / WN / 32;
-  constexpr int NA = BM * 8 / NT, NB = BN * 8 / NT;
+  constexpr int NA = BM * 4 / NT, NB = BN * 4 / NT;
+  constexpr int SLOT = (BM + BN) * 64;
   constexpr bool A_K = MODE == LCE_LOGITS, B_K = MODE != LCE_DW;
-  __shared__ __attribute__((aligned(1024))) char lds[2][(BM + BN) * 128];
+  __shared__ __attribute__((aligned(1024))) char lds[NS * SLOT];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
@@ -117,64 +131,91 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
   const int k_begin = split * g.kchunk, k_end = min(g.K, k_begin + g.kchunk);
   const int nk = (k_end - k_begin + LCE_BK - 1) / LCE_BK;
 
-  // sources of this thread's chunks of a K-tile (the tile's own offset is added as it goes)
-  const char* sa[NA];
-  const char* sb[NB];
+  // this thread's chunks of a K-tile, as offsets from the tile's first k; none where the operand ends
+  uint32_t oa[NA], ob[NB];
+  const char *pa, *pb0;
   int64_t step_a, step_b;
+  const int ck = (tid & 3) ^ ((tid >> 3) & 3);                          // k-runs: chunk of this thread
   if (A_K) {
-    const int c = (tid & 7) ^ ((tid >> 3) & 7);
 #pragma unroll
-    for (int i = 0; i < NA; ++i) sa[i] = g.A + (int64_t)min(m0 + i * (NT / 8) + (tid >> 3), g.M - 1) * g.lda + c * 16;
+    for (int i = 0; i < NA; ++i) {
+      const int r = i * (NT / 4) + (tid >> 2);
+      oa[i] = m0 + r < g.M ? (uint32_t)r * (uint32_t)g.lda + ck * 16 : LCE_NONE;
+    }
+    pa = g.A + (int64_t)m0 * g.lda;
     step_a = LCE_BK * 2;
   } else {
     constexpr int CR = BM / 8;
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
       const int k = i * (NT / CR) + tid / CR, c = (tid % CR) ^ (2 * (k & 3));
-      sa[i] = g.A + (int64_t)(k_begin + k) * g.lda + min(m0 / 8 + c, g.M / 8 - 1) * 16;
+      oa[i] = m0 + c * 8 < g.M ? (uint32_t)k * (uint32_t)g.lda + c * 16 : LCE_NONE;
     }
+    pa = g.A + (int64_t)k_begin * g.lda + (int64_t)m0 * 2;
     step_a = LCE_BK * g.lda;
   }
   if (MODE == LCE_LOGITS) {
-    const int c = (tid & 7) ^ ((tid >> 3) & 7);
 #pragma unroll
-    for (int i = 0; i < NB; ++i) sb[i] = g.B + (int64_t)min(n0 + i * (NT / 8) + (tid >> 3), g.N - 1) * g.ldb + c * 16;
+    for (int i = 0; i < NB; ++i) {
+      const int r = i * (NT / 4) + (tid >> 2);
+      ob[i] = n0 + r < g.N ? (uint32_t)r * (uint32_t)g.ldb + ck * 16 : LCE_NONE;
+    }
+    pb0 = g.B + (int64_t)n0 * g.ldb;
     step_b = LCE_BK * 2;
   } else if (MODE == LCE_DH) {
-    const int c = (tid & 7) ^ ((tid >> 3) & 7);
 #pragma unroll
-    for (int i = 0; i < NB; ++i) sb[i] = g.P + ((int64_t)(k_begin / 8 + c) * g.prow + n0 + i * (NT / 8) + (tid >> 3)) * 16;
-    step_b = 8 * g.prow * 16;
+    for (int i = 0; i < NB; ++i) ob[i] = ((uint32_t)ck * (uint32_t)g.prow + i * (NT / 4) + (tid >> 2)) * 16;
+    pb0 = g.P + ((int64_t)(k_begin / 8) * g.prow + n0) * 16;
+    step_b = LCE_BK / 8 * g.prow * 16;
   } else {
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      const int n8 = i * (NT / 64) + (tid >> 6), k = (tid & 63) ^ (4 * (n8 & 1));
-      sb[i] = g.P + ((int64_t)(n0 / 8 + n8) * g.prow + k_begin + k) * 16;
+      const int n8 = i * (NT / 32) + (tid >> 5), k = (tid & 31) ^ (4 * (n8 & 1));
+      ob[i] = ((uint32_t)n8 * (uint32_t)g.prow + k) * 16;
     }
+    pb0 = g.P + ((int64_t)(n0 / 8) * g.prow + k_begin) * 16;
     step_b = LCE_BK * 16;
   }
   const auto issue = [&](int kt, char* buf) {
     const int k0 = k_begin + kt * LCE_BK;
-    const bool tail = k0 + LCE_BK > g.K;
+    char* at = buf + wave * 1024;
+    const char *qa = pa + kt * step_a, *qb = pb0 + kt * step_b;
+    if (MODE == LCE_DW || k0 + LCE_BK <= g.K) {                         // (DW: K is whole tiles)
 #pragma unroll
-    for (int i = 0; i < NA; ++i) {
-      const char* s = sa[i] + kt * step_a;
-      if (tail) {
-        if (A_K) {
-          if (k0 / 8 + ((tid & 7) ^ ((tid >> 3) & 7)) >= g.K / 8) s = g.zero;
-        } else if (MODE == LCE_DH) {            // (rows of W past the vocabulary: any finite row, P holds 0 there)
-          const int k = k0 + i * (NT / (BM / 8)) + tid / (BM / 8);
-          s -= (int64_t)max(0, k - (g.K - 1)) * g.lda;
-        }
-      }
-      lce_dma(s, buf + (i * NT + wave * 64) * 16);
-    }
+      for (int i = 0; i < NA; ++i) lce_dma(qa, oa[i], at + i * NT * 16);
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const char* s = sb[i] + kt * step_b;
-      if (tail && MODE == LCE_LOGITS && k0 / 8 + ((tid & 7) ^ ((tid >> 3) & 7)) >= g.K / 8) s = g.zero;
-      lce_dma(s, buf + BM * 128 + (i * NT + wave * 64) * 16);
+      for (int i = 0; i < NB; ++i) lce_dma(qb, ob[i], at + BM * 64 + i * NT * 16);
+    } else {                                                            // the tile that crosses the end of K
+      const bool kend = k0 / 8 + ck >= g.K / 8;
+#pragma unroll
+      for (int i = 0; i < NA; ++i) lce_dma(qa, (A_K ? kend : k0 + i * (NT / (BM / 8)) + tid / (BM / 8) >= g.K) ? LCE_NONE : oa[i], at + i * NT * 16);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) lce_dma(qb, MODE == LCE_LOGITS && kend ? LCE_NONE : ob[i], at + BM * 64 + i * NT * 16);
     }
+  };
+
+  // lane addresses inside an image
+  const int l16 = lane & 15, G = lane >> 4;
+  const int kq = (lane & 31) * 64 + (((lane >> 5) ^ ((lane >> 1) & 3)) * 16);     // k-runs: chunk half of row; step 1 flips bit 1
+  const int mk = (8 * (G >> 1) + (l16 >> 2)) * (BM * 2) + (l16 & 1) * 8;            // m-runs [k][chunk]
+  const int mc = 2 * (G & 1) + ((l16 & 3) >> 1), mx = 2 * (l16 >> 2);
+  const int ma[2] = {mk + ((mc ^ mx) * 16), mk + (((4 + mc) ^ mx) * 16)};           // even and odd 32-row blocks
+  const int pb = ((l16 >> 1) & 1) * 64;
+  const int pq = mc * 512 + (8 * (G >> 1) + (l16 >> 2)) * 16 + (l16 & 1) * 8;       // m-runs [chunk][k]
+  const auto frag_a = [&](const char* buf, int s, int i) -> typename H::v8 {
+    const int r0 = (wm * SM + i) * 32;
+    if (A_K) return *reinterpret_cast<const typename H::v8*>(buf + r0 * 64 + (kq ^ (s * 32)));
+    const char* q = buf + s * 16 * (BM * 2) + (r0 & ~63) * 2 + ma[SM % 2 == 0 ? i & 1 : (wm * SM + i) & 1];
+    const u32x2 lo = lce_tr(q), hi = lce_tr(q + 4 * (BM * 2));
+    return __builtin_bit_cast(typename H::v8, u32x4{lo.x, lo.y, hi.x, hi.y});
+  };
+  const auto frag_b = [&](const char* buf, int s, int j) -> typename H::v8 {
+    const int r0 = (wn * SN + j) * 32;
+    buf += BM * 64;
+    if (B_K) return *reinterpret_cast<const typename H::v8*>(buf + r0 * 64 + (kq ^ (s * 32)));
+    const char* q = buf + r0 * 64 + s * 256 + pq;
+    const u32x2 lo = lce_tr(q + pb), hi = lce_tr(q + (64 - pb));
+    return __builtin_bit_cast(typename H::v8, u32x4{lo.x, lo.y, hi.x, hi.y});
   };
 
   f32x16 acc[SM][SN];
@@ -184,46 +225,68 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
     for (int j = 0; j < SN; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-
-  // lane addresses inside an image
-  const int l16 = lane & 15, G = lane >> 4;
-  const int krow = (lane & 31) * 128;                                  // k-runs: row of this lane
-  const int mk = (8 * (G >> 1) + (l16 >> 2)) * (BM * 2);                // m-runs [k][chunk]: k of this lane
-  const int mc = 2 * (G & 1) + ((l16 & 3) >> 1), mx = 2 * (l16 >> 2), mh = (l16 & 1) * 8;
-  const int pb = ((l16 >> 1) & 1) * 4;                                  // m-runs [chunk][k]
-  const auto frag_a = [&](const char* buf, int s, int i) -> typename H::v8 {
-    const int r0 = (wm * SM + i) * 32;
-    if (A_K) return *reinterpret_cast<const typename H::v8*>(buf + r0 * 128 + krow + (((2 * s + (lane >> 5)) ^ (lane & 7)) * 16));
-    const char* q = buf + mk + s * 16 * (BM * 2) + (((r0 / 8 + mc) ^ mx) * 16) + mh;
-    const u32x2 lo = lce_tr(q), hi = lce_tr(q + 4 * (BM * 2));
-    return __builtin_bit_cast(typename H::v8, u32x4{lo.x, lo.y, hi.x, hi.y});
+  typename H::v8 a0[SM], b0[SN], a1[SM], b1[SN];
+  const auto read = [&](const char* buf, int s, typename H::v8* a, typename H::v8* b) {
+#pragma unroll
+    for (int i = 0; i < SM; ++i) a[i] = frag_a(buf, s, i);
+#pragma unroll
+    for (int j = 0; j < SN; ++j) b[j] = frag_b(buf, s, j);
   };
-  const auto frag_b = [&](const char* buf, int s, int j) -> typename H::v8 {
-    const int r0 = (wn * SN + j) * 32;
-    if (B_K) return *reinterpret_cast<const typename H::v8*>(buf + r0 * 128 + krow + (((2 * s + (lane >> 5)) ^ (lane & 7)) * 16));
-    const char* q = buf + (r0 / 8 + mc) * 1024 + (s * 16 + 8 * (G >> 1) + (l16 >> 2)) * 16 + mh;
-    const u32x2 lo = lce_tr(q + pb * 16), hi = lce_tr(q + (4 - pb) * 16);
-    return __builtin_bit_cast(typename H::v8, u32x4{lo.x, lo.y, hi.x, hi.y});
+  const auto multiply = [&](const typename H::v8* a, const typename H::v8* b) {
+#pragma unroll
+    for (int i = 0; i < SM; ++i)
+#pragma unroll
+      for (int j = 0; j < SN; ++j) acc[i][j] = H::mfma(a[i], b[j], acc[i][j]);
+  };
+  // The next tile has landed for every wave, with at most `ahead` tiles behind it on their way; this one has been read.
+  const auto meet = [&](int ahead) {
+    constexpr int L = NA + NB;
+    if (ahead >= NS - 2) lce_wait_vm<(NS - 2) * L>();
+    else if (NS > 3 && ahead == NS - 3) lce_wait_vm<(NS - 3) * L>();
+    else lce_wait_vm<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
   };
 
-  if (nk > 0) issue(0, lds[0]);
-  for (int kt = 0; kt < nk; ++kt) {
-    const char* buf = lds[kt & 1];
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                    // this wave's share of tile kt has landed ...
-    __syncthreads();                                                    // ... every wave's; and tile kt - 1 has been read
-    if (kt + 1 < nk) issue(kt + 1, lds[(kt + 1) & 1]);
+  if (nk > 0) {
 #pragma unroll
-    for (int s = 0; s < LCE_BK / 16; ++s) {
-      typename H::v8 a[SM], b[SN];
-#pragma unroll
-      for (int i = 0; i < SM; ++i) a[i] = frag_a(buf, s, i);
-#pragma unroll
-      for (int j = 0; j < SN; ++j) b[j] = frag_b(buf + BM * 128, s, j);
-#pragma unroll
-      for (int i = 0; i < SM; ++i)
-#pragma unroll
-        for (int j = 0; j < SN; ++j) acc[i][j] = H::mfma(a[i], b[j], acc[i][j]);
+    for (int k = 0; k < NS - 1; ++k)
+      if (k < nk) issue(k, lds + k * SLOT);
+    meet(min(NS - 2, nk - 1));
+    if (NS - 1 < nk) issue(NS - 1, lds + (NS - 1) * SLOT);
+    read(lds, 0, a0, b0);
+    int cur = 0, kt = 0;
+    for (; kt + NS < nk; ++kt) {
+      const int nxt = cur + 1 == NS ? 0 : cur + 1;
+      read(lds + cur * SLOT, 1, a1, b1);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(a0, b0);
+      __builtin_amdgcn_sched_barrier(0);
+      meet(NS - 2);
+      issue(kt + NS, lds + cur * SLOT);
+      read(lds + nxt * SLOT, 0, a0, b0);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(a1, b1);
+      __builtin_amdgcn_sched_barrier(0);
+      cur = nxt;
     }
+    for (; kt + 1 < nk; ++kt) {                                         // nothing more to load
+      const int nxt = cur + 1 == NS ? 0 : cur + 1;
+      read(lds + cur * SLOT, 1, a1, b1);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(a0, b0);
+      __builtin_amdgcn_sched_barrier(0);
+      meet(nk - 2 - kt);
+      read(lds + nxt * SLOT, 0, a0, b0);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(a1, b1);
+      __builtin_amdgcn_sched_barrier(0);
+      cur = nxt;
+    }
+    read(lds + cur * SLOT, 1, a1, b1);
+    multiply(a0, b0);
+    multiply(a1, b1);
   }
 
   // C layout of a 32 x 32 block: n = lane & 31, m = (e & 3) + 8 (e >> 2) + 4 (lane >> 5)
@@ -318,7 +381,7 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
 }
 
 // ---- the passes between the products --------------------------------------------------------------------------------
-// alpha = gscale / (rows that count, or 1) / lift; zero: 16 zero bytes; count as a float for the mean of the losses
+// head = {alpha = gscale / (rows that count, or 1) / lift, that count, 1}
 __global__ __launch_bounds__(1024) void lce_begin_kernel(const int64_t* target, int64_t T, int64_t ignore, int V, int mean, float gscale,
                                                          float lift, float* head) {
   __shared__ int red[16];
@@ -332,7 +395,6 @@ __global__ __launch_bounds__(1024) void lce_begin_kernel(const int64_t* target, 
     head[1] = n;
     head[2] = 1.f;
   }
-  if (threadIdx.x < 4) head[4 + threadIdx.x] = 0.f;
 }
 
 // Per row: lse from the slabs' (max, sum) pairs.  32 rows x 8 lanes of slabs per block.
@@ -521,7 +583,7 @@ static LceLayout lce_layout(int64_t T, int D, int V, int dtype, bool grads, bool
   if (l.rows < 1) l.rows = 1;
   l.pieces = (int)dpc_cdiv(T < 1 ? 1 : T, l.rows);
   l.prow = lce_up(l.rows, 256);
-  int64_t at = 256;                                                    // head: alpha, count, 16 zero bytes
+  int64_t at = 256;                                                    // head
   const auto take = [&](int64_t bytes) { const int64_t o = at; at += lce_up(bytes, 256); return o; };
   l.lt = take(l.prow * 4);
   l.glse = take(l.prow * 4);
@@ -579,7 +641,7 @@ static void lce_launch(LceArgs& g, hipStream_t st) {
   g.tiles_n = (int)dpc_cdiv(g.N, 256);
   if (g.splits < 1) g.splits = 1;
   g.kchunk = (int)lce_up(dpc_cdiv(g.K, g.splits), LCE_BK);
-  hipLaunchKernelGGL((lce_product_kernel<E, MODE, 256, 256, 2, 4>), dim3(g.tiles_m * g.tiles_n * g.splits), dim3(512), 0, st, g);
+  hipLaunchKernelGGL((lce_product_kernel<E, MODE, 256, 256, 2, 4, 4>), dim3(g.tiles_m * g.tiles_n * g.splits), dim3(512), 0, st, g);
 }
 
 struct LceCall {
@@ -602,7 +664,7 @@ static int lce_half(const LceCall& c, const LceLayout& l, hipStream_t st) {
     const char* h = c.h + r0 * c.ldh * 2;
     LceArgs g;
     memset(&g, 0, sizeof(g));
-    g.P = c.ws + l.P; g.prow = l.prow; g.zero = (const char*)(head + 4); g.alpha = head; g.target = c.target + r0;
+    g.P = c.ws + l.P; g.prow = l.prow; g.alpha = head; g.target = c.target + r0;
     g.stat = (f32x2*)(c.ws + l.stat); g.lt = (float*)(c.ws + l.lt); g.grads = grads;
     g.A = c.w; g.lda = c.ldw * 2; g.B = h; g.ldb = c.ldh * 2;
     g.M = c.V; g.N = rows; g.K = c.D;
@@ -723,12 +785,14 @@ extern "C" int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* 
   if (!f32) {
     const uintptr_t al = (uintptr_t)h | (uintptr_t)w | (uintptr_t)dh | (uintptr_t)dw | (uintptr_t)(ldh * 2) | (uintptr_t)(ldw * 2);
     DPC_CHECK_ARG((al & 15) == 0, "linear_cross_entropy: half-precision rows must be 16-byte aligned");
+    DPC_CHECK_ARG(ldh < (1 << 21) && ldw < (1 << 21), "linear_cross_entropy: rows are too long");     // (256 rows within 32-bit offsets)
     DPC_CHECK_ARG((!dh || lddh % 8 == 0) && (!dw || lddw % (dw_f32 ? 4 : 8) == 0), "linear_cross_entropy: gradient rows must be 16-byte aligned");
   }
   DPC_CHECK_ARG(((uintptr_t)ws & 255) == 0, "linear_cross_entropy: the workspace must be 256-byte aligned");
   const bool grads = dh || dw;
   if (piece_rows <= 0) piece_rows = lce_rows_default(V, dtype, grads);
   DPC_CHECK_ARG(dpc_cdiv(V, 256) * dpc_cdiv(piece_rows < T ? piece_rows : T, 256) * 32 < (1ll << 31), "linear_cross_entropy: the piece is too large");
+  DPC_CHECK_ARG(f32 || !grads || piece_rows <= (1 << 21) || T <= (1 << 21), "linear_cross_entropy: the piece is too large");
   const LceLayout l = lce_layout(T, D, V, dtype, grads, !f32 && !dw_f32, piece_rows);
   DPC_CHECK_ARG(ws_bytes >= l.bytes, "linear_cross_entropy: the workspace is smaller than dpc_linear_cross_entropy_ws says");
   hipStream_t st = (hipStream_t)stream;
