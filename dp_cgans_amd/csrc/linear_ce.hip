@@ -176,22 +176,28 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
     pb0 = g.P + ((int64_t)(n0 / 8) * g.prow + k_begin) * 16;
     step_b = LCE_BK * 16;
   }
-  const auto issue = [&](int kt, char* buf) {
-    const int k0 = k_begin + kt * LCE_BK;
-    char* at = buf + wave * 1024;
-    const char *qa = pa + kt * step_a, *qb = pb0 + kt * step_b;
-    if (MODE == LCE_DW || k0 + LCE_BK <= g.K) {                         // (DW: K is whole tiles)
+  // Tiles are loaded in order; before the one that crosses the end of K, what lies past it becomes "none" (DW: K is whole tiles).
+  const int kt_cut = MODE != LCE_DW && k_begin + nk * LCE_BK > g.K ? nk - 1 : -1;
+  const auto cut = [&]() {
+    const int k0 = k_begin + kt_cut * LCE_BK;
+    const bool kend = k0 / 8 + ck >= g.K / 8;
 #pragma unroll
-      for (int i = 0; i < NA; ++i) lce_dma(qa, oa[i], at + i * NT * 16);
+    for (int i = 0; i < NA; ++i)
+      if (A_K ? kend : k0 + i * (NT / (BM / 8)) + tid / (BM / 8) >= g.K) oa[i] = LCE_NONE;
+    if (MODE == LCE_LOGITS && kend) {
 #pragma unroll
-      for (int i = 0; i < NB; ++i) lce_dma(qb, ob[i], at + BM * 64 + i * NT * 16);
-    } else {                                                            // the tile that crosses the end of K
-      const bool kend = k0 / 8 + ck >= g.K / 8;
-#pragma unroll
-      for (int i = 0; i < NA; ++i) lce_dma(qa, (A_K ? kend : k0 + i * (NT / (BM / 8)) + tid / (BM / 8) >= g.K) ? LCE_NONE : oa[i], at + i * NT * 16);
-#pragma unroll
-      for (int i = 0; i < NB; ++i) lce_dma(qb, MODE == LCE_LOGITS && kend ? LCE_NONE : ob[i], at + BM * 64 + i * NT * 16);
+      for (int i = 0; i < NB; ++i) ob[i] = LCE_NONE;
     }
+  };
+  const auto issue_one = [&](int kt, char* buf, int l) {                // load l (of NA + NB) of tile kt
+    char* at = buf + wave * 1024;
+    if (l < NA) lce_dma(pa + kt * step_a, oa[l < NA ? l : 0], at + l * NT * 16);
+    else lce_dma(pb0 + kt * step_b, ob[l < NA ? 0 : l - NA], at + BM * 64 + (l - NA) * NT * 16);
+  };
+  const auto issue = [&](int kt, char* buf) {
+    if (kt == kt_cut) cut();
+#pragma unroll
+    for (int l = 0; l < NA + NB; ++l) issue_one(kt, buf, l);
   };
 
   // lane addresses inside an image
@@ -238,6 +244,30 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
 #pragma unroll
       for (int j = 0; j < SN; ++j) acc[i][j] = H::mfma(a[i], b[j], acc[i][j]);
   };
+  // One half-tile's products with the next half's reads, and a tile's loads, between them: a wave that waits for the
+  // matrix unit has them behind it.  In this order, pinned: products run for 32 cycles each, and what stands before the
+  // first one after a barrier holds up every wave at once.
+  const auto half_tile = [&](const typename H::v8* a, const typename H::v8* b, const char* buf, int s, typename H::v8* an, typename H::v8* bn, int load,
+                             char* into) {
+    constexpr int READS = SM + SN, SLOTS = SM * SN;
+#pragma unroll
+    for (int i = 0; i < SM; ++i)
+#pragma unroll
+      for (int j = 0; j < SN; ++j) {
+        acc[i][j] = H::mfma(a[i], b[j], acc[i][j]);
+        const int p = i * SN + j;
+#pragma unroll
+        for (int r = p * READS / (SLOTS - 2); r < (p + 1) * READS / (SLOTS - 2) && r < READS; ++r) {
+          if (r < SN) bn[r] = frag_b(buf, s, r);
+          else an[r - SN] = frag_a(buf, s, r - SN);
+        }
+        if (load >= 0) {
+#pragma unroll
+          for (int l = p * (NA + NB) / SLOTS; l < (p + 1) * (NA + NB) / SLOTS; ++l) issue_one(load, into, l);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  };
   // The next tile has landed for every wave, with at most `ahead` tiles behind it on their way; this one has been read.
   const auto meet = [&](int ahead) {
     constexpr int L = NA + NB;
@@ -259,29 +289,17 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
     int cur = 0, kt = 0;
     for (; kt + NS < nk; ++kt) {
       const int nxt = cur + 1 == NS ? 0 : cur + 1;
-      read(lds + cur * SLOT, 1, a1, b1);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(a0, b0);
-      __builtin_amdgcn_sched_barrier(0);
+      half_tile(a0, b0, lds + cur * SLOT, 1, a1, b1, -1, nullptr);
       meet(NS - 2);
-      issue(kt + NS, lds + cur * SLOT);
-      read(lds + nxt * SLOT, 0, a0, b0);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(a1, b1);
-      __builtin_amdgcn_sched_barrier(0);
+      if (kt + NS == kt_cut) cut();
+      half_tile(a1, b1, lds + nxt * SLOT, 0, a0, b0, kt + NS, lds + cur * SLOT);
       cur = nxt;
     }
     for (; kt + 1 < nk; ++kt) {                                         // nothing more to load
       const int nxt = cur + 1 == NS ? 0 : cur + 1;
-      read(lds + cur * SLOT, 1, a1, b1);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(a0, b0);
-      __builtin_amdgcn_sched_barrier(0);
+      half_tile(a0, b0, lds + cur * SLOT, 1, a1, b1, -1, nullptr);
       meet(nk - 2 - kt);
-      read(lds + nxt * SLOT, 0, a0, b0);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(a1, b1);
-      __builtin_amdgcn_sched_barrier(0);
+      half_tile(a1, b1, lds + nxt * SLOT, 0, a0, b0, -1, nullptr);
       cur = nxt;
     }
     read(lds + cur * SLOT, 1, a1, b1);
@@ -360,22 +378,32 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
       const int n = nw + j * 32;
       if (n >= g.N) continue;
 #pragma unroll
-      for (int i = 0; i < SM; ++i)
+      for (int i = 0; i < SM; ++i) {
+        const int m = mw + i * 32 + 4 * half;
+        const int64_t o = (int64_t)n * g.ldc + m + split * g.slab;
+        f32x4 v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[q][e] = alpha * acc[i][j][4 * q + e];
+        if (g.add) {
+          f32x4 x[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (m + 8 * q < g.M) x[q] = *reinterpret_cast<const f32x4*>(g.add + (int64_t)n * g.ldadd + m + 8 * q);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] += x[q];
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int m = mw + i * 32 + 8 * q + 4 * half;
-          if (m >= g.M) continue;
-          f32x4 v;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = alpha * acc[i][j][4 * q + e];
-          if (g.add) v += *reinterpret_cast<const f32x4*>(g.add + (int64_t)n * g.ldadd + m);
-          const int64_t o = (int64_t)n * g.ldc + m + split * g.slab;
-          if (g.c_f32) *reinterpret_cast<f32x4*>((float*)g.C + o) = v;
+          if (m + 8 * q >= g.M) continue;
+          if (g.c_f32) *reinterpret_cast<f32x4*>((float*)g.C + o + 8 * q) = v[q];
           else {
             typedef E e4 __attribute__((ext_vector_type(4)));
-            *reinterpret_cast<e4*>((E*)g.C + o) = __builtin_convertvector(v, e4);
+            *reinterpret_cast<e4*>((E*)g.C + o + 8 * q) = __builtin_convertvector(v[q], e4);
           }
         }
+      }
     }
   }
 }
@@ -635,13 +663,28 @@ extern "C" int64_t dpc_linear_cross_entropy_ws(int64_t T, int D, int V, int dtyp
   return lce_layout(T, D, V, dtype, grads != 0, dtype != DPC_F32 && !dw_f32, piece_rows).bytes;
 }
 
+#ifndef LCE_CFG_0
+#define LCE_CFG_0 256, 256, 2, 4, 4
+#endif
+#ifndef LCE_CFG_1
+#define LCE_CFG_1 256, 256, 2, 4, 4
+#endif
+#ifndef LCE_CFG_2
+#define LCE_CFG_2 256, 256, 2, 4, 4
+#endif
+template <typename E, int MODE, int BM, int BN, int WM, int WN, int NS>
+static void lce_launch_tile(LceArgs& g, hipStream_t st) {
+  g.tiles_m = (int)dpc_cdiv(g.M, BM);
+  g.tiles_n = (int)dpc_cdiv(g.N, BN);
+  if (g.splits < 1) g.splits = 1;
+  g.kchunk = (int)lce_up(dpc_cdiv(g.K, g.splits), 64);
+  hipLaunchKernelGGL((lce_product_kernel<E, MODE, BM, BN, WM, WN, NS>), dim3(g.tiles_m * g.tiles_n * g.splits), dim3(WM * WN * 64), 0, st, g);
+}
 template <typename E, int MODE>
 static void lce_launch(LceArgs& g, hipStream_t st) {
-  g.tiles_m = (int)dpc_cdiv(g.M, 256);
-  g.tiles_n = (int)dpc_cdiv(g.N, 256);
-  if (g.splits < 1) g.splits = 1;
-  g.kchunk = (int)lce_up(dpc_cdiv(g.K, g.splits), LCE_BK);
-  hipLaunchKernelGGL((lce_product_kernel<E, MODE, 256, 256, 2, 4, 4>), dim3(g.tiles_m * g.tiles_n * g.splits), dim3(512), 0, st, g);
+  if constexpr (MODE == LCE_LOGITS) lce_launch_tile<E, MODE, LCE_CFG_0>(g, st);
+  else if constexpr (MODE == LCE_DH) lce_launch_tile<E, MODE, LCE_CFG_1>(g, st);
+  else lce_launch_tile<E, MODE, LCE_CFG_2>(g, st);
 }
 
 struct LceCall {
