@@ -23,8 +23,8 @@
 #include "../../include/dpcgan_hip.h"
 #include <math.h>
 #include <string.h>
+#include <type_traits>
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -41,16 +41,18 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 enum { LCE_LOGITS = 0, LCE_DH = 1, LCE_DW = 2 };
 
-// 16-bit element types: the matrix instruction, and the conversion of 8 results
+// 16-bit element types and their matrix instruction.  16 x 16 x 32 and not 32 x 32 x 16: the chip lowers its clock under
+// these products, and with half the accumulator traffic per multiplication the smaller block keeps a higher one (nothing
+// but matrix instructions on random bf16: 1946 against 1707 TFLOP/s; on zeros both reach 2450).
 template <typename E> struct Half;
 template <> struct Half<__bf16> {
   typedef bf16x8 v8;
-  static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ f32x4 mfma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
   static constexpr float kUp = 1.f;         // d as it is: bf16 has fp32's range
 };
 template <> struct Half<_Float16> {
   typedef f16x8 v8;
-  static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ f32x4 mfma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
   static constexpr float kUp = 16384.f;     // |d| <= 1 lifted by 2^14: probabilities stay normal numbers down to 2^-28
 };
 
@@ -95,6 +97,17 @@ __device__ __forceinline__ u32x2 lce_tr(const char* __restrict lds) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lds));
 }
 
+// Two 16 x 16 blocks' results, 4 consecutive m per lane, as 8 consecutive m per lane: lanes of group G (of 16) come to hold
+// chunk G / 2 of block G & 1.
+__device__ __forceinline__ u32x4 lce_pair(u32x2 x, u32x2 y) {
+  const auto lo = __builtin_amdgcn_permlane16_swap(x.x, y.x, false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(x.y, y.y, false, false);
+  return u32x4{lo[0], hi[0], lo[1], hi[1]};
+}
+
+typedef std::integral_constant<bool, true> Yes;
+typedef std::integral_constant<bool, false> No;
+
 // Waits until at most N of this wave's memory operations are in flight.
 template <int N>
 __device__ __forceinline__ void lce_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
@@ -107,14 +120,14 @@ __device__ __forceinline__ void lce_wait_vm() { asm volatile("s_waitcnt vmcnt(%0
 // The transposing read gives lane i of 16 the column i of a 4 x 16 block whose row r comes from lanes 4r .. 4r+3; the
 // swizzles put what the lanes of one LDS cycle read on different banks.
 //
-// NS tiles are in flight or in use.  Iteration kt: the second half's fragments are read while the first half's products
-// run; then, once tile kt + 1 has landed for every wave and tile kt has been read by all (one barrier), tile kt + NS goes
-// on its way into the freed slot and the next tile's first fragments are read while the second half's products run.
+// NS tiles are in flight or in use.  Iteration kt: while the products of the wave's upper rows run, its lower rows' fragments
+// are read; then, once tile kt + 1 has landed for every wave and tile kt has been read by all (one barrier), tile kt + NS
+// goes on its way into the freed slot and the next tile's first fragments are read while the lower rows' products run.
 template <typename E, int MODE, int BM, int BN, int WM, int WN, int NS>
 __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
   using H = Half<E>;
   constexpr int NT = WM * WN * 64;
-  constexpr int SM = BM / WM / 32, SN = BN / WN / 32;
+  constexpr int SM = BM / WM / 16, SN = BN / WN / 16, SH = SM / 2;
   constexpr int NA = BM * 4 / NT, NB = BN * 4 / NT;
   constexpr int SLOT = (BM + BN) * 64;
   constexpr bool A_K = MODE == LCE_LOGITS, B_K = MODE != LCE_DW;
@@ -202,71 +215,55 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
 
   // lane addresses inside an image
   const int l16 = lane & 15, G = lane >> 4;
-  const int kq = (lane & 31) * 64 + (((lane >> 5) ^ ((lane >> 1) & 3)) * 16);     // k-runs: chunk half of row; step 1 flips bit 1
-  const int mk = (8 * (G >> 1) + (l16 >> 2)) * (BM * 2) + (l16 & 1) * 8;            // m-runs [k][chunk]
-  const int mc = 2 * (G & 1) + ((l16 & 3) >> 1), mx = 2 * (l16 >> 2);
-  const int ma[2] = {mk + ((mc ^ mx) * 16), mk + (((4 + mc) ^ mx) * 16)};           // even and odd 32-row blocks
+  const int kq = l16 * 64 + ((G ^ ((l16 >> 1) & 3)) * 16);                          // k-runs: row and chunk of this lane
+  const int mk = (8 * G + (l16 >> 2)) * (BM * 2) + (l16 & 1) * 8;                   // m-runs [k][chunk]
+  const int mc = (l16 & 3) >> 1, mx = 2 * (l16 >> 2);
+  const int ma[4] = {mk + ((mc ^ mx) * 16), mk + (((2 + mc) ^ mx) * 16), mk + (((4 + mc) ^ mx) * 16), mk + (((6 + mc) ^ mx) * 16)};
   const int pb = ((l16 >> 1) & 1) * 64;
-  const int pq = mc * 512 + (8 * (G >> 1) + (l16 >> 2)) * 16 + (l16 & 1) * 8;       // m-runs [chunk][k]
-  const auto frag_a = [&](const char* buf, int s, int i) -> typename H::v8 {
-    const int r0 = (wm * SM + i) * 32;
-    if (A_K) return *reinterpret_cast<const typename H::v8*>(buf + r0 * 64 + (kq ^ (s * 32)));
-    const char* q = buf + s * 16 * (BM * 2) + (r0 & ~63) * 2 + ma[SM % 2 == 0 ? i & 1 : (wm * SM + i) & 1];
+  const int pq = mc * 512 + (8 * G + (l16 >> 2)) * 16 + (l16 & 1) * 8;              // m-runs [chunk][k]
+  static_assert(SM % 4 == 0 && SN % 2 == 0, "a wave's rows in whole 64s, its columns in whole 32s");
+  const auto frag_a = [&](const char* buf, int i) -> typename H::v8 {
+    if (A_K) return *reinterpret_cast<const typename H::v8*>(buf + (wm * SM + i) * 1024 + kq);
+    const char* q = buf + (wm * SM + (i & ~3)) * 32 + ma[i & 3];
     const u32x2 lo = lce_tr(q), hi = lce_tr(q + 4 * (BM * 2));
     return __builtin_bit_cast(typename H::v8, u32x4{lo.x, lo.y, hi.x, hi.y});
   };
-  const auto frag_b = [&](const char* buf, int s, int j) -> typename H::v8 {
-    const int r0 = (wn * SN + j) * 32;
-    buf += BM * 64;
-    if (B_K) return *reinterpret_cast<const typename H::v8*>(buf + r0 * 64 + (kq ^ (s * 32)));
-    const char* q = buf + r0 * 64 + s * 256 + pq;
-    const u32x2 lo = lce_tr(q + pb), hi = lce_tr(q + (64 - pb));
+  const auto frag_b = [&](const char* buf, int j) -> typename H::v8 {
+    const char* q = buf + BM * 64 + (wn * SN + j) * 1024;
+    if (B_K) return *reinterpret_cast<const typename H::v8*>(q + kq);
+    const u32x2 lo = lce_tr(q + pq + pb), hi = lce_tr(q + pq + (64 - pb));
     return __builtin_bit_cast(typename H::v8, u32x4{lo.x, lo.y, hi.x, hi.y});
   };
 
-  f32x16 acc[SM][SN];
+  f32x4 acc[SM][SN];
 #pragma unroll
   for (int i = 0; i < SM; ++i)
 #pragma unroll
-    for (int j = 0; j < SN; ++j)
+    for (int j = 0; j < SN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  typename H::v8 a0[SH], a1[SH], b[SN];
+  // One half of a tile's products with the reads of the next half, and a tile's loads, between them: a wave that waits for
+  // the matrix unit has them behind it.  In this order, pinned: what stands before the first product after a barrier holds
+  // up every wave at once.  Column by column, so that b[j] is free for the next tile's once its products have been issued.
+  const auto half_tile = [&](auto lower, auto more, auto load, const char* buf, int kt, char* into) {
+    constexpr bool LOW = decltype(lower)::value, MORE = decltype(more)::value, LOAD = decltype(load)::value;
+    constexpr int SLOTS = SH * SN, L = NA + NB;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  typename H::v8 a0[SM], b0[SN], a1[SM], b1[SN];
-  const auto read = [&](const char* buf, int s, typename H::v8* a, typename H::v8* b) {
+    for (int j = 0; j < SN; ++j) {
 #pragma unroll
-    for (int i = 0; i < SM; ++i) a[i] = frag_a(buf, s, i);
+      for (int i = 0; i < SH; ++i) {
+        acc[(LOW ? SH : 0) + i][j] = H::mfma((LOW ? a1 : a0)[i], b[j], acc[(LOW ? SH : 0) + i][j]);
+        const int p = j * SH + i;
+        if (!LOW && p < SH) a1[p < SH ? p : 0] = frag_a(buf, SH + p);
+        if (LOW && MORE && (p & 1) == 0 && p / 2 < SH) a0[p / 2 < SH ? p / 2 : 0] = frag_a(buf, p / 2);
+        if (LOW && MORE && i == SH - 1) b[j] = frag_b(buf, j);
+        if (LOAD) {
 #pragma unroll
-    for (int j = 0; j < SN; ++j) b[j] = frag_b(buf, s, j);
-  };
-  const auto multiply = [&](const typename H::v8* a, const typename H::v8* b) {
-#pragma unroll
-    for (int i = 0; i < SM; ++i)
-#pragma unroll
-      for (int j = 0; j < SN; ++j) acc[i][j] = H::mfma(a[i], b[j], acc[i][j]);
-  };
-  // One half-tile's products with the next half's reads, and a tile's loads, between them: a wave that waits for the
-  // matrix unit has them behind it.  In this order, pinned: products run for 32 cycles each, and what stands before the
-  // first one after a barrier holds up every wave at once.
-  const auto half_tile = [&](const typename H::v8* a, const typename H::v8* b, const char* buf, int s, typename H::v8* an, typename H::v8* bn, int load,
-                             char* into) {
-    constexpr int READS = SM + SN, SLOTS = SM * SN;
-#pragma unroll
-    for (int i = 0; i < SM; ++i)
-#pragma unroll
-      for (int j = 0; j < SN; ++j) {
-        acc[i][j] = H::mfma(a[i], b[j], acc[i][j]);
-        const int p = i * SN + j;
-#pragma unroll
-        for (int r = p * READS / (SLOTS - 2); r < (p + 1) * READS / (SLOTS - 2) && r < READS; ++r) {
-          if (r < SN) bn[r] = frag_b(buf, s, r);
-          else an[r - SN] = frag_a(buf, s, r - SN);
-        }
-        if (load >= 0) {
-#pragma unroll
-          for (int l = p * (NA + NB) / SLOTS; l < (p + 1) * (NA + NB) / SLOTS; ++l) issue_one(load, into, l);
+          for (int l = 0; l < L; ++l)
+            if (l * SLOTS / L + 1 == p) issue_one(kt, into, l);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+    }
   };
   // The next tile has landed for every wave, with at most `ahead` tiles behind it on their way; this one has been read.
   const auto meet = [&](int ahead) {
@@ -285,123 +282,114 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
       if (k < nk) issue(k, lds + k * SLOT);
     meet(min(NS - 2, nk - 1));
     if (NS - 1 < nk) issue(NS - 1, lds + (NS - 1) * SLOT);
-    read(lds, 0, a0, b0);
+#pragma unroll
+    for (int j = 0; j < SN; ++j) b[j] = frag_b(lds, j);
+#pragma unroll
+    for (int i = 0; i < SH; ++i) a0[i] = frag_a(lds, i);
     int cur = 0, kt = 0;
-    for (; kt + NS < nk; ++kt) {
+    const auto tile = [&](auto more, auto load, int ahead) {
       const int nxt = cur + 1 == NS ? 0 : cur + 1;
-      half_tile(a0, b0, lds + cur * SLOT, 1, a1, b1, -1, nullptr);
-      meet(NS - 2);
-      if (kt + NS == kt_cut) cut();
-      half_tile(a1, b1, lds + nxt * SLOT, 0, a0, b0, kt + NS, lds + cur * SLOT);
+      half_tile(No(), No(), No(), lds + cur * SLOT, 0, nullptr);
+      if (decltype(more)::value) meet(ahead);
+      if (decltype(load)::value && kt + NS == kt_cut) cut();
+      half_tile(Yes(), more, load, lds + nxt * SLOT, kt + NS, lds + cur * SLOT);
       cur = nxt;
-    }
-    for (; kt + 1 < nk; ++kt) {                                         // nothing more to load
-      const int nxt = cur + 1 == NS ? 0 : cur + 1;
-      half_tile(a0, b0, lds + cur * SLOT, 1, a1, b1, -1, nullptr);
-      meet(nk - 2 - kt);
-      half_tile(a1, b1, lds + nxt * SLOT, 0, a0, b0, -1, nullptr);
-      cur = nxt;
-    }
-    read(lds + cur * SLOT, 1, a1, b1);
-    multiply(a0, b0);
-    multiply(a1, b1);
+    };
+    for (; kt + NS < nk; ++kt) tile(Yes(), Yes(), NS - 2);
+    for (; kt + 1 < nk; ++kt) tile(Yes(), No(), nk - 2 - kt);           // nothing more to load
+    tile(No(), No(), 0);
   }
 
-  // C layout of a 32 x 32 block: n = lane & 31, m = (e & 3) + 8 (e >> 2) + 4 (lane >> 5)
-  const int half = lane >> 5;
-  const int mw = m0 + wm * SM * 32, nw = n0 + wn * SN * 32 + (lane & 31);
+  // C layout of a 16 x 16 block: n = lane & 15, m = 4 (lane >> 4) + e
+  const int mw = m0 + wm * SM * 16, nw = n0 + wn * SN * 16 + l16;
   if (MODE == LCE_LOGITS) {
-    if (mw + SM * 32 > g.M) {
+    if (mw + SM * 16 > g.M) {
 #pragma unroll
       for (int i = 0; i < SM; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (mw + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * half >= g.M)
+        for (int e = 0; e < 4; ++e)
+          if (mw + i * 16 + 4 * G + e >= g.M)
 #pragma unroll
             for (int j = 0; j < SN; ++j) acc[i][j][e] = -INFINITY;
     }
 #pragma unroll
     for (int j = 0; j < SN; ++j) {
-      const int n = nw + j * 32;
-      const bool row = n < g.N;
-      const int64_t t = row ? g.target[n] : -1;
-      if (__any(t >= mw && t < mw + SM * 32)) {
-        const int at = (int)(t - mw);
+      const int n = nw + j * 16;
+      const int64_t t = n < g.N ? g.target[n] : -1;
+      if (__any(t >= mw && t < mw + SM * 16)) {
+        const int at = t >= mw && t < mw + SM * 16 ? (int)(t - mw) : -1;
 #pragma unroll
         for (int i = 0; i < SM; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (t >= mw && at == i * 32 + (e & 3) + 8 * (e >> 2) + 4 * half) g.lt[n] = acc[i][j][e];
+          for (int e = 0; e < 4; ++e)
+            if (at == i * 16 + 4 * G + e) g.lt[n] = acc[i][j][e];
       }
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < SM; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, acc[i][j][e]);
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64)) * LCE_LOG2E;
       const float ref = top == -INFINITY ? 0.f : top;                  // (all -inf: e^(l - 0) = 0, not NaN)
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < SM; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < 4; ++e) {
           acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], LCE_LOG2E, -ref));
           sum += acc[i][j][e];
         }
+      sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
-      if (half == 0 && mw < g.M) g.stat[(int64_t)(mw / LCE_SLAB) * g.prow + n] = f32x2{top, sum};
+      if (G == 0 && mw < g.M) g.stat[(int64_t)(mw / LCE_SLAB) * g.prow + n] = f32x2{top, sum};
       if (g.grads) {
 #pragma unroll
-        for (int i = 0; i < SM; ++i)
+        for (int i = 0; i < SM; i += 2) {
+          u32x2 x[2];
 #pragma unroll
-          for (int q = 0; q < 4; q += 2) {
-            u32x2 x[2];
+          for (int w = 0; w < 2; ++w)
 #pragma unroll
-            for (int w = 0; w < 2; ++w)
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const f16x2 v = {(_Float16)acc[i][j][4 * (q + w) + 2 * c], (_Float16)acc[i][j][4 * (q + w) + 2 * c + 1]};
-                x[w][c] = __builtin_bit_cast(uint32_t, v);
-              }
-            // lanes below 32 come to hold chunk q of their row, the others chunk q + 1 of the same rows
-            const auto s0 = __builtin_amdgcn_permlane32_swap(x[0].x, x[1].x, false, false);
-            const auto s1 = __builtin_amdgcn_permlane32_swap(x[0].y, x[1].y, false, false);
-            const int64_t chunk = (mw + i * 32) / 8 + q + half;
-            *reinterpret_cast<u32x4*>(g.P + (chunk * g.prow + n) * 16) = u32x4{s0[0], s1[0], s0[1], s1[1]};
-          }
+            for (int c = 0; c < 2; ++c) {
+              const f16x2 v = {(_Float16)acc[i + w][j][2 * c], (_Float16)acc[i + w][j][2 * c + 1]};
+              x[w][c] = __builtin_bit_cast(uint32_t, v);
+            }
+          *reinterpret_cast<u32x4*>(g.P + ((int64_t)((mw + (i + (G & 1)) * 16) / 8 + (G >> 1)) * g.prow + n) * 16) = lce_pair(x[0], x[1]);
+        }
       }
     }
   } else {
     const float alpha = g.splits > 1 ? 1.f : g.alpha[0];
 #pragma unroll
     for (int j = 0; j < SN; ++j) {
-      const int n = nw + j * 32;
-      if (n >= g.N) continue;
+      const int n = nw + j * 16;
+      const bool row = n < g.N;
+      const int64_t o = (int64_t)n * g.ldc + split * g.slab;
+      if (g.add && row) {
+        f32x4 x[SM];
 #pragma unroll
-      for (int i = 0; i < SM; ++i) {
-        const int m = mw + i * 32 + 4 * half;
-        const int64_t o = (int64_t)n * g.ldc + m + split * g.slab;
-        f32x4 v[4];
+        for (int i = 0; i < SM; ++i)
+          if (mw + i * 16 + 4 * G < g.M) x[i] = *reinterpret_cast<const f32x4*>(g.add + (int64_t)n * g.ldadd + mw + i * 16 + 4 * G);
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int i = 0; i < SM; ++i) acc[i][j] = alpha * acc[i][j] + x[i];
+      } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[q][e] = alpha * acc[i][j][4 * q + e];
-        if (g.add) {
-          f32x4 x[4];
+        for (int i = 0; i < SM; ++i) acc[i][j] *= alpha;
+      }
+      if (g.c_f32) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (m + 8 * q < g.M) x[q] = *reinterpret_cast<const f32x4*>(g.add + (int64_t)n * g.ldadd + m + 8 * q);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) v[q] += x[q];
+        for (int i = 0; i < SM; ++i) {
+          const int m = mw + i * 16 + 4 * G;
+          if (row && m < g.M) *reinterpret_cast<f32x4*>((float*)g.C + o + m) = acc[i][j];
         }
+      } else {
+        typedef E e4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (m + 8 * q >= g.M) continue;
-          if (g.c_f32) *reinterpret_cast<f32x4*>((float*)g.C + o + 8 * q) = v[q];
-          else {
-            typedef E e4 __attribute__((ext_vector_type(4)));
-            *reinterpret_cast<e4*>((E*)g.C + o + 8 * q) = __builtin_convertvector(v[q], e4);
-          }
+        for (int i = 0; i < SM; i += 2) {
+          const u32x4 v = lce_pair(__builtin_bit_cast(u32x2, __builtin_convertvector(acc[i][j], e4)),
+                                   __builtin_bit_cast(u32x2, __builtin_convertvector(acc[i + 1][j], e4)));
+          const int m = mw + (i + (G & 1)) * 16 + (G >> 1) * 8;
+          if (row && m < g.M) *reinterpret_cast<u32x4*>((E*)g.C + o + m) = v;
         }
       }
     }
