@@ -4,7 +4,7 @@
 //   d_rv = e^(l_rv - lse_r) - [v = t_r],  dh = alpha d W,  dW = alpha d^T h,  alpha = gscale / rows that count.
 //
 // Half-precision operands (bf16, fp16), per piece of rows:
-//   1. logits tiles on the matrix cores, fp32 accumulators.  A wave reduces its 128 vocabulary entries of a row to
+//   1. logits tiles on the matrix cores, fp32 accumulators.  A wave reduces its 128 (or 64) vocabulary entries of a row to
 //      (max, sum of e^(l - max)) in fp32 and, for training, leaves e^(l - max) in fp16 (values in (0, 1]: 11 bits where a
 //      later bf16 holds 8, so what reaches the gradients is rounded once) in P.
 //   2. per row: lse from the (max, sum) pairs, the loss, p_t - 1 by expm1 (no cancellation for sure rows).
@@ -35,7 +35,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 #define LCE_BK 32               // k of one tile of an operand
-#define LCE_SLAB 128            // vocabulary entries of one (max, sum) pair
 #define LCE_LOG2E 1.4426950408889634f
 #define LCE_LN2 0.6931471805599453f
 
@@ -64,7 +63,7 @@ struct LceArgs {
   int M, N, K;
   int tiles_m, tiles_n;
   // LOGITS
-  f32x2* stat;                    // [slab][prow] (max * log2 e, sum)
+  f32x2* stat;                    // [slab][prow] (max * log2 e, sum); a slab is a wave's vocabulary entries
   float* lt;                      // [row] logit of the target
   const int64_t* target;
   int grads;
@@ -115,10 +114,10 @@ __device__ __forceinline__ void lce_wait_vm() { asm volatile("s_waitcnt vmcnt(%0
 // One BM x BN tile of a product, WM x WN waves.  A tile of an operand is 32 k; it goes from memory straight into LDS, 16
 // bytes per lane, in one of three images:
 //   k-runs  (W and h of LOGITS, P of DH): [row][4 chunks of 8 k], chunk c of row r at c ^ (r / 2 & 3) - read 16 bytes a lane
-//   m-runs  (W of DH, h of DW): [k][chunks of 8 m], chunk c of row k at c ^ 2 (k & 3)                - read transposed
+//   m-runs  (W of DH, h of DW): [k][chunks of 8 m], chunk c of row k at c ^ (2 (k & 3) + (k & 8))      - read transposed
 //           (P of DW): [chunk of 8 m][k], k at k ^ 4 (chunk & 1)                                       - read transposed
 // The transposing read gives lane i of 16 the column i of a 4 x 16 block whose row r comes from lanes 4r .. 4r+3; the
-// swizzles put what the lanes of one LDS cycle read on different banks.
+// swizzles put what the 32 lanes of one LDS cycle read on different banks.
 //
 // NS tiles are in flight or in use.  Iteration kt: while the products of the wave's upper rows run, its lower rows' fragments
 // are read; then, once tile kt + 1 has landed for every wave and tile kt has been read by all (one barrier), tile kt + NS
@@ -161,7 +160,7 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
     constexpr int CR = BM / 8;
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
-      const int k = i * (NT / CR) + tid / CR, c = (tid % CR) ^ (2 * (k & 3));
+      const int k = i * (NT / CR) + tid / CR, c = (tid % CR) ^ (2 * (k & 3) + (k & 8));
       oa[i] = m0 + c * 8 < g.M ? (uint32_t)k * (uint32_t)g.lda + c * 16 : LCE_NONE;
     }
     pa = g.A + (int64_t)k_begin * g.lda + (int64_t)m0 * 2;
@@ -217,14 +216,16 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
   const int l16 = lane & 15, G = lane >> 4;
   const int kq = l16 * 64 + ((G ^ ((l16 >> 1) & 3)) * 16);                          // k-runs: row and chunk of this lane
   const int mk = (8 * G + (l16 >> 2)) * (BM * 2) + (l16 & 1) * 8;                   // m-runs [k][chunk]
-  const int mc = (l16 & 3) >> 1, mx = 2 * (l16 >> 2);
-  const int ma[4] = {mk + ((mc ^ mx) * 16), mk + (((2 + mc) ^ mx) * 16), mk + (((4 + mc) ^ mx) * 16), mk + (((6 + mc) ^ mx) * 16)};
+  const int mc = (l16 & 3) >> 1, mx = 2 * (l16 >> 2) + 8 * (G & 1);
+  int ma[SM];
+#pragma unroll
+  for (int i = 0; i < SM; ++i) ma[i] = mk + (((2 * (wm * SM + i) + mc) ^ mx) * 16);
   const int pb = ((l16 >> 1) & 1) * 64;
   const int pq = mc * 512 + (8 * G + (l16 >> 2)) * 16 + (l16 & 1) * 8;              // m-runs [chunk][k]
   static_assert(SM % 4 == 0 && SN % 2 == 0, "a wave's rows in whole 64s, its columns in whole 32s");
   const auto frag_a = [&](const char* buf, int i) -> typename H::v8 {
     if (A_K) return *reinterpret_cast<const typename H::v8*>(buf + (wm * SM + i) * 1024 + kq);
-    const char* q = buf + (wm * SM + (i & ~3)) * 32 + ma[i & 3];
+    const char* q = buf + ma[i];
     const u32x2 lo = lce_tr(q), hi = lce_tr(q + 4 * (BM * 2));
     return __builtin_bit_cast(typename H::v8, u32x4{lo.x, lo.y, hi.x, hi.y});
   };
@@ -342,7 +343,7 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
         }
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
-      if (G == 0 && mw < g.M) g.stat[(int64_t)(mw / LCE_SLAB) * g.prow + n] = f32x2{top, sum};
+      if (G == 0 && mw < g.M) g.stat[(int64_t)(mw / (SM * 16)) * g.prow + n] = f32x2{top, sum};
       if (g.grads) {
 #pragma unroll
         for (int i = 0; i < SM; i += 2) {
@@ -354,7 +355,9 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
               const f16x2 v = {(_Float16)acc[i + w][j][2 * c], (_Float16)acc[i + w][j][2 * c + 1]};
               x[w][c] = __builtin_bit_cast(uint32_t, v);
             }
-          *reinterpret_cast<u32x4*>(g.P + ((int64_t)((mw + (i + (G & 1)) * 16) / 8 + (G >> 1)) * g.prow + n) * 16) = lce_pair(x[0], x[1]);
+          // (past the caches: nothing reads P before all of it is there - 8192 x 131072: 3.84 -> 3.57 ms)
+          __builtin_nontemporal_store(lce_pair(x[0], x[1]),
+                                      reinterpret_cast<u32x4*>(g.P + ((int64_t)((mw + (i + (G & 1)) * 16) / 8 + (G >> 1)) * g.prow + n) * 16));
         }
       }
     }
@@ -397,7 +400,7 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
 }
 
 // ---- the passes between the products --------------------------------------------------------------------------------
-// head = {alpha = gscale / (rows that count, or 1) / lift, that count, 1}
+// head = {alpha = gscale / (rows that count, or 1) / lift, 1}
 __global__ __launch_bounds__(1024) void lce_begin_kernel(const int64_t* target, int64_t T, int64_t ignore, int V, int mean, float gscale,
                                                          float lift, float* head) {
   __shared__ int red[16];
@@ -406,14 +409,14 @@ __global__ __launch_bounds__(1024) void lce_begin_kernel(const int64_t* target, 
     for (int64_t i = threadIdx.x; i < T; i += 1024) c += target[i] != ignore;
   c = dpc_block_sum(c, red);
   if (threadIdx.x == 0) {
-    const float n = mean ? (float)max(c, 1) : 1.f;
-    head[0] = gscale / n / lift;
-    head[1] = n;
-    head[2] = 1.f;
+    head[0] = gscale / (mean ? (float)max(c, 1) : 1.f) / lift;
+    head[1] = 1.f;
   }
 }
 
-// Per row: lse from the slabs' (max, sum) pairs.  32 rows x 8 lanes of slabs per block.
+// Per row: lse from the slabs' (max, sum) pairs.  16 rows x 64 runs of slabs per block (one row of 8192 x 1024 slabs: 64 MB
+// that arrive as 128-byte pieces; with 8 runs a thread's chain of 128 dependent loads and exponents took 65 us for half
+// of that).
 struct LceRowArgs {
   const f32x2* stat; int64_t prow; int slabs; int rows; int V;
   const float* lt; const int64_t* target; int64_t ignore;
@@ -432,35 +435,30 @@ __device__ __forceinline__ void lce_row_end(const LceRowArgs& a, int n, float ls
     a.pm1[n] = off || bad ? 0.f : expm1f(-loss);
   }
 }
-__global__ __launch_bounds__(256) void lce_rows_kernel(LceRowArgs a) {
-  __shared__ f32x2 red[8][32];
-  const int r = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int n = blockIdx.x * 32 + r;
-  float top = -INFINITY, sum = 0.f;
+__device__ __forceinline__ f32x2 lce_join(f32x2 x, f32x2 y) {
+  const float m = fmaxf(x.x, y.x), ref = m == -INFINITY ? 0.f : m;
+  return f32x2{m, x.y * __builtin_amdgcn_exp2f(x.x - ref) + y.y * __builtin_amdgcn_exp2f(y.x - ref)};
+}
+__global__ __launch_bounds__(1024) void lce_rows_kernel(LceRowArgs a) {
+  __shared__ f32x2 red[64][16];
+  const int r = threadIdx.x & 15, w = threadIdx.x >> 4;
+  const int n = blockIdx.x * 16 + r;
+  f32x2 x = {-INFINITY, 0.f};
   if (n < a.rows) {
-    for (int s = w; s < a.slabs; s += 8) {
-      const f32x2 x = a.stat[(int64_t)s * a.prow + n];
-      const float m = fmaxf(top, x.x);
-      const float ref = m == -INFINITY ? 0.f : m;
-      sum = sum * __builtin_amdgcn_exp2f(top - ref) + x.y * __builtin_amdgcn_exp2f(x.x - ref);
-      top = m;
-    }
+    for (int s = w; s < a.slabs; s += 64) x = lce_join(x, a.stat[(int64_t)s * a.prow + n]);
   }
-  red[w][r] = f32x2{top, sum};
-  __syncthreads();
-  if (w == 0 && n < a.rows) {
-    float m = top;
-    for (int k = 1; k < 8; ++k) m = fmaxf(m, red[k][r].x);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float s = 0.f;
-    for (int k = 0; k < 8; ++k) s += red[k][r].y * __builtin_amdgcn_exp2f(red[k][r].x - ref);
-    lce_row_end(a, n, (ref + __builtin_amdgcn_logf(s)) * LCE_LN2, a.lt[n]);
+  red[w][r] = x;
+  for (int k = 32; k > 0; k >>= 1) {
+    __syncthreads();
+    if (w < k) red[w][r] = x = lce_join(x, red[w + k][r]);
   }
+  if (w == 0 && n < a.rows) lce_row_end(a, n, ((x.x == -INFINITY ? 0.f : x.x) + __builtin_amdgcn_logf(x.y)) * LCE_LN2, a.lt[n]);
 }
 
 // P from e^(l - slab max) in fp16 to d in the operands' type, in place.  One thread per row and slab.
-template <typename E>
-__global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, const f32x2* stat, int rows, int V, int chunks, const float* glse,
+// NT: P is much larger than the 256 MB of the last-level cache - read and written past it (2 GB: 846 -> 780 us; 0.3 GB: 96 -> 103 us).
+template <typename E, bool NT>
+__global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, const f32x2* stat, int rows, int slab_rows, const float* glse,
                                                         const float* pm1, const int64_t* target) {
   const int n = blockIdx.x * 256 + threadIdx.x, slab = blockIdx.y;
   const float gl = n < rows ? glse[n] : INFINITY;
@@ -469,18 +467,27 @@ __global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, c
   int at = -1;
   float pt = 0.f;
   if (live) {
-    const int64_t t = target[n] - (int64_t)slab * LCE_SLAB;
-    if (t >= 0 && t < LCE_SLAB) { at = (int)t; pt = pm1[n] * Half<E>::kUp; }
+    const int64_t t = target[n] - (int64_t)slab * slab_rows;
+    if (t >= 0 && t < slab_rows) { at = (int)t; pt = pm1[n] * Half<E>::kUp; }
   }
-#pragma unroll 4
-  for (int c = 0; c < LCE_SLAB / 8; ++c) {
-    if (slab * (LCE_SLAB / 8) + c >= chunks) break;
-    u32x4* q = reinterpret_cast<u32x4*>(P + ((int64_t)(slab * (LCE_SLAB / 8) + c) * prow + n) * 16);
-    const f16x8 x = __builtin_bit_cast(f16x8, *q);
-    typename Half<E>::v8 y;
+  char* p = P + ((int64_t)slab * (slab_rows / 8) * prow + n) * 16;
+  for (int c0 = 0; c0 < slab_rows / 8; c0 += 8) {
+    u32x4 q[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = (E)(live ? (c * 8 + e == at ? pt : (float)x[e] * f) : 0.f);
-    *q = __builtin_bit_cast(u32x4, y);
+    for (int c = 0; c < 8; ++c) {
+      const u32x4* at = reinterpret_cast<const u32x4*>(p + (c0 + c) * prow * 16);
+      q[c] = NT ? __builtin_nontemporal_load(at) : *at;
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const f16x8 x = __builtin_bit_cast(f16x8, q[c]);
+      typename Half<E>::v8 y;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = (E)(live ? ((c0 + c) * 8 + e == at ? pt : (float)x[e] * f) : 0.f);
+      u32x4* to = reinterpret_cast<u32x4*>(p + (c0 + c) * prow * 16);
+      if (NT) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, y), to);
+      else *to = __builtin_bit_cast(u32x4, y);
+    }
   }
 }
 
@@ -563,34 +570,51 @@ __global__ __launch_bounds__(256) void lce_zero_kernel(uint16_t* out, int64_t ld
   }
 }
 
-// sum of the rows' losses over the rows that count (one block, fixed order)
-__global__ __launch_bounds__(1024) void lce_total_kernel(const float* loss, int64_t T, const float* head, float* total) {
+// sum of the rows' losses, over the rows that count if `mean` (one block, fixed order)
+__global__ __launch_bounds__(1024) void lce_total_kernel(const float* loss, const int64_t* target, int64_t T, int64_t ignore, int mean, float* total) {
   __shared__ double red[16];
+  __shared__ int redi[16];
   double s = 0.0;
-  for (int64_t i = threadIdx.x; i < T; i += 1024) s += (double)loss[i];
+  int c = 0;
+  for (int64_t i = threadIdx.x; i < T; i += 1024) {
+    s += (double)loss[i];
+    c += target[i] != ignore;
+  }
   s = dpc_block_sum(s, red);
-  if (threadIdx.x == 0) total[0] = (float)(s / (double)head[1]);
+  c = dpc_block_sum(c, redi);
+  if (threadIdx.x == 0) total[0] = (float)(s / (mean ? (double)max(c, 1) : 1.0));
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
 static int64_t lce_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 static int lce_size(int dtype) { return dtype == DPC_F32 ? 4 : 2; }
 
-// Where things lie in the workspace for pieces of `rows` rows.
-struct LceLayout {
-  int64_t rows, prow;           // rows of a piece; padded to whole tiles
-  int64_t stat, lt, glse, pm1, P, hm, slabs, acc, bytes;   // byte offsets, and the whole
-  int splits_h, splits_w;
-  int pieces;
-};
+// Tiles of a product: 256 x 256 wherever that makes at least 192 of them; else 128 x 128, four times as many and three to a
+// CU; at most 64 rows of logits, which are bound by reading W once, 128 entries x 64 rows, four to a CU.
+enum { LCE_BIG = 0, LCE_MID = 1, LCE_ROW = 2 };
+static int64_t lce_tiles(int64_t M, int64_t N, int64_t bm, int64_t bn) { return dpc_cdiv(M, bm) * dpc_cdiv(N, bn); }
+static int lce_tile_kind(int64_t M, int64_t N, bool logits) {
+  if (logits && N <= 64) return LCE_ROW;
+  return lce_tiles(M, N, 256, 256) >= 192 ? LCE_BIG : LCE_MID;
+}
+static int lce_slab_rows(int kind) { return kind == LCE_BIG ? 128 : 64; }
 
-// K ranges of a product with `tiles` tiles: enough to give every CU a tile, none shorter than 512
-static int lce_splits(int64_t tiles, int64_t K) {
-  int64_t s = 256 / (tiles < 1 ? 1 : tiles);
+// K ranges of a product with `tiles` tiles: enough to give every CU `per` of them, none shorter than 512
+static int lce_splits(int64_t tiles, int64_t per, int64_t K) {
+  int64_t s = 256 * per / (tiles < 1 ? 1 : tiles);
   if (s > K / 512) s = K / 512;
   if (s > 32) s = 32;
   return s < 1 ? 1 : (int)s;
 }
+
+// Where things lie in the workspace for pieces of `rows` rows.
+struct LceLayout {
+  int64_t rows, prow;           // rows of a piece; padded to whole tiles
+  int64_t stat, lt, glse, pm1, P, hm, slabs, acc, bytes;   // byte offsets, and the whole
+  int tile_l, tile_h, tile_w;   // kinds of the three products' tiles
+  int splits_h, splits_w;
+  int pieces;
+};
 
 static LceLayout lce_layout(int64_t T, int D, int V, int dtype, bool grads, bool dw16, int64_t rows) {
   LceLayout l;
@@ -608,17 +632,22 @@ static LceLayout lce_layout(int64_t T, int D, int V, int dtype, bool grads, bool
   if (dtype == DPC_F32) {
     l.P = take(l.rows * (int64_t)V * 4);
     if (grads) {
-      l.splits_h = lce_splits(dpc_cdiv(l.rows, 64) * dpc_cdiv(D, 64), V);
+      l.splits_h = lce_splits(lce_tiles(D, l.rows, 64, 64), 1, V);
       if (l.splits_h > 1) l.slabs = take(l.splits_h * l.rows * (int64_t)D * 4);
       l.hm = take(l.rows * (int64_t)D * 4);
     }
   } else {
-    l.stat = take(dpc_cdiv(V, LCE_SLAB) * l.prow * 8);
+    l.tile_l = lce_tile_kind(V, l.rows, true);
+    l.stat = take(dpc_cdiv(V, lce_slab_rows(l.tile_l)) * l.prow * 8);
     if (grads) {
       l.P = take(lce_up(V, 256) * l.prow * 2);
       l.hm = take(l.prow * (int64_t)D * 2);
-      l.splits_h = lce_splits(dpc_cdiv(l.rows, 256) * dpc_cdiv(D, 256), V);
-      l.splits_w = lce_splits(dpc_cdiv(V, 256) * dpc_cdiv(D, 256), l.prow);
+      // (dh's K is the vocabulary: 256 x 256 tiles with K cut where they are few)
+      l.tile_h = lce_tiles(D, l.rows, 256, 256) * (V / 512) >= 256 ? LCE_BIG : LCE_MID;
+      l.tile_w = lce_tile_kind(D, V, false);
+      const int bh = l.tile_h == LCE_BIG ? 256 : 128, bw = l.tile_w == LCE_BIG ? 256 : 128;
+      l.splits_h = lce_splits(lce_tiles(D, l.rows, bh, bh), l.tile_h == LCE_BIG ? 1 : 2, V);
+      l.splits_w = lce_splits(lce_tiles(D, V, bw, bw), l.tile_w == LCE_BIG ? 1 : 2, l.prow);
       int64_t sl = 0;
       if (l.splits_h > 1) sl = l.splits_h * l.rows * (int64_t)D * 4;
       if (l.splits_w > 1 && l.splits_w * (int64_t)V * D * 4 > sl) sl = l.splits_w * (int64_t)V * D * 4;
@@ -638,28 +667,21 @@ static int lce_check(int64_t T, int D, int V, int dtype) {
 }
 
 // Rows of a piece where the caller names none: as many whole tiles as 1 GiB holds of what a row leaves (d, or the slabs'
-// pairs alone).
-static int64_t lce_rows_default(int V, int dtype, bool grads) {
-  const int64_t row = grads || dtype == DPC_F32 ? (int64_t)V * lce_size(dtype) : dpc_cdiv(V, LCE_SLAB) * 8;
-  const int64_t rows = (1ll << 30) / row / 256 * 256;
+// pairs alone) - and all of them where the fp32 sums of dW over several pieces would take the rest's place.
+static int64_t lce_rows_default(int64_t T, int D, int V, int dtype, bool grads, bool dw16) {
+  const int64_t row = grads || dtype == DPC_F32 ? (int64_t)V * lce_size(dtype) : dpc_cdiv(V, 64) * 8;
+  const int64_t room = 1ll << 30;
+  if (T * row <= room + (grads && dw16 ? (int64_t)V * D * 4 : 0)) return T < 1 ? 1 : T;
+  const int64_t rows = room / row / 256 * 256;
   return rows < 256 ? 256 : rows;
 }
 
 extern "C" int64_t dpc_linear_cross_entropy_ws(int64_t T, int D, int V, int dtype, int grads, int dw_f32, int64_t piece_rows) {
   if (lce_check(T, D, V, dtype) != DPC_OK) return -1;
-  if (piece_rows <= 0) piece_rows = lce_rows_default(V, dtype, grads != 0);
+  if (piece_rows <= 0) piece_rows = lce_rows_default(T, D, V, dtype, grads != 0, dtype != DPC_F32 && !dw_f32);
   return lce_layout(T, D, V, dtype, grads != 0, dtype != DPC_F32 && !dw_f32, piece_rows).bytes;
 }
 
-#ifndef LCE_CFG_0
-#define LCE_CFG_0 256, 256, 2, 4, 4
-#endif
-#ifndef LCE_CFG_1
-#define LCE_CFG_1 256, 256, 2, 4, 4
-#endif
-#ifndef LCE_CFG_2
-#define LCE_CFG_2 256, 256, 2, 4, 4
-#endif
 template <typename E, int MODE, int BM, int BN, int WM, int WN, int NS>
 static void lce_launch_tile(LceArgs& g, hipStream_t st) {
   g.tiles_m = (int)dpc_cdiv(g.M, BM);
@@ -668,9 +690,22 @@ static void lce_launch_tile(LceArgs& g, hipStream_t st) {
   g.kchunk = (int)lce_up(dpc_cdiv(g.K, g.splits), 64);
   hipLaunchKernelGGL((lce_product_kernel<E, MODE, BM, BN, WM, WN, NS>), dim3(g.tiles_m * g.tiles_n * g.splits), dim3(WM * WN * 64), 0, st, g);
 }
+#ifndef LCE_CFG_0
+#define LCE_CFG_0 256, 256, 2, 4, 3
+#endif
+#ifndef LCE_CFG_1
+#define LCE_CFG_1 256, 256, 2, 4, 3
+#endif
+#ifndef LCE_CFG_2
+#define LCE_CFG_2 256, 256, 2, 4, 3
+#endif
 template <typename E, int MODE>
-static void lce_launch(LceArgs& g, hipStream_t st) {
-  if constexpr (MODE == LCE_LOGITS) lce_launch_tile<E, MODE, LCE_CFG_0>(g, st);
+static void lce_launch(LceArgs& g, int kind, hipStream_t st) {
+  if (kind == LCE_MID) lce_launch_tile<E, MODE, 128, 128, 2, 2, 3>(g, st);
+  else if constexpr (MODE == LCE_LOGITS) {
+    if (kind == LCE_ROW) lce_launch_tile<E, MODE, 128, 64, 2, 1, 3>(g, st);
+    else lce_launch_tile<E, MODE, LCE_CFG_0>(g, st);
+  }
   else if constexpr (MODE == LCE_DH) lce_launch_tile<E, MODE, LCE_CFG_1>(g, st);
   else lce_launch_tile<E, MODE, LCE_CFG_2>(g, st);
 }
@@ -688,7 +723,7 @@ template <typename E>
 static int lce_half(const LceCall& c, const LceLayout& l, hipStream_t st) {
   float* head = (float*)c.ws;
   const bool grads = c.dh || c.dw;
-  const int slabs = (int)dpc_cdiv(c.V, LCE_SLAB);
+  const int slab_rows = lce_slab_rows(l.tile_l), slabs = (int)dpc_cdiv(c.V, slab_rows);
   for (int p = 0; p < l.pieces; ++p) {
     const int64_t r0 = p * l.rows;
     const int rows = (int)(c.T - r0 < l.rows ? c.T - r0 : l.rows);
@@ -699,22 +734,22 @@ static int lce_half(const LceCall& c, const LceLayout& l, hipStream_t st) {
     g.stat = (f32x2*)(c.ws + l.stat); g.lt = (float*)(c.ws + l.lt); g.grads = grads;
     g.A = c.w; g.lda = c.ldw * 2; g.B = h; g.ldb = c.ldh * 2;
     g.M = c.V; g.N = rows; g.K = c.D;
-    lce_launch<E, LCE_LOGITS>(g, st);
+    lce_launch<E, LCE_LOGITS>(g, l.tile_l, st);
     LceRowArgs ra;
     ra.stat = g.stat; ra.prow = l.prow; ra.slabs = slabs; ra.rows = rows; ra.V = c.V; ra.lt = g.lt; ra.target = g.target; ra.ignore = c.ignore;
     ra.loss = c.loss + r0; ra.lse = c.lse ? c.lse + r0 : nullptr;
     ra.glse = grads ? (float*)(c.ws + l.glse) : nullptr; ra.pm1 = (float*)(c.ws + l.pm1);
-    hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)dpc_cdiv(rows, 32)), dim3(256), 0, st, ra);
+    hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)dpc_cdiv(rows, 16)), dim3(1024), 0, st, ra);
     if (!grads) continue;
-    const int chunks = (int)(lce_up(c.V, 256) / 8);
-    hipLaunchKernelGGL(lce_scale_kernel<E>, dim3((unsigned)(l.prow / 256), (unsigned)slabs), dim3(256), 0, st, g.P, l.prow, g.stat, rows, c.V,
-                       chunks, ra.glse, ra.pm1, g.target);
+    const auto scale = lce_up(c.V, 256) * l.prow * 2 > (1ll << 30) ? lce_scale_kernel<E, true> : lce_scale_kernel<E, false>;
+    hipLaunchKernelGGL(scale, dim3((unsigned)(l.prow / 256), (unsigned)slabs), dim3(256), 0, st, g.P, l.prow, g.stat, rows, slab_rows, ra.glse, ra.pm1,
+                       g.target);
     if (c.dh) {
       LceArgs d = g;
       d.A = c.w; d.lda = c.ldw * 2; d.M = c.D; d.N = rows; d.K = c.V; d.splits = l.splits_h;
       if (l.splits_h > 1) { d.C = c.ws + l.slabs; d.ldc = c.D; d.c_f32 = 1; d.slab = (int64_t)rows * c.D; }
       else { d.C = c.dh + r0 * c.lddh * 2; d.ldc = c.lddh; }
-      lce_launch<E, LCE_DH>(d, st);
+      lce_launch<E, LCE_DH>(d, l.tile_h, st);
       if (l.splits_h > 1)
         hipLaunchKernelGGL(lce_fold_kernel<E>, dim3(dpc_grid((int64_t)rows * c.D / 4, 256)), dim3(256), 0, st, (const float*)(c.ws + l.slabs),
                            (int64_t)rows * c.D, l.splits_h, rows, c.D, head, nullptr, 0, c.dh + r0 * c.lddh * 2, c.lddh, 0);
@@ -736,7 +771,7 @@ static int lce_half(const LceCall& c, const LceLayout& l, hipStream_t st) {
       const int f32 = via ? !last : c.dw_f32;
       if (l.splits_w > 1) { d.C = c.ws + l.slabs; d.ldc = c.D; d.c_f32 = 1; d.slab = (int64_t)c.V * c.D; }
       else { d.C = out; d.ldc = ldo; d.c_f32 = f32; d.add = add; d.ldadd = ldadd; }
-      lce_launch<E, LCE_DW>(d, st);
+      lce_launch<E, LCE_DW>(d, l.tile_w, st);
       if (l.splits_w > 1)
         hipLaunchKernelGGL(lce_fold_kernel<E>, dim3(dpc_grid((int64_t)c.V * c.D / 4, 256)), dim3(256), 0, st, (const float*)(c.ws + l.slabs),
                            (int64_t)c.V * c.D, l.splits_w, c.V, c.D, head, add, ldadd, out, ldo, f32);
@@ -821,7 +856,7 @@ extern "C" int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* 
   }
   DPC_CHECK_ARG(((uintptr_t)ws & 255) == 0, "linear_cross_entropy: the workspace must be 256-byte aligned");
   const bool grads = dh || dw;
-  if (piece_rows <= 0) piece_rows = lce_rows_default(V, dtype, grads);
+  if (piece_rows <= 0) piece_rows = lce_rows_default(T, D, V, dtype, grads, !f32 && !dw_f32);
   DPC_CHECK_ARG(dpc_cdiv(V, 256) * dpc_cdiv(piece_rows < T ? piece_rows : T, 256) * 32 < (1ll << 31), "linear_cross_entropy: the piece is too large");
   DPC_CHECK_ARG(f32 || !grads || piece_rows <= (1 << 21) || T <= (1 << 21), "linear_cross_entropy: the piece is too large");
   const LceLayout l = lce_layout(T, D, V, dtype, grads, !f32 && !dw_f32, piece_rows);
@@ -832,13 +867,13 @@ extern "C" int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* 
   c.D = D; c.V = V; c.loss = loss; c.lse = lse; c.total = total; c.dh = (char*)dh; c.lddh = lddh; c.dw = (char*)dw; c.lddw = lddw;
   c.dw_f32 = dw_f32 || f32; c.accumulate = accumulate; c.gscale = gscale; c.mean = mean; c.ws = (char*)ws;
   const float lift = dtype == DPC_F16 ? Half<_Float16>::kUp : 1.f;
-  hipLaunchKernelGGL(lce_begin_kernel, dim3(1), dim3(1024), 0, st, target, T, ignore_index, V, mean, gscale, lift, (float*)ws);
+  if (grads) hipLaunchKernelGGL(lce_begin_kernel, dim3(1), dim3(1024), 0, st, target, T, ignore_index, V, mean, gscale, lift, (float*)ws);
   if (T == 0 && dw && !accumulate)
     hipLaunchKernelGGL(lce_zero_kernel, dim3(dpc_grid((int64_t)V * D, 256)), dim3(256), 0, st, (uint16_t*)dw, c.dw_f32 ? 2 * lddw : lddw, (int64_t)V,
                        c.dw_f32 ? 2 * D : D);
   const int rc = T == 0 ? DPC_OK : f32 ? lce_full(c, l, st) : (dtype == DPC_BF16 ? lce_half<__bf16>(c, l, st) : lce_half<_Float16>(c, l, st));
   if (rc != DPC_OK) return rc;
-  if (total) hipLaunchKernelGGL(lce_total_kernel, dim3(1), dim3(1024), 0, st, loss, T, (const float*)ws, total);
+  if (total) hipLaunchKernelGGL(lce_total_kernel, dim3(1), dim3(1024), 0, st, loss, target, T, ignore_index, mean, total);
   DPC_LAUNCH_CHECK();
   return DPC_OK;
 }

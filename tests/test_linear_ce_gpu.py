@@ -94,7 +94,8 @@ def call(ops, h, w, target, grads=True, dw=None, dh=None, piece_rows=0, **kw):
 
 
 SHAPES = [(1, 8, 1), (1, 64, 300), (3, 72, 129), (257, 128, 1000), (300, 200, 2049), (700, 264, 511), (513, 1024, 777),
-          (31, 2048, 257), (256, 64, 256), (1000, 136, 130), (40, 512, 9001)]
+          (31, 2048, 257), (256, 64, 256), (1000, 136, 130), (40, 512, 9001),
+          (64, 128, 700), (65, 128, 700), (128, 64, 25000), (3500, 72, 3500), (2, 1024, 30011)]
 
 
 def check(o, ref, grads=True):
