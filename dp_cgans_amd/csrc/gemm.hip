@@ -45,6 +45,7 @@ struct GemmArgs {
   const uint64_t* rng; uint32_t site;
   float leak;
   int splitk, kchunk;
+  int64_t split_slab;    // != 0: K range s stores its own partial product at C + s * split_slab (no atomics)
   int tiles_m, tiles_n;
   int a_vec, b_vec;
   const float* kscale;   // optional: A(m,k) *= kscale[k] (fused clip-scale-sum; m-contiguous A only)
@@ -811,8 +812,9 @@ __global__ __launch_bounds__(256, (BM == 128 ? 2 : 3)) void gemm_f32_kernel(Gemm
   gemm_tile_coords(g, slot - split * tiles, tile_m, tile_n);
   int k_begin = split * g.kchunk;
   int k_end = min(g.K, k_begin + g.kchunk);
-  if (k_begin >= k_end && split > 0) return;
-  gemm_segment<BM, BN, A_KC, B_KC, PF, KS>(g, lds, tile_m * BM, tile_n * BN, k_begin, k_end, g.splitk > 1 || g.force_atomic, split == 0);
+  if (k_begin >= k_end && split > 0 && !g.split_slab) return;
+  g.C += split * g.split_slab;
+  gemm_segment<BM, BN, A_KC, B_KC, PF, KS>(g, lds, tile_m * BM, tile_n * BN, k_begin, k_end, (g.splitk > 1 && !g.split_slab) || g.force_atomic, split == 0);
   DPC_STAMP(3);                                     // epilogue issued
 #ifdef DPC_GEMM_STAMP
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -1085,6 +1087,10 @@ static int gemm_one(const dpc_gemm_desc& d, hipStream_t st, GemmPlan* plan = nul
                             d.ld_bn_y >= d.stat_n && d.ld_bn_z >= d.stat_n && (beta == 0.f || beta == 1.f)),
                 "gemm: BatchNorm-backward statistics need colstat, y, z, mean, invstd and 1 <= stat_n <= N");
   g.force_atomic = d.atomic ? 1 : 0;
+  g.split_slab = d.split_slab;
+  DPC_CHECK_ARG(!d.split_slab || (d.splitk > 1 && d.tile == 64 && beta == 0.f && epi == EPI_NONE && !d.bias && !d.gat && !d.atomic && !d.seg_c && !plan &&
+                                  d.split_slab >= (int64_t)(M - 1) * d.ldc + N),
+                "gemm: slabs go with a forced split-K of a plain product on the 64x64 tile (beta == 0, not grouped) and must hold a product each");
   g.seed_out = d.seed_out; g.ld_seed = d.ld_seed; g.seed_row = d.seed_row; g.seed_col = d.seed_col;
   DPC_CHECK_ARG(!d.seed_out || (epi == EPI_LEAKY_DROPOUT && d.seed_row && d.seed_col && d.ld_seed >= N),
                 "gemm: the chain seed goes with the LeakyReLU + Dropout epilogue and needs seed_row, seed_col and ld_seed >= N");
@@ -1172,7 +1178,7 @@ static int gemm_one(const dpc_gemm_desc& d, hipStream_t st, GemmPlan* plan = nul
   const int ktiles = (int)dpc_cdiv(K, BK);
   g.kchunk = (int)dpc_cdiv(ktiles, splitk) * BK;
   if (K == 0) g.kchunk = BK;
-  if (splitk > 1 && beta == 0.f) {
+  if (splitk > 1 && beta == 0.f && !d.split_slab) {
     hipError_t e = hipMemset2DAsync(d.C, d.ldc * sizeof(float), 0, (size_t)N * sizeof(float), (size_t)M, st);
     if (e != hipSuccess) { dpc_set_error(hipGetErrorString(e)); return DPC_EHIP; }
     g.beta = 1.f;   // accumulate into the zeroed C

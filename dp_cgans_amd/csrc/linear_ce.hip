@@ -63,18 +63,29 @@ struct LceArgs {
   int M, N, K;
   int tiles_m, tiles_n;
   // LOGITS
-  f32x2* stat;                    // [slab][prow] (max * log2 e, sum); a slab is a wave's vocabulary entries
+  f32x2* stat;                    // [slab][prow] (reference, sum of 2^(l log2 e - reference)); a slab is a wave's vocabulary entries
   float* lt;                      // [row] logit of the target
   const int64_t* target;
   int grads;
   // DH / DW
   const float* alpha;
   void* C; int64_t ldc;           // elements
-  int c_f32;                      // C is fp32 (a slab of a split product, or the gradient itself)
+  int c_f32;                      // C is fp32
   const float* add;               // fp32 [n][ldadd] added to the result (accumulation over pieces, or into dW)
   int64_t ldadd;
-  int splits; int kchunk; int64_t slab;   // K ranges, each into its own fp32 slab (elements)
+  // tiles from `whole` on - the last, incomplete round of the chip - are cut into `splits` ranges of K, each of which leaves
+  // its fp32 sums in a slab of its own: part [split][tile][BN][BM]
+  int whole, splits, kchunk;
+  float* part;
 };
+
+// Tile `tl` of a product: groups of 8 m-tiles run through all n-tiles, so that the tiles an XCD works on at a time share
+// rows of both operands.
+__device__ __forceinline__ void lce_tile_at(int tl, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int per = 8 * tiles_n, grp = tl / per, gm = min(8, tiles_m - grp * 8);
+  tm = grp * 8 + (tl - grp * per) % gm;
+  tn = (tl - grp * per) / gm;
+}
 
 // Runs of neighbouring tiles per XCD: blocks go to the 8 XCDs in turn; each XCD takes a contiguous run of tile numbers
 // (the tail that does not divide by 8 stays in place).
@@ -134,13 +145,21 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  // tile: groups of 8 m-tiles run through all n-tiles, so that the tiles an XCD works on at a time share rows of both operands
-  const int tiles = g.tiles_m * g.tiles_n;
-  const int slot = lce_xcd(blockIdx.x, gridDim.x);
-  const int split = slot / tiles, tl = slot - split * tiles;
-  const int per = 8 * g.tiles_n, grp = tl / per, gm = min(8, g.tiles_m - grp * 8);
-  const int m0 = (grp * 8 + (tl - grp * per) % gm) * BM, n0 = ((tl - grp * per) / gm) * BN;
-  const int k_begin = split * g.kchunk, k_end = min(g.K, k_begin + g.kchunk);
+  const int rest = g.tiles_m * g.tiles_n - g.whole;
+  int tl, split = 0, k_begin = 0, k_end = g.K;
+  if ((int)blockIdx.x < g.whole) {
+    tl = lce_xcd(blockIdx.x, g.whole);
+  } else {
+    const int u = lce_xcd(blockIdx.x - g.whole, rest * g.splits);
+    split = u / rest;
+    tl = g.whole + u - split * rest;
+    k_begin = split * g.kchunk;
+    k_end = min(g.K, k_begin + g.kchunk);
+  }
+  int m0, n0;
+  lce_tile_at(tl, g.tiles_m, g.tiles_n, m0, n0);
+  m0 *= BM;
+  n0 *= BN;
   const int nk = (k_end - k_begin + LCE_BK - 1) / LCE_BK;
 
   // this thread's chunks of a K-tile, as offsets from the tile's first k; none where the operand ends
@@ -332,18 +351,19 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
         for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64)) * LCE_LOG2E;
-      const float ref = top == -INFINITY ? 0.f : top;                  // (all -inf: e^(l - 0) = 0, not NaN)
-      float sum = 0.f;
+      // the reference: the largest logit, rounded; what follows is exact relative to it.  (All -inf: 2^(l - 0) = 0, not NaN.)
+      const float ref = top == -INFINITY ? 0.f : top;
+      f32x4 run = {0.f, 0.f, 0.f, 0.f};                                // (four short sums: a sure row's is 1 and what little there is beside it)
 #pragma unroll
-      for (int i = 0; i < SM; ++i)
+      for (int i = 0; i < SM; ++i) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], LCE_LOG2E, -ref));
-          sum += acc[i][j][e];
-        }
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], LCE_LOG2E, -ref));
+        run += acc[i][j];
+      }
+      float sum = (run.x + run.y) + (run.z + run.w);
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
-      if (G == 0 && mw < g.M) g.stat[(int64_t)(mw / (SM * 16)) * g.prow + n] = f32x2{top, sum};
+      if (G == 0 && mw < g.M) g.stat[(int64_t)(mw / (SM * 16)) * g.prow + n] = f32x2{ref, sum};
       if (g.grads) {
 #pragma unroll
         for (int i = 0; i < SM; i += 2) {
@@ -362,12 +382,20 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
       }
     }
   } else {
-    const float alpha = g.splits > 1 ? 1.f : g.alpha[0];
+    if (tl >= g.whole) {
+      float* q = g.part + ((int64_t)(split * rest + tl - g.whole) * BN + wn * SN * 16 + l16) * BM + wm * SM * 16 + 4 * G;
+#pragma unroll
+      for (int j = 0; j < SN; ++j)
+#pragma unroll
+        for (int i = 0; i < SM; ++i) *reinterpret_cast<f32x4*>(q + j * 16 * BM + i * 16) = acc[i][j];
+      return;
+    }
+    const float alpha = g.alpha[0];
 #pragma unroll
     for (int j = 0; j < SN; ++j) {
       const int n = nw + j * 16;
       const bool row = n < g.N;
-      const int64_t o = (int64_t)n * g.ldc + split * g.slab;
+      const int64_t o = (int64_t)n * g.ldc;
       if (g.add && row) {
         f32x4 x[SM];
 #pragma unroll
@@ -400,51 +428,40 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
 }
 
 // ---- the passes between the products --------------------------------------------------------------------------------
-// head = {alpha = gscale / (rows that count, or 1) / lift, 1}
-__global__ __launch_bounds__(1024) void lce_begin_kernel(const int64_t* target, int64_t T, int64_t ignore, int V, int mean, float gscale,
-                                                         float lift, float* head) {
+// head[0] = alpha = gscale / (rows that count, or 1) / lift
+__global__ __launch_bounds__(1024) void lce_begin_kernel(const int64_t* target, int64_t T, int64_t ignore, int mean, float gscale, float lift, float* head) {
   __shared__ int red[16];
   int c = 0;
   if (mean)
     for (int64_t i = threadIdx.x; i < T; i += 1024) c += target[i] != ignore;
   c = dpc_block_sum(c, red);
-  if (threadIdx.x == 0) {
-    head[0] = gscale / (mean ? (float)max(c, 1) : 1.f) / lift;
-    head[1] = 1.f;
-  }
+  if (threadIdx.x == 0) head[0] = gscale / (mean ? (float)max(c, 1) : 1.f) / lift;
 }
 
-// Per row: lse from the slabs' (max, sum) pairs.  16 rows x 64 runs of slabs per block (one row of 8192 x 1024 slabs: 64 MB
-// that arrive as 128-byte pieces; with 8 runs a thread's chain of 128 dependent loads and exponents took 65 us for half
-// of that).
+// Two (reference, sum) pairs of a row as one.  (A sum of 0 - all logits -inf - leaves the other as it is.)
+__device__ __forceinline__ f32x2 lce_join(f32x2 x, f32x2 y) {
+  if (x.y == 0.f) return y;
+  if (y.y == 0.f) return x;
+  const float m = fmaxf(x.x, y.x);
+  return f32x2{m, x.y * __builtin_amdgcn_exp2f(x.x - m) + y.y * __builtin_amdgcn_exp2f(y.x - m)};
+}
+
+// Per row: the slabs' pairs become one, lse, the loss and what the gradient needs.  16 rows x 64 runs of slabs per block (with
+// 32 rows x 8 runs a thread's chain of 128 dependent loads and exponents took 65 us for 4096 x 1024 pairs, now 8).
 struct LceRowArgs {
   const f32x2* stat; int64_t prow; int slabs; int rows; int V;
   const float* lt; const int64_t* target; int64_t ignore;
   float* loss; float* lse;      // lse nullable
-  float* glse;                  // lse * log2 e, +inf in rows that take no part in the gradient
+  f32x2* live;                  // (reference, 1 / sum) of a row, (0, 0) where it takes no part in the gradient; nullable
   float* pm1;                   // p_t - 1
 };
-__device__ __forceinline__ void lce_row_end(const LceRowArgs& a, int n, float lse, float lt) {
-  const int64_t t = a.target[n];
-  const bool off = t == a.ignore, bad = !off && (t < 0 || t >= a.V);
-  const float loss = off ? 0.f : (bad ? NAN : lse - lt);
-  a.loss[n] = loss;
-  if (a.lse) a.lse[n] = lse;
-  if (a.glse) {
-    a.glse[n] = off || bad ? INFINITY : lse * LCE_LOG2E;
-    a.pm1[n] = off || bad ? 0.f : expm1f(-loss);
-  }
-}
-__device__ __forceinline__ f32x2 lce_join(f32x2 x, f32x2 y) {
-  const float m = fmaxf(x.x, y.x), ref = m == -INFINITY ? 0.f : m;
-  return f32x2{m, x.y * __builtin_amdgcn_exp2f(x.x - ref) + y.y * __builtin_amdgcn_exp2f(y.x - ref)};
-}
 __global__ __launch_bounds__(1024) void lce_rows_kernel(LceRowArgs a) {
   __shared__ f32x2 red[64][16];
   const int r = threadIdx.x & 15, w = threadIdx.x >> 4;
   const int n = blockIdx.x * 16 + r;
-  f32x2 x = {-INFINITY, 0.f};
+  f32x2 x = {0.f, 0.f};
   if (n < a.rows) {
+#pragma unroll 4
     for (int s = w; s < a.slabs; s += 64) x = lce_join(x, a.stat[(int64_t)s * a.prow + n]);
   }
   red[w][r] = x;
@@ -452,21 +469,33 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(LceRowArgs a) {
     __syncthreads();
     if (w < k) red[w][r] = x = lce_join(x, red[w + k][r]);
   }
-  if (w == 0 && n < a.rows) lce_row_end(a, n, ((x.x == -INFINITY ? 0.f : x.x) + __builtin_amdgcn_logf(x.y)) * LCE_LN2, a.lt[n]);
+  if (w != 0 || n >= a.rows) return;
+  const int64_t t = a.target[n];
+  const bool off = t == a.ignore, bad = !off && (t < 0 || t >= a.V);
+  // The loss from what is exact near it: where the target is the row's largest logit the difference of the references is the
+  // rounding of one product, and the loss the logarithm of the sum - not the difference of two numbers of the logits' size.
+  const float l2 = log2f(x.y);
+  const float loss = off ? 0.f : (bad ? NAN : LCE_LN2 * (fmaf(-a.lt[n], LCE_LOG2E, x.x) + l2));
+  a.loss[n] = loss;
+  if (a.lse) a.lse[n] = LCE_LN2 * (x.x + l2);
+  if (a.live) {
+    a.live[n] = off || bad ? f32x2{0.f, 0.f} : f32x2{x.x, 1.f / x.y};
+    a.pm1[n] = off || bad ? 0.f : expm1f(-loss);
+  }
 }
 
 // P from e^(l - slab max) in fp16 to d in the operands' type, in place.  One thread per row and slab.
 // NT: P is much larger than the 256 MB of the last-level cache - read and written past it (2 GB: 846 -> 780 us; 0.3 GB: 96 -> 103 us).
 template <typename E, bool NT>
-__global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, const f32x2* stat, int rows, int slab_rows, const float* glse,
+__global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, const f32x2* stat, int rows, int slab_rows, const f32x2* live,
                                                         const float* pm1, const int64_t* target) {
-  const int n = blockIdx.x * 256 + threadIdx.x, slab = blockIdx.y;
-  const float gl = n < rows ? glse[n] : INFINITY;
-  const bool live = gl != INFINITY;
-  const float f = live ? __builtin_amdgcn_exp2f(stat[(int64_t)slab * prow + n].x - gl) * Half<E>::kUp : 0.f;
+  const int nb = (int)(prow / 256), slab = blockIdx.x / nb, n = (blockIdx.x - slab * nb) * 256 + threadIdx.x;
+  const f32x2 gl = n < rows ? live[n] : f32x2{0.f, 0.f};
+  const bool on = gl.y != 0.f;                                         // (NaN is on: such a row keeps its NaN)
+  const float f = on ? __builtin_amdgcn_exp2f(stat[(int64_t)slab * prow + n].x - gl.x) * gl.y * Half<E>::kUp : 0.f;
   int at = -1;
   float pt = 0.f;
-  if (live) {
+  if (on) {
     const int64_t t = target[n] - (int64_t)slab * slab_rows;
     if (t >= 0 && t < slab_rows) { at = (int)t; pt = pm1[n] * Half<E>::kUp; }
   }
@@ -483,7 +512,7 @@ __global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, c
       const f16x8 x = __builtin_bit_cast(f16x8, q[c]);
       typename Half<E>::v8 y;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = (E)(live ? ((c0 + c) * 8 + e == at ? pt : (float)x[e] * f) : 0.f);
+      for (int e = 0; e < 8; ++e) y[e] = (E)(on ? ((c0 + c) * 8 + e == at ? pt : (float)x[e] * f) : 0.f);
       u32x4* to = reinterpret_cast<u32x4*>(p + (c0 + c) * prow * 16);
       if (NT) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, y), to);
       else *to = __builtin_bit_cast(u32x4, y);
@@ -493,69 +522,109 @@ __global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, c
 
 // h with its ignored rows, and the rows up to the end of the piece's last tile, set to 0: what such a row holds must
 // not reach dW (0 x NaN)
-__global__ __launch_bounds__(256) void lce_mask_rows_kernel(const char* h, int64_t ldh, int rows, int64_t total16, int row16, const float* glse, char* out) {
+__global__ __launch_bounds__(256) void lce_mask_rows_kernel(const char* h, int64_t ldh, int rows, int64_t total16, int row16, const f32x2* live, char* out) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total16; i += (int64_t)gridDim.x * 256) {
     const int n = (int)(i / row16), c = (int)(i - (int64_t)n * row16);
     u32x4 v = {0u, 0u, 0u, 0u};
-    if (n < rows && glse[n] != INFINITY) v = *reinterpret_cast<const u32x4*>(h + (int64_t)n * ldh + c * 16);
+    if (n < rows && live[n].y != 0.f) v = *reinterpret_cast<const u32x4*>(h + (int64_t)n * ldh + c * 16);
     *reinterpret_cast<u32x4*>(out + i * 16) = v;
   }
 }
 
-// out[n][m] = alpha * sum of the split product's slabs, in their order
-template <typename E>
-__global__ __launch_bounds__(256) void lce_fold_kernel(const float* slabs, int64_t slab, int splits, int N, int M, const float* alpha,
-                                                       const float* add, int64_t ldadd, void* out, int64_t ldo, int out_f32) {
-  const int m4 = M / 4;
-  const float al = alpha[0];
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)N * m4; i += (int64_t)gridDim.x * 256) {
-    const int n = (int)(i / m4), m = (int)(i - (int64_t)n * m4) * 4;
-    f32x4 v = *reinterpret_cast<const f32x4*>(slabs + i * 4);
-    for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(slabs + s * slab + i * 4);
-    v *= al;
-    if (add) v += *reinterpret_cast<const f32x4*>(add + (int64_t)n * ldadd + m);
-    if (out_f32) *reinterpret_cast<f32x4*>((float*)out + (int64_t)n * ldo + m) = v;
-    else {
-      typedef E e4 __attribute__((ext_vector_type(4)));
-      *reinterpret_cast<e4*>((E*)out + (int64_t)n * ldo + m) = __builtin_convertvector(v, e4);
-    }
+// C[n][m] = alpha * (sum of the K ranges' slabs, in their order) [+ add] for the tiles that were cut.  One block per 1024 entries.
+template <typename E, int BM, int BN>
+__global__ __launch_bounds__(256) void lce_fold_kernel(LceArgs g) {
+  const int rest = g.tiles_m * g.tiles_n - g.whole;
+  const int t = blockIdx.x / (BM * BN / 1024), at = (blockIdx.x % (BM * BN / 1024)) * 1024 + threadIdx.x * 4;
+  int tm, tn;
+  lce_tile_at(g.whole + t, g.tiles_m, g.tiles_n, tm, tn);
+  const int n = tn * BN + at / BM, m = tm * BM + at % BM;
+  if (n >= g.N || m >= g.M) return;
+  const float* q = g.part + (int64_t)t * BM * BN + at;
+  f32x4 v = *reinterpret_cast<const f32x4*>(q);
+#pragma unroll 4
+  for (int s = 1; s < g.splits; ++s) v += *reinterpret_cast<const f32x4*>(q + (int64_t)s * rest * (BM * BN));
+  v *= g.alpha[0];
+  if (g.add) v += *reinterpret_cast<const f32x4*>(g.add + (int64_t)n * g.ldadd + m);
+  const int64_t o = (int64_t)n * g.ldc + m;
+  if (g.c_f32) *reinterpret_cast<f32x4*>((float*)g.C + o) = v;
+  else {
+    typedef E e4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<e4*>((E*)g.C + o) = __builtin_convertvector(v, e4);
   }
 }
 
-// fp32: a row of logits to its loss and, in place, to alpha d; and h with its ignored rows set to 0.  One block per row.
-__global__ __launch_bounds__(256) void lce_rows_f32_kernel(float* logits, int64_t ld, LceRowArgs a, const float* alpha, const float* h, int64_t ldh,
-                                                           float* hm, int D) {
+// ---- fp32 -------------------------------------------------------------------------------------------------------------
+// A block's 4096 logits of a row: their pair, the target's logit.  [row][ld], rows 16-byte aligned.
+#define LCE_SEG 4096
+__global__ __launch_bounds__(256) void lce_stat_f32_kernel(const float* logits, int64_t ld, int V, const int64_t* target, f32x2* stat, int64_t prow, float* lt) {
   __shared__ float red[16];
-  const int n = blockIdx.x;
-  float* x = logits + (int64_t)n * ld;
-  const int64_t t = a.target[n];
-  const bool live = t != a.ignore && t >= 0 && t < a.V;
+  const int segs = (V + LCE_SEG - 1) / LCE_SEG, n = blockIdx.x / segs, seg = blockIdx.x - n * segs, v0 = seg * LCE_SEG;
+  const float* x = logits + (int64_t)n * ld + v0;
+  f32x4 q[4];
   float top = -INFINITY;
-  for (int v = threadIdx.x; v < a.V; v += 256) top = fmaxf(top, x[v]);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int v = k * 1024 + threadIdx.x * 4;
+    q[k] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (v0 + v < V) q[k] = *reinterpret_cast<const f32x4*>(x + v);      // (the row's padding is within its stride)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (v0 + v + e >= V) q[k][e] = -INFINITY;
+      top = fmaxf(top, q[k][e]);
+    }
+  }
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float ref = top == -INFINITY ? 0.f : top * LCE_LOG2E;
-  float sum = 0.f;
-  for (int v = threadIdx.x; v < a.V; v += 256) sum += __builtin_amdgcn_exp2f(fmaf(x[v], LCE_LOG2E, -ref));
-  sum = dpc_block_sum(sum, red);
-  const float lse2 = ref + __builtin_amdgcn_logf(sum), lse = lse2 * LCE_LN2;
-  const float lt = live ? x[t] : 0.f;
-  if (threadIdx.x == 0) lce_row_end(a, n, lse, lt);
-  if (!alpha) return;
-  __syncthreads();                                                     // x[t] has been read
-  const float al = alpha[0];
-  for (int v = threadIdx.x; v < a.V; v += 256)
-    x[v] = live ? al * (v == t ? expm1f(lt - lse) : __builtin_amdgcn_exp2f(fmaf(x[v], LCE_LOG2E, -lse2))) : 0.f;
-  if (hm)
-    for (int k = threadIdx.x; k < D; k += 256) hm[(int64_t)n * D + k] = live ? h[(int64_t)n * ldh + k] : 0.f;
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) * LCE_LOG2E;
+  const float ref = top == -INFINITY ? 0.f : top;
+  f32x4 run = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) run[e] += __builtin_amdgcn_exp2f(fmaf(q[k][e], LCE_LOG2E, -ref));
+  const float sum = dpc_block_sum((run.x + run.y) + (run.z + run.w), red);
+  if (threadIdx.x == 0) {
+    stat[(int64_t)seg * prow + n] = f32x2{ref, sum};
+    const int64_t t = target[n] - v0;
+    if (t >= 0 && t < LCE_SEG && v0 + t < V) lt[n] = x[t];
+  }
 }
 
-// out[n][m] = sum of the split product's fp32 slabs [n][M], in their order
-__global__ __launch_bounds__(256) void lce_fold_f32_kernel(const float* slabs, int64_t slab, int splits, int64_t N, int M, float* out, int64_t ldo) {
+// Logits to alpha * d, in place.
+__global__ __launch_bounds__(256) void lce_d_f32_kernel(float* logits, int64_t ld, int V, const int64_t* target, const f32x2* live, const float* pm1,
+                                                        const float* alpha) {
+  const int segs = (V + LCE_SEG - 1) / LCE_SEG, n = blockIdx.x / segs, seg = blockIdx.x - n * segs;
+  const f32x2 gl = live[n];
+  const bool on = gl.y != 0.f;
+  const int64_t t = target[n];
+  const float al = alpha[0], f = al * gl.y, pt = al * pm1[n];
+  float* x = logits + (int64_t)n * ld;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int v = seg * LCE_SEG + k * 1024 + threadIdx.x * 4;
+    if (v >= V) break;
+    f32x4 q = *reinterpret_cast<const f32x4*>(x + v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = on ? (v + e == t ? pt : f * __builtin_amdgcn_exp2f(fmaf(q[e], LCE_LOG2E, -gl.x))) : 0.f;
+    *reinterpret_cast<f32x4*>(x + v) = q;
+  }
+}
+
+// h with its ignored rows set to 0
+__global__ __launch_bounds__(256) void lce_mask_rows_f32_kernel(const float* h, int64_t ldh, int64_t total, int D, const f32x2* live, float* out) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t n = i / D;
+    out[i] = live[n].y != 0.f ? h[n * ldh + (i - n * D)] : 0.f;
+  }
+}
+
+// out[n][m] = sum of the split product's slabs [n][M], in their order
+__global__ __launch_bounds__(256) void lce_fold_f32_kernel(const float* slabs, int64_t slab, int splits, int M, float* out, int64_t ldo) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < slab; i += (int64_t)gridDim.x * 256) {
     float v = slabs[i];
+#pragma unroll 4
     for (int s = 1; s < splits; ++s) v += slabs[s * slab + i];
     const int64_t n = i / M;
     out[n * ldo + (i - n * M)] = v;
@@ -599,20 +668,33 @@ static int lce_tile_kind(int64_t M, int64_t N, bool logits) {
 }
 static int lce_slab_rows(int kind) { return kind == LCE_BIG ? 128 : 64; }
 
-// K ranges of a product with `tiles` tiles: enough to give every CU `per` of them, none shorter than 512
-static int lce_splits(int64_t tiles, int64_t per, int64_t K) {
-  int64_t s = 256 * per / (tiles < 1 ? 1 : tiles);
-  if (s > K / 512) s = K / 512;
+// The tiles of a product that make whole rounds of the chip (256 CUs, `per` blocks each), and the K ranges of the others:
+// as many as fill a round, none shorter than `least`; not cut at all where two would be (a round of them saves less
+// than writing and adding up their sums costs).
+struct LceCut { int whole, splits; int64_t part; };
+static LceCut lce_cut(int64_t tiles, int kind, int64_t K) {
+  const int64_t slots = kind == LCE_BIG ? 256 : 512, least = kind == LCE_BIG ? 1024 : 512;
+  const int64_t rest = tiles % slots;
+  int64_t s = rest ? slots / rest : 1;
+  if (s > K / least) s = K / least;
   if (s > 32) s = 32;
-  return s < 1 ? 1 : (int)s;
+  LceCut c = {(int)tiles, 1, 0};
+  if (s >= 2) {
+    const int edge = kind == LCE_BIG ? 256 : 128;
+    c.whole = (int)(tiles - rest);
+    c.splits = (int)s;
+    c.part = s * rest * edge * edge * 4;
+  }
+  return c;
 }
+static int lce_edge(int kind) { return kind == LCE_BIG ? 256 : 128; }
 
 // Where things lie in the workspace for pieces of `rows` rows.
 struct LceLayout {
   int64_t rows, prow;           // rows of a piece; padded to whole tiles
-  int64_t stat, lt, glse, pm1, P, hm, slabs, acc, bytes;   // byte offsets, and the whole
+  int64_t stat, lt, live, pm1, P, ldp, hm, part, acc, bytes;   // byte offsets (ldp: fp32 logits' row length), and the whole
   int tile_l, tile_h, tile_w;   // kinds of the three products' tiles
-  int splits_h, splits_w;
+  int splits;                   // fp32: K ranges of dh
   int pieces;
 };
 
@@ -626,14 +708,23 @@ static LceLayout lce_layout(int64_t T, int D, int V, int dtype, bool grads, bool
   int64_t at = 256;                                                    // head
   const auto take = [&](int64_t bytes) { const int64_t o = at; at += lce_up(bytes, 256); return o; };
   l.lt = take(l.prow * 4);
-  l.glse = take(l.prow * 4);
+  l.live = take(l.prow * 8);
   l.pm1 = take(l.prow * 4);
-  l.splits_h = l.splits_w = 1;
+  l.splits = 1;
   if (dtype == DPC_F32) {
-    l.P = take(l.rows * (int64_t)V * 4);
+    l.ldp = lce_up(V, 4);
+    l.stat = take(dpc_cdiv(V, LCE_SEG) * l.prow * 8);
+    l.P = take(l.rows * l.ldp * 4);
     if (grads) {
-      l.splits_h = lce_splits(lce_tiles(D, l.rows, 64, 64), 1, V);
-      if (l.splits_h > 1) l.slabs = take(l.splits_h * l.rows * (int64_t)D * 4);
+      // 64 x 64 tiles, three to a CU; no range shorter than 256, none empty
+      const int64_t tiles = lce_tiles(D, l.rows, 64, 64), kt = dpc_cdiv(V, 32);
+      int64_t s = 768 / tiles;
+      if (s > V / 256) s = V / 256;
+      if (s > 32) s = 32;
+      if (s > 1) {
+        l.splits = (int)dpc_cdiv(kt, dpc_cdiv(kt, s));
+        l.part = take(l.splits * l.rows * (int64_t)D * 4);
+      }
       l.hm = take(l.rows * (int64_t)D * 4);
     }
   } else {
@@ -642,16 +733,15 @@ static LceLayout lce_layout(int64_t T, int D, int V, int dtype, bool grads, bool
     if (grads) {
       l.P = take(lce_up(V, 256) * l.prow * 2);
       l.hm = take(l.prow * (int64_t)D * 2);
-      // (dh's K is the vocabulary: 256 x 256 tiles with K cut where they are few)
-      l.tile_h = lce_tiles(D, l.rows, 256, 256) * (V / 512) >= 256 ? LCE_BIG : LCE_MID;
+      // (dh's K is the vocabulary: 256 x 256 tiles also where they are few, if K can be cut into as many ranges as fill the chip)
+      l.tile_h = lce_tiles(D, l.rows, 256, 256) * (V / 1024) >= 192 ? LCE_BIG : LCE_MID;
       l.tile_w = lce_tile_kind(D, V, false);
-      const int bh = l.tile_h == LCE_BIG ? 256 : 128, bw = l.tile_w == LCE_BIG ? 256 : 128;
-      l.splits_h = lce_splits(lce_tiles(D, l.rows, bh, bh), l.tile_h == LCE_BIG ? 1 : 2, V);
-      l.splits_w = lce_splits(lce_tiles(D, V, bw, bw), l.tile_w == LCE_BIG ? 1 : 2, l.prow);
-      int64_t sl = 0;
-      if (l.splits_h > 1) sl = l.splits_h * l.rows * (int64_t)D * 4;
-      if (l.splits_w > 1 && l.splits_w * (int64_t)V * D * 4 > sl) sl = l.splits_w * (int64_t)V * D * 4;
-      if (sl) l.slabs = take(sl);
+      const LceCut h = lce_cut(lce_tiles(D, l.rows, lce_edge(l.tile_h), lce_edge(l.tile_h)), l.tile_h, V);
+      const LceCut w = lce_cut(lce_tiles(D, V, lce_edge(l.tile_w), lce_edge(l.tile_w)), l.tile_w, l.prow);
+      // (the last piece has fewer rows: fewer tiles of dh, then cut into more ranges - a round of them at most)
+      const int64_t most = 256ll * 256 * 256 * 4;
+      const int64_t part = l.pieces > 1 ? most : (h.part > w.part ? h.part : w.part);
+      if (part) l.part = take(part);
       if (dw16 && l.pieces > 1) l.acc = take((int64_t)V * D * 4);
     }
   }
@@ -660,7 +750,7 @@ static LceLayout lce_layout(int64_t T, int D, int V, int dtype, bool grads, bool
 }
 
 static int lce_check(int64_t T, int D, int V, int dtype) {
-  DPC_CHECK_ARG(T >= 0 && T < (1ll << 31) && D >= 1 && V >= 1 && V <= (1 << 30), "linear_cross_entropy: bad size");
+  DPC_CHECK_ARG(T >= 0 && T < (1ll << 31) && D >= 1 && V >= 1 && V <= (1 << 28), "linear_cross_entropy: bad size");
   DPC_CHECK_ARG(dtype == DPC_F32 || dtype == DPC_BF16 || dtype == DPC_F16, "linear_cross_entropy: unknown element type");
   DPC_CHECK_ARG(dtype == DPC_F32 || D % 8 == 0, "linear_cross_entropy: half-precision rows need a width that is a multiple of 8");
   return DPC_OK;
@@ -683,12 +773,17 @@ extern "C" int64_t dpc_linear_cross_entropy_ws(int64_t T, int D, int V, int dtyp
 }
 
 template <typename E, int MODE, int BM, int BN, int WM, int WN, int NS>
-static void lce_launch_tile(LceArgs& g, hipStream_t st) {
+static void lce_launch_tile(LceArgs& g, int kind, hipStream_t st) {
   g.tiles_m = (int)dpc_cdiv(g.M, BM);
   g.tiles_n = (int)dpc_cdiv(g.N, BN);
-  if (g.splits < 1) g.splits = 1;
-  g.kchunk = (int)lce_up(dpc_cdiv(g.K, g.splits), 64);
-  hipLaunchKernelGGL((lce_product_kernel<E, MODE, BM, BN, WM, WN, NS>), dim3(g.tiles_m * g.tiles_n * g.splits), dim3(WM * WN * 64), 0, st, g);
+  const int tiles = g.tiles_m * g.tiles_n;
+  const LceCut c = MODE == LCE_LOGITS ? LceCut{tiles, 1, 0} : lce_cut(tiles, kind, g.K);
+  g.whole = c.whole;
+  g.splits = c.splits;
+  g.kchunk = (int)lce_up(dpc_cdiv(g.K, g.splits), LCE_BK);
+  hipLaunchKernelGGL((lce_product_kernel<E, MODE, BM, BN, WM, WN, NS>), dim3(g.whole + (tiles - g.whole) * g.splits), dim3(WM * WN * 64), 0, st, g);
+  if (MODE != LCE_LOGITS && g.whole < tiles)
+    hipLaunchKernelGGL((lce_fold_kernel<E, BM, BN>), dim3((tiles - g.whole) * (BM * BN / 1024)), dim3(256), 0, st, g);
 }
 #ifndef LCE_CFG_0
 #define LCE_CFG_0 256, 256, 2, 4, 3
@@ -701,13 +796,13 @@ static void lce_launch_tile(LceArgs& g, hipStream_t st) {
 #endif
 template <typename E, int MODE>
 static void lce_launch(LceArgs& g, int kind, hipStream_t st) {
-  if (kind == LCE_MID) lce_launch_tile<E, MODE, 128, 128, 2, 2, 3>(g, st);
+  if (kind == LCE_MID) lce_launch_tile<E, MODE, 128, 128, 2, 2, 3>(g, kind, st);
   else if constexpr (MODE == LCE_LOGITS) {
-    if (kind == LCE_ROW) lce_launch_tile<E, MODE, 128, 64, 2, 1, 3>(g, st);
-    else lce_launch_tile<E, MODE, LCE_CFG_0>(g, st);
+    if (kind == LCE_ROW) lce_launch_tile<E, MODE, 128, 64, 2, 1, 3>(g, kind, st);
+    else lce_launch_tile<E, MODE, LCE_CFG_0>(g, kind, st);
   }
-  else if constexpr (MODE == LCE_DH) lce_launch_tile<E, MODE, LCE_CFG_1>(g, st);
-  else lce_launch_tile<E, MODE, LCE_CFG_2>(g, st);
+  else if constexpr (MODE == LCE_DH) lce_launch_tile<E, MODE, LCE_CFG_1>(g, kind, st);
+  else lce_launch_tile<E, MODE, LCE_CFG_2>(g, kind, st);
 }
 
 struct LceCall {
@@ -738,43 +833,34 @@ static int lce_half(const LceCall& c, const LceLayout& l, hipStream_t st) {
     LceRowArgs ra;
     ra.stat = g.stat; ra.prow = l.prow; ra.slabs = slabs; ra.rows = rows; ra.V = c.V; ra.lt = g.lt; ra.target = g.target; ra.ignore = c.ignore;
     ra.loss = c.loss + r0; ra.lse = c.lse ? c.lse + r0 : nullptr;
-    ra.glse = grads ? (float*)(c.ws + l.glse) : nullptr; ra.pm1 = (float*)(c.ws + l.pm1);
+    ra.live = grads ? (f32x2*)(c.ws + l.live) : nullptr; ra.pm1 = (float*)(c.ws + l.pm1);
     hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)dpc_cdiv(rows, 16)), dim3(1024), 0, st, ra);
     if (!grads) continue;
     const auto scale = lce_up(c.V, 256) * l.prow * 2 > (1ll << 30) ? lce_scale_kernel<E, true> : lce_scale_kernel<E, false>;
-    hipLaunchKernelGGL(scale, dim3((unsigned)(l.prow / 256), (unsigned)slabs), dim3(256), 0, st, g.P, l.prow, g.stat, rows, slab_rows, ra.glse, ra.pm1,
+    hipLaunchKernelGGL(scale, dim3((unsigned)(l.prow / 256 * slabs)), dim3(256), 0, st, g.P, l.prow, g.stat, rows, slab_rows, ra.live, ra.pm1,
                        g.target);
     if (c.dh) {
       LceArgs d = g;
-      d.A = c.w; d.lda = c.ldw * 2; d.M = c.D; d.N = rows; d.K = c.V; d.splits = l.splits_h;
-      if (l.splits_h > 1) { d.C = c.ws + l.slabs; d.ldc = c.D; d.c_f32 = 1; d.slab = (int64_t)rows * c.D; }
-      else { d.C = c.dh + r0 * c.lddh * 2; d.ldc = c.lddh; }
+      d.A = c.w; d.lda = c.ldw * 2; d.M = c.D; d.N = rows; d.K = c.V;
+      d.C = c.dh + r0 * c.lddh * 2; d.ldc = c.lddh; d.part = (float*)(c.ws + l.part);
       lce_launch<E, LCE_DH>(d, l.tile_h, st);
-      if (l.splits_h > 1)
-        hipLaunchKernelGGL(lce_fold_kernel<E>, dim3(dpc_grid((int64_t)rows * c.D / 4, 256)), dim3(256), 0, st, (const float*)(c.ws + l.slabs),
-                           (int64_t)rows * c.D, l.splits_h, rows, c.D, head, nullptr, 0, c.dh + r0 * c.lddh * 2, c.lddh, 0);
     }
     if (c.dw) {
       const int64_t row16 = c.D / 8;
       char* hm = c.ws + l.hm;
       hipLaunchKernelGGL(lce_mask_rows_kernel, dim3(dpc_grid(l.prow * row16, 256)), dim3(256), 0, st, h, c.ldh * 2, rows, l.prow * row16, (int)row16,
-                         ra.glse, hm);
+                         ra.live, hm);
       LceArgs d = g;
-      d.A = hm; d.lda = (int64_t)c.D * 2; d.M = c.D; d.N = c.V; d.K = (int)lce_up(rows, LCE_BK); d.splits = l.splits_w;
+      d.A = hm; d.lda = (int64_t)c.D * 2; d.M = c.D; d.N = c.V; d.K = (int)lce_up(rows, LCE_BK); d.part = (float*)(c.ws + l.part);
       // where the piece's share goes: dW itself, or the fp32 sums over the pieces until the last one
-      const bool last = p + 1 == l.pieces;
-      const bool via = !c.dw_f32 && l.pieces > 1;
+      const bool last = p + 1 == l.pieces, via = !c.dw_f32 && l.pieces > 1;
       float* acc = (float*)(c.ws + l.acc);
-      const float* add = via ? (p > 0 ? acc : nullptr) : (c.dw_f32 && (p > 0 || c.accumulate) ? (const float*)c.dw : nullptr);
-      void* out = via && !last ? (void*)acc : (void*)c.dw;
-      const int64_t ldo = via && !last ? c.D : c.lddw, ldadd = via ? c.D : c.lddw;
-      const int f32 = via ? !last : c.dw_f32;
-      if (l.splits_w > 1) { d.C = c.ws + l.slabs; d.ldc = c.D; d.c_f32 = 1; d.slab = (int64_t)c.V * c.D; }
-      else { d.C = out; d.ldc = ldo; d.c_f32 = f32; d.add = add; d.ldadd = ldadd; }
+      d.add = via ? (p > 0 ? acc : nullptr) : (c.dw_f32 && (p > 0 || c.accumulate) ? (const float*)c.dw : nullptr);
+      d.ldadd = via ? c.D : c.lddw;
+      d.C = via && !last ? (void*)acc : (void*)c.dw;
+      d.ldc = via && !last ? c.D : c.lddw;
+      d.c_f32 = via ? !last : c.dw_f32;
       lce_launch<E, LCE_DW>(d, l.tile_w, st);
-      if (l.splits_w > 1)
-        hipLaunchKernelGGL(lce_fold_kernel<E>, dim3(dpc_grid((int64_t)c.V * c.D / 4, 256)), dim3(256), 0, st, (const float*)(c.ws + l.slabs),
-                           (int64_t)c.V * c.D, l.splits_w, c.V, c.D, head, add, ldadd, out, ldo, f32);
     }
   }
   return DPC_OK;
@@ -789,12 +875,6 @@ static dpc_gemm_desc lce_desc(int M, int N, int K, const float* A, int64_t a_rs,
   d.C = C; d.ldc = ldc; d.splitk = 1;
   return d;
 }
-static int lce_gemm(int M, int N, int K, const float* A, int64_t a_rs, int64_t a_cs, const float* B, int64_t b_rs, int64_t b_cs, float beta,
-                    float* C, int64_t ldc, hipStream_t st) {
-  const dpc_gemm_desc d = lce_desc(M, N, K, A, a_rs, a_cs, B, b_rs, b_cs, beta, C, ldc);
-  return dpc_gemm_f32_ex(&d, 1, st);
-}
-
 static int lce_full(const LceCall& c, const LceLayout& l, hipStream_t st) {
   float* head = (float*)c.ws;
   const bool grads = c.dh || c.dw;
@@ -805,33 +885,38 @@ static int lce_full(const LceCall& c, const LceLayout& l, hipStream_t st) {
     const float* w = (const float*)c.w;
     float* P = (float*)(c.ws + l.P);
     float* hm = (float*)(c.ws + l.hm);
-    int rc = lce_gemm(rows, c.V, c.D, h, c.ldh, 1, w, 1, c.ldw, 0.f, P, c.V, st);
-    if (rc != DPC_OK) return rc;
+    const int segs = (int)dpc_cdiv(c.V, LCE_SEG);
     LceRowArgs ra;
     memset(&ra, 0, sizeof(ra));
-    ra.rows = rows; ra.V = c.V; ra.target = c.target + r0; ra.ignore = c.ignore; ra.loss = c.loss + r0; ra.lse = c.lse ? c.lse + r0 : nullptr;
-    hipLaunchKernelGGL(lce_rows_f32_kernel, dim3(rows), dim3(256), 0, st, P, (int64_t)c.V, ra, grads ? head : nullptr, h, c.ldh,
-                       c.dw ? hm : nullptr, c.D);
+    ra.stat = (f32x2*)(c.ws + l.stat); ra.prow = l.prow; ra.slabs = segs; ra.rows = rows; ra.V = c.V; ra.lt = (float*)(c.ws + l.lt);
+    ra.target = c.target + r0; ra.ignore = c.ignore; ra.loss = c.loss + r0; ra.lse = c.lse ? c.lse + r0 : nullptr;
+    ra.live = grads ? (f32x2*)(c.ws + l.live) : nullptr; ra.pm1 = (float*)(c.ws + l.pm1);
+    // (64 x 64 tiles below 768 of 128 x 128: 500 x 18000 x 256 56 against 71 us; 4000 x 4000 x 512 166 against 162)
+    dpc_gemm_desc lg = lce_desc(rows, c.V, c.D, h, c.ldh, 1, w, 1, c.ldw, 0.f, P, l.ldp);
+    lg.tile = lce_tiles(rows, c.V, 128, 128) < 768 ? 64 : 128;
+    int rc = dpc_gemm_f32_ex(&lg, 1, st);
+    if (rc != DPC_OK) return rc;
+    hipLaunchKernelGGL(lce_stat_f32_kernel, dim3((unsigned)segs * rows), dim3(256), 0, st, P, l.ldp, c.V, ra.target, (f32x2*)(c.ws + l.stat), l.prow,
+                       (float*)(c.ws + l.lt));
+    hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)dpc_cdiv(rows, 16)), dim3(1024), 0, st, ra);
+    if (!grads) continue;
+    hipLaunchKernelGGL(lce_d_f32_kernel, dim3((unsigned)segs * rows), dim3(256), 0, st, P, l.ldp, c.V, ra.target, ra.live, ra.pm1, head);
     if (c.dh) {
       float* dh = (float*)c.dh + r0 * c.lddh;
-      if (l.splits_h > 1) {
-        float* slabs = (float*)(c.ws + l.slabs);
-        const int64_t slab = (int64_t)rows * c.D;
-        const int chunk = (int)lce_up(dpc_cdiv(c.V, l.splits_h), 32);
-        dpc_gemm_desc d[64];
-        int n = 0;
-        for (int k = 0; k < c.V; k += chunk, ++n)
-          d[n] = lce_desc(rows, c.D, c.V - k < chunk ? c.V - k : chunk, P + k, c.V, 1, w + k * c.ldw, c.ldw, 1, 0.f, slabs + n * slab, c.D);
-        rc = dpc_gemm_f32_group(d, n, st);
-        if (rc != DPC_OK) return rc;
-        hipLaunchKernelGGL(lce_fold_f32_kernel, dim3(dpc_grid(slab, 256)), dim3(256), 0, st, slabs, slab, n, (int64_t)rows, c.D, dh, c.lddh);
-      } else {
-        rc = lce_gemm(rows, c.D, c.V, P, c.V, 1, w, c.ldw, 1, 0.f, dh, c.lddh, st);
-        if (rc != DPC_OK) return rc;
-      }
+      const bool cut = l.splits > 1;
+      dpc_gemm_desc d = lce_desc(rows, c.D, c.V, P, l.ldp, 1, w, c.ldw, 1, 0.f, cut ? (float*)(c.ws + l.part) : dh, cut ? c.D : c.lddh);
+      if (cut) { d.splitk = l.splits; d.tile = 64; d.split_slab = (int64_t)rows * c.D; }
+      rc = dpc_gemm_f32_ex(&d, 1, st);
+      if (rc != DPC_OK) return rc;
+      if (cut)
+        hipLaunchKernelGGL(lce_fold_f32_kernel, dim3(dpc_grid(d.split_slab, 256)), dim3(256), 0, st, (const float*)(c.ws + l.part), d.split_slab, l.splits,
+                           c.D, dh, c.lddh);
     }
     if (c.dw) {
-      rc = lce_gemm(c.V, c.D, rows, P, 1, c.V, hm, c.D, 1, p > 0 || c.accumulate ? 1.f : 0.f, (float*)c.dw, c.lddw, st);
+      hipLaunchKernelGGL(lce_mask_rows_f32_kernel, dim3(dpc_grid((int64_t)rows * c.D, 256)), dim3(256), 0, st, h, c.ldh, (int64_t)rows * c.D, c.D,
+                         ra.live, hm);
+      const dpc_gemm_desc d = lce_desc(c.V, c.D, rows, P, 1, l.ldp, hm, c.D, 1, p > 0 || c.accumulate ? 1.f : 0.f, (float*)c.dw, c.lddw);
+      rc = dpc_gemm_f32_ex(&d, 1, st);
       if (rc != DPC_OK) return rc;
     }
   }
@@ -857,7 +942,8 @@ extern "C" int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* 
   DPC_CHECK_ARG(((uintptr_t)ws & 255) == 0, "linear_cross_entropy: the workspace must be 256-byte aligned");
   const bool grads = dh || dw;
   if (piece_rows <= 0) piece_rows = lce_rows_default(T, D, V, dtype, grads, !f32 && !dw_f32);
-  DPC_CHECK_ARG(dpc_cdiv(V, 256) * dpc_cdiv(piece_rows < T ? piece_rows : T, 256) * 32 < (1ll << 31), "linear_cross_entropy: the piece is too large");
+  const int64_t most = piece_rows < T ? piece_rows : T;
+  DPC_CHECK_ARG(dpc_cdiv(V, 64) * dpc_cdiv(most, 64) < (1ll << 30) && dpc_cdiv(V, LCE_SEG) * most < (1ll << 31), "linear_cross_entropy: the piece is too large");
   DPC_CHECK_ARG(f32 || !grads || piece_rows <= (1 << 21) || T <= (1 << 21), "linear_cross_entropy: the piece is too large");
   const LceLayout l = lce_layout(T, D, V, dtype, grads, !f32 && !dw_f32, piece_rows);
   DPC_CHECK_ARG(ws_bytes >= l.bytes, "linear_cross_entropy: the workspace is smaller than dpc_linear_cross_entropy_ws says");
@@ -867,7 +953,7 @@ extern "C" int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* 
   c.D = D; c.V = V; c.loss = loss; c.lse = lse; c.total = total; c.dh = (char*)dh; c.lddh = lddh; c.dw = (char*)dw; c.lddw = lddw;
   c.dw_f32 = dw_f32 || f32; c.accumulate = accumulate; c.gscale = gscale; c.mean = mean; c.ws = (char*)ws;
   const float lift = dtype == DPC_F16 ? Half<_Float16>::kUp : 1.f;
-  if (grads) hipLaunchKernelGGL(lce_begin_kernel, dim3(1), dim3(1024), 0, st, target, T, ignore_index, V, mean, gscale, lift, (float*)ws);
+  if (grads) hipLaunchKernelGGL(lce_begin_kernel, dim3(1), dim3(1024), 0, st, target, T, ignore_index, mean, gscale, lift, (float*)ws);
   if (T == 0 && dw && !accumulate)
     hipLaunchKernelGGL(lce_zero_kernel, dim3(dpc_grid((int64_t)V * D, 256)), dim3(256), 0, st, (uint16_t*)dw, c.dw_f32 ? 2 * lddw : lddw, (int64_t)V,
                        c.dw_f32 ? 2 * D : D);

@@ -99,7 +99,7 @@ class GemmDesc(ctypes.Structure):
                 ('bn_z', ctypes.c_void_p), ('ld_bn_z', ctypes.c_int64), ('bn_mean', ctypes.c_void_p),
                 ('bn_invstd', ctypes.c_void_p), ('stat_n', ctypes.c_int32), ('stat_slots', ctypes.c_int32),
                 ('seed_out', ctypes.c_void_p), ('ld_seed', ctypes.c_int64), ('seed_row', ctypes.c_void_p),
-                ('seed_col', ctypes.c_void_p)]
+                ('seed_col', ctypes.c_void_p), ('split_slab', ctypes.c_int64)]
 
 
 def _addr(t):

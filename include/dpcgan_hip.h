@@ -134,6 +134,9 @@ typedef struct dpc_gemm_desc {
    * hidden layer the seed of the backward chain, rowscale * w_head * slope (what dpc_disc_out_fwd's `delta` is):
    * the chain's first product can then follow the forward product directly (dp_cgan.py:629-631,652-655) */
   float* seed_out; int64_t ld_seed; const float* seed_row; const float* seed_col;
+  /* with splitk = n > 1, tile = 64, beta 0 and no epilogue: != 0 stores the n partial products at C + s * split_slab
+   * instead of adding them up with atomics (the caller sums them, in an order of its own) */
+  int64_t split_slab;
 } dpc_gemm_desc;
 /* `count` (1..64) products, descriptors in host memory, issued in order on `stream`.  The library keeps no
  * GEMM state: two callers in one process cannot disturb each other's tiling or reproducibility. */

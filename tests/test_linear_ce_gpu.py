@@ -324,6 +324,51 @@ def test_a_vocabulary_of_many_tiles(ops):
     check(call(ops, h, w, target), Oracle(h, w, target))
 
 
+def test_a_vocabulary_of_millions(ops):
+    """More slabs than a grid's second dimension holds; three rows."""
+    T, D, V = 3, 8, 4200011
+    h, w, target = inputs(T, D, V, torch.bfloat16, 14, ignored=0.0)
+    target[1] = V - 1
+    check(call(ops, h, w, target), Oracle(h, w, target))
+    check(call(ops, h.float(), w.float(), target), Oracle(h.float(), w.float(), target))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('offset', [0, 200])
+def test_sure_rows_keep_a_small_loss(ops, dtype, offset):
+    """Rows whose target leads by 13 to 21: the small loss comes from the sum and not from the difference of two numbers of
+    the logits' size.  The logits are exact here.  The sum is 1 and little beside it: a rounding of at most u each for
+    the leading term's exponential (its hardware's last bit: 2), up to 8 additions in a thread's run, 2 that join four
+    runs, 2 across the lanes of a row or 8 across a block, 6 that join the slabs with 2 factors each, the logarithm and
+    the last product (4): 40 u in all.  The others' exponents are off by at most 2 * 32 u of their own: u of the loss
+    times 64.  (The difference of two logarithms near 221 is off by up to 221 u, which the second offset would show.)"""
+    T, D, V = 64, 64, 1000
+    g = torch.Generator(device=DEV).manual_seed(15)
+    w = torch.zeros(V, D, device=DEV)
+    w[:D] = 4 * torch.eye(D, device=DEV)                     # logits 4 h, exact in every type
+    target = torch.arange(T, device=DEV)
+    h = torch.zeros(T, D, device=DEV)
+    lead = torch.linspace(13, 21, T, device=DEV).round(decimals=0)
+    h[target, target] = lead / 4
+    if offset:
+        h, w = torch.cat([h, torch.zeros(T, 8, device=DEV)], 1), torch.cat([w, torch.zeros(V, 8, device=DEV)], 1)
+        h[:, D], w[:, D] = offset, 1
+    h, w = h.to(dtype), w.to(dtype)
+    o = call(ops, h, w, target)
+    l = h.double() @ w.double().t()
+    loss = torch.logsumexp(l, 1) - l[target, target]
+    assert float(loss.min()) < 1e-5 * 1000
+    assert ((o['loss'].double() - loss).abs() <= 40 * U + 64 * U * loss).all()
+    d = torch.softmax(l, 1)
+    pm1 = torch.expm1(-loss) / T
+    got = o['dw'][target].double() if dtype == torch.float32 else None
+    if got is not None:                                       # dW's row t, column t: (p_t - 1) h, and the other rows' share
+        want = (d.t() @ h.double() / T)[:T]
+        want += (pm1 - d[target, target] / T)[:, None] * h.double()
+        # (the loss's own error in p_t - 1, and the softmax's)
+        assert ((got - want).abs() <= (40 * U + 64 * U * loss)[:, None] * h.double().abs() / T + 128 * U * (d.t() @ h.double().abs() / T)[:T]).all()
+
+
 def test_refusals(ops):
     z = lambda *s, t=torch.bfloat16: torch.zeros(*s, dtype=t, device=DEV)  # noqa: E731
     T, D, V = 16, 64, 100
