@@ -428,16 +428,6 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
 }
 
 // ---- the passes between the products --------------------------------------------------------------------------------
-// head[0] = alpha = gscale / (rows that count, or 1) / lift
-__global__ __launch_bounds__(1024) void lce_begin_kernel(const int64_t* target, int64_t T, int64_t ignore, int mean, float gscale, float lift, float* head) {
-  __shared__ int red[16];
-  int c = 0;
-  if (mean)
-    for (int64_t i = threadIdx.x; i < T; i += 1024) c += target[i] != ignore;
-  c = dpc_block_sum(c, red);
-  if (threadIdx.x == 0) head[0] = gscale / (mean ? (float)max(c, 1) : 1.f) / lift;
-}
-
 // Two (reference, sum) pairs of a row as one.  (A sum of 0 - all logits -inf - leaves the other as it is.)
 __device__ __forceinline__ f32x2 lce_join(f32x2 x, f32x2 y) {
   if (x.y == 0.f) return y;
@@ -454,9 +444,28 @@ struct LceRowArgs {
   float* loss; float* lse;      // lse nullable
   f32x2* live;                  // (reference, 1 / sum) of a row, (0, 0) where it takes no part in the gradient; nullable
   float* pm1;                   // p_t - 1
+  // one block more: *alpha = scale / (rows of the whole call that count, or 1)
+  float* alpha; float scale; int mean; const int64_t* all; int64_t T;
+  float* total;                 // of a call that is one block: the mean (or sum) of the losses; nullable
 };
+// (sum, count) of the losses over the block -> total
+__device__ __forceinline__ void lce_total(double s, int c, int mean, float* total) {
+  __shared__ double red[16];
+  __shared__ int redi[16];
+  s = dpc_block_sum(s, red);
+  c = dpc_block_sum(c, redi);
+  if (threadIdx.x == 0) total[0] = (float)(s / (mean ? (double)max(c, 1) : 1.0));
+}
 __global__ __launch_bounds__(1024) void lce_rows_kernel(LceRowArgs a) {
   __shared__ f32x2 red[64][16];
+  if (a.alpha && blockIdx.x + 1 == gridDim.x) {
+    int c = 0;
+    if (a.mean)
+      for (int64_t i = threadIdx.x; i < a.T; i += 1024) c += a.all[i] != a.ignore;
+    c = dpc_block_sum(c, reinterpret_cast<int*>(red));
+    if (threadIdx.x == 0) a.alpha[0] = a.scale / (a.mean ? (float)max(c, 1) : 1.f);
+    return;
+  }
   const int r = threadIdx.x & 15, w = threadIdx.x >> 4;
   const int n = blockIdx.x * 16 + r;
   f32x2 x = {0.f, 0.f};
@@ -469,26 +478,44 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(LceRowArgs a) {
     __syncthreads();
     if (w < k) red[w][r] = x = lce_join(x, red[w + k][r]);
   }
-  if (w != 0 || n >= a.rows) return;
-  const int64_t t = a.target[n];
-  const bool off = t == a.ignore, bad = !off && (t < 0 || t >= a.V);
-  // The loss from what is exact near it: where the target is the row's largest logit the difference of the references is the
-  // rounding of one product, and the loss the logarithm of the sum - not the difference of two numbers of the logits' size.
-  const float l2 = log2f(x.y);
-  const float loss = off ? 0.f : (bad ? NAN : LCE_LN2 * (fmaf(-a.lt[n], LCE_LOG2E, x.x) + l2));
-  a.loss[n] = loss;
-  if (a.lse) a.lse[n] = LCE_LN2 * (x.x + l2);
-  if (a.live) {
-    a.live[n] = off || bad ? f32x2{0.f, 0.f} : f32x2{x.x, 1.f / x.y};
-    a.pm1[n] = off || bad ? 0.f : expm1f(-loss);
+  double sum = 0.0;
+  int count = 0;
+  if (w == 0 && n < a.rows) {
+    const int64_t t = a.target[n];
+    const bool off = t == a.ignore, bad = !off && (t < 0 || t >= a.V);
+    // The loss from what is exact near it: where the target is the row's largest logit the difference of the references is
+    // the rounding of one product, and the loss the logarithm of the sum - not the difference of two numbers of the logits' size.
+    const float l2 = log2f(x.y);
+    const float loss = off ? 0.f : (bad ? NAN : LCE_LN2 * (fmaf(-a.lt[n], LCE_LOG2E, x.x) + l2));
+    a.loss[n] = loss;
+    if (a.lse) a.lse[n] = LCE_LN2 * (x.x + l2);
+    if (a.live) {
+      a.live[n] = off || bad ? f32x2{0.f, 0.f} : f32x2{x.x, 1.f / x.y};
+      a.pm1[n] = off || bad ? 0.f : expm1f(-loss);
+    }
+    sum = (double)loss;
+    count = !off;
   }
+  if (a.total) lce_total(sum, count, a.mean, a.total);
 }
 
 // P from e^(l - slab max) in fp16 to d in the operands' type, in place.  One thread per row and slab.
 // NT: P is much larger than the 256 MB of the last-level cache - read and written past it (2 GB: 846 -> 780 us; 0.3 GB: 96 -> 103 us).
+// Blocks from `slabs` * prow / 256 on copy h with its ignored rows, and the rows up to the end of the piece's last tile, set to
+// 0: what such a row holds must not reach dW (0 x NaN).
 template <typename E, bool NT>
-__global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, const f32x2* stat, int rows, int slab_rows, const f32x2* live,
-                                                        const float* pm1, const int64_t* target) {
+__global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, const f32x2* stat, int slabs, int rows, int slab_rows, const f32x2* live,
+                                                        const float* pm1, const int64_t* target, const char* h, int64_t ldh, int row16, char* hm) {
+  const int first = slabs * (int)(prow / 256);
+  if ((int)blockIdx.x >= first) {
+    for (int64_t i = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x; i < prow * row16; i += (int64_t)(gridDim.x - first) * 256) {
+      const int n = (int)(i / row16), c = (int)(i - (int64_t)n * row16);
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if (n < rows && live[n].y != 0.f) v = *reinterpret_cast<const u32x4*>(h + (int64_t)n * ldh + c * 16);
+      *reinterpret_cast<u32x4*>(hm + i * 16) = v;
+    }
+    return;
+  }
   const int nb = (int)(prow / 256), slab = blockIdx.x / nb, n = (blockIdx.x - slab * nb) * 256 + threadIdx.x;
   const f32x2 gl = n < rows ? live[n] : f32x2{0.f, 0.f};
   const bool on = gl.y != 0.f;                                         // (NaN is on: such a row keeps its NaN)
@@ -517,17 +544,6 @@ __global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, c
       if (NT) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, y), to);
       else *to = __builtin_bit_cast(u32x4, y);
     }
-  }
-}
-
-// h with its ignored rows, and the rows up to the end of the piece's last tile, set to 0: what such a row holds must
-// not reach dW (0 x NaN)
-__global__ __launch_bounds__(256) void lce_mask_rows_kernel(const char* h, int64_t ldh, int rows, int64_t total16, int row16, const f32x2* live, char* out) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total16; i += (int64_t)gridDim.x * 256) {
-    const int n = (int)(i / row16), c = (int)(i - (int64_t)n * row16);
-    u32x4 v = {0u, 0u, 0u, 0u};
-    if (n < rows && live[n].y != 0.f) v = *reinterpret_cast<const u32x4*>(h + (int64_t)n * ldh + c * 16);
-    *reinterpret_cast<u32x4*>(out + i * 16) = v;
   }
 }
 
@@ -592,9 +608,17 @@ __global__ __launch_bounds__(256) void lce_stat_f32_kernel(const float* logits, 
   }
 }
 
-// Logits to alpha * d, in place.
-__global__ __launch_bounds__(256) void lce_d_f32_kernel(float* logits, int64_t ld, int V, const int64_t* target, const f32x2* live, const float* pm1,
-                                                        const float* alpha) {
+// Logits to alpha * d, in place; the blocks behind them copy h with its ignored rows set to 0.
+__global__ __launch_bounds__(256) void lce_d_f32_kernel(float* logits, int64_t ld, int rows, int V, const int64_t* target, const f32x2* live, const float* pm1,
+                                                        const float* alpha, const float* h, int64_t ldh, int D, float* hm) {
+  const int first = rows * ((V + LCE_SEG - 1) / LCE_SEG);
+  if ((int)blockIdx.x >= first) {
+    for (int64_t i = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x; i < (int64_t)rows * D; i += (int64_t)(gridDim.x - first) * 256) {
+      const int64_t n = i / D;
+      hm[i] = live[n].y != 0.f ? h[n * ldh + (i - n * D)] : 0.f;
+    }
+    return;
+  }
   const int segs = (V + LCE_SEG - 1) / LCE_SEG, n = blockIdx.x / segs, seg = blockIdx.x - n * segs;
   const f32x2 gl = live[n];
   const bool on = gl.y != 0.f;
@@ -609,14 +633,6 @@ __global__ __launch_bounds__(256) void lce_d_f32_kernel(float* logits, int64_t l
 #pragma unroll
     for (int e = 0; e < 4; ++e) q[e] = on ? (v + e == t ? pt : f * __builtin_amdgcn_exp2f(fmaf(q[e], LCE_LOG2E, -gl.x))) : 0.f;
     *reinterpret_cast<f32x4*>(x + v) = q;
-  }
-}
-
-// h with its ignored rows set to 0
-__global__ __launch_bounds__(256) void lce_mask_rows_f32_kernel(const float* h, int64_t ldh, int64_t total, int D, const f32x2* live, float* out) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t n = i / D;
-    out[i] = live[n].y != 0.f ? h[n * ldh + (i - n * D)] : 0.f;
   }
 }
 
@@ -641,17 +657,14 @@ __global__ __launch_bounds__(256) void lce_zero_kernel(uint16_t* out, int64_t ld
 
 // sum of the rows' losses, over the rows that count if `mean` (one block, fixed order)
 __global__ __launch_bounds__(1024) void lce_total_kernel(const float* loss, const int64_t* target, int64_t T, int64_t ignore, int mean, float* total) {
-  __shared__ double red[16];
-  __shared__ int redi[16];
   double s = 0.0;
   int c = 0;
+#pragma unroll 8
   for (int64_t i = threadIdx.x; i < T; i += 1024) {
     s += (double)loss[i];
     c += target[i] != ignore;
   }
-  s = dpc_block_sum(s, red);
-  c = dpc_block_sum(c, redi);
-  if (threadIdx.x == 0) total[0] = (float)(s / (mean ? (double)max(c, 1) : 1.0));
+  lce_total(s, c, mean, total);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
@@ -814,6 +827,16 @@ struct LceCall {
   char* ws;
 };
 
+// Rows of a piece: with the first one's the call's alpha, and the total where one block sees all rows.
+static void lce_rows(const LceCall& c, LceRowArgs& a, int piece, const LceLayout& l, hipStream_t st) {
+  const bool begin = piece == 0 && (c.dh || c.dw);
+  a.alpha = begin ? (float*)c.ws : nullptr;
+  a.scale = c.dtype == DPC_F16 ? c.gscale / Half<_Float16>::kUp : c.gscale;
+  a.mean = c.mean; a.all = c.target; a.T = c.T;
+  a.total = c.T <= 16 && l.pieces == 1 ? c.total : nullptr;
+  hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)dpc_cdiv(a.rows, 16) + begin), dim3(1024), 0, st, a);
+}
+
 template <typename E>
 static int lce_half(const LceCall& c, const LceLayout& l, hipStream_t st) {
   float* head = (float*)c.ws;
@@ -834,11 +857,13 @@ static int lce_half(const LceCall& c, const LceLayout& l, hipStream_t st) {
     ra.stat = g.stat; ra.prow = l.prow; ra.slabs = slabs; ra.rows = rows; ra.V = c.V; ra.lt = g.lt; ra.target = g.target; ra.ignore = c.ignore;
     ra.loss = c.loss + r0; ra.lse = c.lse ? c.lse + r0 : nullptr;
     ra.live = grads ? (f32x2*)(c.ws + l.live) : nullptr; ra.pm1 = (float*)(c.ws + l.pm1);
-    hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)dpc_cdiv(rows, 16)), dim3(1024), 0, st, ra);
+    lce_rows(c, ra, p, l, st);
     if (!grads) continue;
     const auto scale = lce_up(c.V, 256) * l.prow * 2 > (1ll << 30) ? lce_scale_kernel<E, true> : lce_scale_kernel<E, false>;
-    hipLaunchKernelGGL(scale, dim3((unsigned)(l.prow / 256 * slabs)), dim3(256), 0, st, g.P, l.prow, g.stat, rows, slab_rows, ra.live, ra.pm1,
-                       g.target);
+    const int row16 = c.D / 8, copies = c.dw ? dpc_grid(l.prow * row16, 256) : 0;
+    char* hm = c.ws + l.hm;
+    hipLaunchKernelGGL(scale, dim3((unsigned)(l.prow / 256 * slabs + copies)), dim3(256), 0, st, g.P, l.prow, g.stat, slabs, rows, slab_rows, ra.live,
+                       ra.pm1, g.target, h, c.ldh * 2, row16, hm);
     if (c.dh) {
       LceArgs d = g;
       d.A = c.w; d.lda = c.ldw * 2; d.M = c.D; d.N = rows; d.K = c.V;
@@ -846,10 +871,6 @@ static int lce_half(const LceCall& c, const LceLayout& l, hipStream_t st) {
       lce_launch<E, LCE_DH>(d, l.tile_h, st);
     }
     if (c.dw) {
-      const int64_t row16 = c.D / 8;
-      char* hm = c.ws + l.hm;
-      hipLaunchKernelGGL(lce_mask_rows_kernel, dim3(dpc_grid(l.prow * row16, 256)), dim3(256), 0, st, h, c.ldh * 2, rows, l.prow * row16, (int)row16,
-                         ra.live, hm);
       LceArgs d = g;
       d.A = hm; d.lda = (int64_t)c.D * 2; d.M = c.D; d.N = c.V; d.K = (int)lce_up(rows, LCE_BK); d.part = (float*)(c.ws + l.part);
       // where the piece's share goes: dW itself, or the fp32 sums over the pieces until the last one
@@ -898,9 +919,11 @@ static int lce_full(const LceCall& c, const LceLayout& l, hipStream_t st) {
     if (rc != DPC_OK) return rc;
     hipLaunchKernelGGL(lce_stat_f32_kernel, dim3((unsigned)segs * rows), dim3(256), 0, st, P, l.ldp, c.V, ra.target, (f32x2*)(c.ws + l.stat), l.prow,
                        (float*)(c.ws + l.lt));
-    hipLaunchKernelGGL(lce_rows_kernel, dim3((unsigned)dpc_cdiv(rows, 16)), dim3(1024), 0, st, ra);
+    lce_rows(c, ra, p, l, st);
     if (!grads) continue;
-    hipLaunchKernelGGL(lce_d_f32_kernel, dim3((unsigned)segs * rows), dim3(256), 0, st, P, l.ldp, c.V, ra.target, ra.live, ra.pm1, head);
+    const int copies = c.dw ? dpc_grid((int64_t)rows * c.D, 256) : 0;
+    hipLaunchKernelGGL(lce_d_f32_kernel, dim3((unsigned)segs * rows + copies), dim3(256), 0, st, P, l.ldp, rows, c.V, ra.target, ra.live, ra.pm1, head, h,
+                       c.ldh, c.D, hm);
     if (c.dh) {
       float* dh = (float*)c.dh + r0 * c.lddh;
       const bool cut = l.splits > 1;
@@ -913,8 +936,6 @@ static int lce_full(const LceCall& c, const LceLayout& l, hipStream_t st) {
                            c.D, dh, c.lddh);
     }
     if (c.dw) {
-      hipLaunchKernelGGL(lce_mask_rows_f32_kernel, dim3(dpc_grid((int64_t)rows * c.D, 256)), dim3(256), 0, st, h, c.ldh, (int64_t)rows * c.D, c.D,
-                         ra.live, hm);
       const dpc_gemm_desc d = lce_desc(c.V, c.D, rows, P, 1, l.ldp, hm, c.D, 1, p > 0 || c.accumulate ? 1.f : 0.f, (float*)c.dw, c.lddw);
       rc = dpc_gemm_f32_ex(&d, 1, st);
       if (rc != DPC_OK) return rc;
@@ -952,14 +973,12 @@ extern "C" int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* 
   c.h = (const char*)h; c.ldh = ldh; c.w = (const char*)w; c.ldw = ldw; c.dtype = dtype; c.target = target; c.ignore = ignore_index; c.T = T;
   c.D = D; c.V = V; c.loss = loss; c.lse = lse; c.total = total; c.dh = (char*)dh; c.lddh = lddh; c.dw = (char*)dw; c.lddw = lddw;
   c.dw_f32 = dw_f32 || f32; c.accumulate = accumulate; c.gscale = gscale; c.mean = mean; c.ws = (char*)ws;
-  const float lift = dtype == DPC_F16 ? Half<_Float16>::kUp : 1.f;
-  if (grads) hipLaunchKernelGGL(lce_begin_kernel, dim3(1), dim3(1024), 0, st, target, T, ignore_index, mean, gscale, lift, (float*)ws);
   if (T == 0 && dw && !accumulate)
     hipLaunchKernelGGL(lce_zero_kernel, dim3(dpc_grid((int64_t)V * D, 256)), dim3(256), 0, st, (uint16_t*)dw, c.dw_f32 ? 2 * lddw : lddw, (int64_t)V,
                        c.dw_f32 ? 2 * D : D);
   const int rc = T == 0 ? DPC_OK : f32 ? lce_full(c, l, st) : (dtype == DPC_BF16 ? lce_half<__bf16>(c, l, st) : lce_half<_Float16>(c, l, st));
   if (rc != DPC_OK) return rc;
-  if (total) hipLaunchKernelGGL(lce_total_kernel, dim3(1), dim3(1024), 0, st, loss, target, T, ignore_index, mean, total);
+  if (total && (T == 0 || T > 16 || l.pieces > 1)) hipLaunchKernelGGL(lce_total_kernel, dim3(1), dim3(1024), 0, st, loss, target, T, ignore_index, mean, total);
   DPC_LAUNCH_CHECK();
   return DPC_OK;
 }
