@@ -30,10 +30,10 @@ struct MtRec {
   int32_t vec;                          // 8-element accesses are aligned in every buffer
   int32_t pad;
 };
-// Chunk b of a plan: elements [start, start + chunk) of tensor t.
+// Chunk b of a plan: elements [start, start + MT_SUB) of tensor t.
 struct MtChunk { int32_t t; int32_t pad; int64_t start; };
 
-struct MtPlan { const MtRec* rec; const MtChunk* chunk; int blocks; int chunk_len; };
+struct MtPlan { const MtRec* rec; const MtChunk* chunk; int blocks; };
 
 static int64_t mt_align(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
@@ -101,18 +101,35 @@ __device__ __forceinline__ void mt_store(void* base, int64_t i, int type, int le
 // ---- global norm ---------------------------------------------------------------------------------------------------
 // sum of g^2 in fp64 (the square of an fp32 gradient overflows at 2e19 and vanishes below 1e-23): one partial per
 // block, chunks b, b + gridDim, ... in that order, so the sum does not depend on which block ends first.
+// NT: the gradients are larger than the 256 MB of the last-level cache and are read past it.
+template <bool NT>
+__device__ __forceinline__ Raw8 mt_load_norm(const MtRec& r, int64_t i, int64_t end, bool full) {
+  if (!full) return mt_load<false>(r.g, i, r.g_t, (int)max((int64_t)0, min((int64_t)8, end - i)));
+  Raw8 o = {u32x4{0u, 0u, 0u, 0u}, u32x4{0u, 0u, 0u, 0u}};
+  const u32x4* q = reinterpret_cast<const u32x4*>((const char*)r.g + i * (r.g_t == DPC_F32 ? 4 : 2));
+  o.a = NT ? __builtin_nontemporal_load(q) : q[0];
+  if (r.g_t == DPC_F32) o.b = NT ? __builtin_nontemporal_load(q + 1) : q[1];
+  return o;
+}
+template <bool NT>
 __global__ __launch_bounds__(256) void grad_sumsq_kernel(MtPlan pl, double* part) {
   __shared__ double red[16];
   double s = 0.0;
-  for (int c = blockIdx.x; c < pl.blocks; c += gridDim.x) {
-    const MtChunk ch = pl.chunk[c];
-    const MtRec r = pl.rec[ch.t];
-    const int64_t end = min(ch.start + (int64_t)pl.chunk_len, r.n);
-    for (int64_t at = ch.start; at < end; at += MT_SUB) {
-      const int64_t i = at + 8 * threadIdx.x;
-      const int left = (int)max((int64_t)0, min((int64_t)8, end - i));
-      const bool full = r.vec && end - at >= MT_SUB;
-      const f32x8 g = mt_float(full ? mt_load<true>(r.g, i, r.g_t, 8) : mt_load<false>(r.g, i, r.g_t, left), r.g_t);
+  // four chunks at a time: their loads are in flight together
+  for (int c0 = blockIdx.x * 4; c0 < pl.blocks; c0 += gridDim.x * 4) {
+    Raw8 raw[4];
+    int type[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const MtChunk ch = pl.chunk[min(c0 + k, pl.blocks - 1)];
+      const MtRec r = pl.rec[ch.t];
+      const int64_t end = c0 + k < pl.blocks ? min(ch.start + MT_SUB, r.n) : ch.start;         // (past the last chunk: nothing of it)
+      type[k] = r.g_t;
+      raw[k] = mt_load_norm<NT>(r, ch.start + 8 * threadIdx.x, end, r.vec && end - ch.start >= MT_SUB);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const f32x8 g = mt_float(raw[k], type[k]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) s = fma((double)g[e], (double)g[e], s);
     }
@@ -156,7 +173,9 @@ __device__ __forceinline__ float adamw_param(const AdamwArgs& a, float p, float 
 
 // ---- 8-bit states.  The moments are updated in fp64 from what is held and rounded ONCE, to 4 significant bits, so what
 // is held is the exact rounding for the given random bits (an update in fp32 lands on the other side of a border for one
-// element in 10^6).
+// element in 10^6).  The vector units are what bounds this: every fp64 instruction here has been counted (205 -> @@ us for 66 M
+// parameters in bf16 with the hardware's reciprocal root in place of a library square root, and products with the scales
+// taken once per lane).
 struct Hold8 { double x[8]; };
 
 // y in [0, 448] to the e4m3 code below or above it, above where the fraction between them plus d / 65536 reaches 1: d is
@@ -169,13 +188,12 @@ __device__ __forceinline__ uint32_t mt_code8(double y, uint32_t d) {
   return ((hi + (d << 1)) >> 17) - (small ? ((1023u - 7u) << 3) + 8u : (1023u - 7u) << 3);
 }
 
-// sqrt(v) to 2^-45: the 1-ulp fp32 root and one Newton step in fp64.  v == 0 and the ends of the fp32 range (also
-// infinities and NaN) take the full routine.
+// sqrt(v) to 2^-46: the hardware's reciprocal root (2^-24, the whole range of fp64) and one Newton step.  0 for 0; NaN for
+// infinities and NaN, which are held as NaN anyway.
 __device__ __forceinline__ double mt_root(double v) {
-  if (!(v > 1e-30 && v < 1e30)) return sqrt(v);
-  const float r = __builtin_amdgcn_sqrtf((float)v);
-  const double rd = (double)r;
-  return fma(fma(-rd, rd, v), (double)(0.5f * __builtin_amdgcn_rcpf(r)), rd);
+  const double q = __builtin_amdgcn_rsq(fmax(v, 1e-300));
+  const double r = v * q;
+  return fma(fma(-r, r, v), 0.5 * q, r);
 }
 
 // Largest of a value over the 16 lanes that hold a state block (rotations inside a DPP row).
@@ -265,15 +283,18 @@ __device__ __forceinline__ void adamw_pass(const AdamwArgs& a, const MtRec& r, i
     uint32_t d[8];
     Hold8 m, rt;
     float odd = 0.f;
+    const double am = a.b1d * ms, ag = a.c1d * gs, bv = a.b2d * (vs * vs), bg = a.c2d * gs * gs;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       d[e] = (dw[e >> 1] >> (16 * (e & 1))) & 0xffffu;
-      const double ge = (double)g[e] * gs, re = (double)rf[e] * vs;
-      m.x[e] = a.b1d * ((double)mf[e] * ms) + a.c1d * ge;
-      rt.x[e] = mt_root(a.b2d * (re * re) + a.c2d * ge * ge);
+      const double ge = (double)g[e];
+      m.x[e] = fma((double)mf[e], am, ag * ge);
+      rt.x[e] = mt_root(fma((double)(rf[e] * rf[e]), bv, bg * ge * ge));           // (the square of a code is exact in fp32)
       const float m32 = (float)m.x[e], r32 = (float)rt.x[e];
-      odd += 0.f * m32 + 0.f * r32;                                    // NaN once a value is not finite
-      p[e] = adamw_param(a, p[e], m32, r32, keep, step_size, inv_bc2s);
+      odd = fmaf(m32, 0.f, fmaf(r32, 0.f, odd));                      // NaN once a value is not finite
+      // (1-ulp reciprocal, of the smallest normal number at least: the step is rounded to the parameter's last bit anyway)
+      const float den = r32 * inv_bc2s + a.eps;
+      p[e] = p[e] * keep - step_size * (m32 * __builtin_amdgcn_rcpf(den < 1.17549435e-38f ? 1.17549435e-38f : den));
     }
     if (__any(odd != 0.f)) {
       mt_hold8<FULL, false, true>(r.m, r.ms, i, left, m, d);
@@ -325,15 +346,12 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwArgs a) {
   }
   const double gs = (double)a.gscale * coef;
   const float keep = 1.f - a.lr * r.wd;
-  const int64_t end = min(ch.start + (int64_t)a.pl.chunk_len, r.n);
-  // (whole passes of the block, also where the tensor ends inside: the 16 lanes of a state block stay together)
-  for (int64_t at = ch.start; at < end; at += MT_SUB) {
-    const int64_t i = at + 8 * threadIdx.x;
-    if (r.vec && end - at >= MT_SUB)
-      adamw_pass<S8, true>(a, r, i, 8, gs, keep, step_size, inv_bc2s);
-    else
-      adamw_pass<S8, false>(a, r, i, (int)max((int64_t)0, min((int64_t)8, end - i)), gs, keep, step_size, inv_bc2s);
-  }
+  // (the block stays whole where the tensor ends inside it: so do the 16 lanes of a state block)
+  const int64_t i = ch.start + 8 * threadIdx.x;
+  if (r.vec && r.n - ch.start >= MT_SUB)
+    adamw_pass<S8, true>(a, r, i, 8, gs, keep, step_size, inv_bc2s);
+  else
+    adamw_pass<S8, false>(a, r, i, (int)max((int64_t)0, min((int64_t)8, r.n - i)), gs, keep, step_size, inv_bc2s);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
@@ -344,7 +362,7 @@ static bool mt_al(const void* p, int bytes) { return ((uintptr_t)p % (uintptr_t)
 
 static int mt_check(const dpc_multi_tensor* t, int count, dpc_multi_info* info) {
   DPC_CHECK_ARG(count >= 0 && (t || count == 0) && info, "multi_plan: null pointer or negative count");
-  int64_t total = 0;
+  int64_t grad_bytes = 0;
   int kinds = 0;
   for (int k = 0; k < count; ++k) {
     const dpc_multi_tensor& x = t[k];
@@ -364,17 +382,17 @@ static int mt_check(const dpc_multi_tensor* t, int count, dpc_multi_info* info) 
       DPC_CHECK_ARG(!x.m && !x.v && !x.copy && !x.m_scale && !x.v_scale, "multi_plan: states without a parameter");
       kinds |= 8;
     }
-    total += x.n;
+    grad_bytes += x.n * mt_size(x.g_type);
   }
   DPC_CHECK_ARG(kinds == 0 || kinds == 1 || kinds == 2 || kinds == 4 || kinds == 8,
                 "multi_plan: the tensors of a plan are of one kind (gradients only, 32-bit states, or 8-bit states with or without given random bits)");
-  // A chunk is one pass of a block while that gives a round of blocks or two (256 CUs x 8 blocks); beyond, four passes
-  // halve the blocks' own cost (record, step size) against the bytes they move.
-  info->chunk_len = total <= (int64_t)MT_SUB * 8192 ? MT_SUB : 4 * MT_SUB;
+  // (a chunk is one pass of a block: with two, four and eight the step of 404 M parameters took 2142, 2165 and 2214 us
+  // against 2114)
   int64_t blocks = 0;
-  for (int k = 0; k < count; ++k) blocks += dpc_cdiv(t[k].n, info->chunk_len);
+  for (int k = 0; k < count; ++k) blocks += dpc_cdiv(t[k].n, MT_SUB);
   DPC_CHECK_ARG(blocks < (1ll << 31), "multi_plan: too many elements");
   info->kind = kinds;
+  info->grad_bytes = grad_bytes;
   info->count = count;
   info->blocks = (int)blocks;
   info->rec_off = 0;
@@ -405,7 +423,7 @@ extern "C" int dpc_multi_plan(const dpc_multi_tensor* t, int count, const dpc_mu
     r.vec = mt_al(x.g, 16) && (!x.p || (mt_al(x.p, 16) && mt_al(x.m, x.m_scale ? 8 : 16) && mt_al(x.v, x.m_scale ? 8 : 16) &&
                                         mt_al(x.copy, 16) && mt_al(x.dither, 16)));
     draw += dpc_cdiv(x.n, 8);
-    for (int64_t s = 0; s < x.n; s += in.chunk_len) { chunk[b].t = k; chunk[b].start = s; ++b; }
+    for (int64_t s = 0; s < x.n; s += MT_SUB) { chunk[b].t = k; chunk[b].start = s; ++b; }
   }
   return DPC_OK;
 }
@@ -415,7 +433,6 @@ static MtPlan mt_view(const dpc_multi_info* info, const void* plan) {
   pl.rec = (const MtRec*)((const char*)plan + info->rec_off);
   pl.chunk = (const MtChunk*)((const char*)plan + info->chunk_off);
   pl.blocks = info->blocks;
-  pl.chunk_len = info->chunk_len;
   return pl;
 }
 
@@ -423,8 +440,10 @@ extern "C" int dpc_grad_clip(const dpc_multi_info* info, void* plan, double max_
   DPC_CHECK_ARG(info && plan && out, "grad_clip: null pointer");
   DPC_CHECK_ARG(max_norm > 0.0 && gscale > 0.0 && gscale <= 3.402823466e38, "grad_clip: max_norm and gscale must be positive");
   double* part = (double*)((char*)plan + info->part_off);
-  const int nb = info->blocks < MT_PARTS ? info->blocks : MT_PARTS;
-  if (nb > 0) hipLaunchKernelGGL(grad_sumsq_kernel, dim3(nb), dim3(256), 0, (hipStream_t)stream, mt_view(info, plan), part);
+  const int64_t quads = dpc_cdiv(info->blocks, 4);
+  const int nb = (int)(quads < MT_PARTS ? quads : MT_PARTS);
+  const auto sumsq = info->grad_bytes > (256ll << 20) ? grad_sumsq_kernel<true> : grad_sumsq_kernel<false>;
+  if (nb > 0) hipLaunchKernelGGL(sumsq, dim3(nb), dim3(256), 0, (hipStream_t)stream, mt_view(info, plan), part);
   hipLaunchKernelGGL(grad_clip_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, part, nb, max_norm, gscale, out, t_dev);
   DPC_LAUNCH_CHECK();
   return DPC_OK;

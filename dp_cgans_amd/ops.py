@@ -726,8 +726,8 @@ class MultiTensor(ctypes.Structure):
 class MultiInfo(ctypes.Structure):
     """dpc_multi_info of include/dpcgan_hip.h."""
     _fields_ = [('bytes', ctypes.c_int64), ('rec_off', ctypes.c_int64), ('chunk_off', ctypes.c_int64),
-                ('part_off', ctypes.c_int64), ('count', ctypes.c_int32), ('blocks', ctypes.c_int32),
-                ('chunk_len', ctypes.c_int32), ('kind', ctypes.c_int32)]
+                ('part_off', ctypes.c_int64), ('grad_bytes', ctypes.c_int64), ('count', ctypes.c_int32),
+                ('blocks', ctypes.c_int32), ('kind', ctypes.c_int32)]
 
 
 class MultiPlan(object):

@@ -493,8 +493,8 @@ typedef struct dpc_multi_tensor {
 } dpc_multi_tensor;
 /* Sizes of a plan (host struct, filled by dpc_multi_plan_size; the caller only reads `bytes`). */
 typedef struct dpc_multi_info {
-  int64_t bytes, rec_off, chunk_off, part_off;
-  int32_t count, blocks, chunk_len, kind;
+  int64_t bytes, rec_off, chunk_off, part_off, grad_bytes;
+  int32_t count, blocks, kind;
 } dpc_multi_info;
 /* A plan is built in host memory (t, info, plan: HOST pointers; nothing is launched) and copied by the caller into
  * `bytes` of 256-byte aligned device memory; it holds addresses, so it serves every step while the tensors stay where

@@ -38,7 +38,7 @@ def test_chunks_cover_every_tensor_once():
     got = {}
     for c in chunks:
         got.setdefault(c.t, []).append(c.start)
-    assert got == {k: list(range(0, n, info.chunk_len)) for k, n in enumerate(ns) if n}
+    assert got == {k: list(range(0, n, 2048)) for k, n in enumerate(ns) if n}
     assert info.part_off + 2048 * 8 == info.bytes and info.chunk_off + 16 * info.blocks <= info.part_off
 
 
