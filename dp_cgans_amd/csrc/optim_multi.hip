@@ -157,6 +157,7 @@ __global__ __launch_bounds__(256) void grad_clip_kernel(const double* part, int 
 struct AdamwArgs {
   MtPlan pl;
   float lr, b1, b2, c1, c2, eps;        // c = 1 - b, taken in fp64
+  float eps8;                           // eps, but a normal number
   double b1d, b2d, c1d, c2d;
   float step_size, inv_bc2s;            // lr / (1 - b1^t), 1 / sqrt(1 - b2^t) where the step count is the host's
   const float* coef; float gscale;
@@ -173,26 +174,19 @@ __device__ __forceinline__ float adamw_param(const AdamwArgs& a, float p, float 
 
 // ---- 8-bit states.  The moments are updated in fp64 from what is held and rounded ONCE, to 4 significant bits, so what
 // is held is the exact rounding for the given random bits (an update in fp32 lands on the other side of a border for one
-// element in 10^6).  The vector units are what bounds this: every fp64 instruction here has been counted (205 -> @@ us for 66 M
-// parameters in bf16 with the hardware's reciprocal root in place of a library square root, and products with the scales
-// taken once per lane).
+// element in 10^6).  The vector units bound this - the counters show them busy all the time - so it is written for few
+// instructions: 66 M parameters in bf16 took 205 us with a library square root and every case of the rounding per element,
+// 186 us with the hardware's reciprocal root, 156 us with the usual case on its own.
 struct Hold8 { double x[8]; };
 
-// y in [0, 448] to the e4m3 code below or above it, above where the fraction between them plus d / 65536 reaches 1: d is
-// added to the bits of the mantissa that go, its top bit on the highest of them.  Below 2^-6 the grid keeps its step of
-// 2^-9, as a mantissa does when 2^-6 (code 8) is added.
-__device__ __forceinline__ uint32_t mt_code8(double y, uint32_t d) {
-  const bool small = y < 0.015625;
-  const double z = small ? y + 0.015625 : y;
-  const uint32_t hi = (uint32_t)(__builtin_bit_cast(uint64_t, z) >> 32);
-  return ((hi + (d << 1)) >> 17) - (small ? ((1023u - 7u) << 3) + 8u : (1023u - 7u) << 3);
-}
+#define MT_ONE8 0x3f900000u      // high word of 2^-6, the smallest normal e4m3 number (code 8)
+#define MT_BIAS8 (1016u << 20)   // fp64's exponent bias less e4m3's, where the high word has its exponent
+#define MT_SOME 1e-300           // added to a second moment: 0 becomes a number with a root
 
-// sqrt(v) to 2^-46: the hardware's reciprocal root (2^-24, the whole range of fp64) and one Newton step.  0 for 0; NaN for
-// infinities and NaN, which are held as NaN anyway.
+// sqrt(v) to 2^-46, v >= MT_SOME: the hardware's reciprocal root (2^-24, the whole range of fp64) and one Newton step.
+// NaN for infinities and NaN, which are held as NaN anyway.
 __device__ __forceinline__ double mt_root(double v) {
-  const double q = __builtin_amdgcn_rsq(fmax(v, 1e-300));
-  const double r = v * q;
+  const double q = __builtin_amdgcn_rsq(v), r = v * q;
   return fma(fma(-r, r, v), 0.5 * q, r);
 }
 
@@ -226,30 +220,63 @@ __device__ __forceinline__ f32x8 mt_float8(u32x2 q) {
   return f32x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
-// Hold the 8 values x of this lane, part of a 128-element block, in 8 bits.  The block's largest finite value is held as
-// 448, the largest e4m3 number; what is not finite (ODD: the wave has such a value), as NaN.  UP: a value that is not 0
-// is not held as 0 (a root held as 0 would divide its moment by eps alone).
-template <bool FULL, bool UP, bool ODD>
-__device__ __forceinline__ void mt_hold8(void* base, float* scales, int64_t i, int left, const Hold8& h, const uint32_t d[8]) {
-  const double most = 3.4028234663852886e38;
+// 448 / top a little up (2^-48): top times it is not below 448.
+__device__ __forceinline__ double mt_scale8(double top) {
+  double q = __builtin_amdgcn_rcp(top);
+  q = fma(fma(-top, q, 1.0), q, q);
+  q = fma(fma(-top, q, 1.0), q, q);
+  return q * (448.0 * (1.0 + 0x1p-48));
+}
+
+// Hold the 8 values x of this lane, part of a 128-element block, in 8 bits: the block's largest finite value as 448, the
+// largest e4m3 number; the others y = 448 x / largest as the code below or above, above where the fraction between them
+// plus d / 65536 reaches 1: 2 d (`d2`, less the exponents' biases) is added to the high word of the fp64 number, whose lowest
+// 17 bits go; the carry rounds up.  ROOT: the value is a square root, not negative, and not held as 0 unless it is 0 (a
+// root held as 0 would divide its moment by eps alone).
+// The usual case has normal numbers only.  `odd`: some value of this wave is not finite.
+template <bool FULL, bool ROOT>
+__device__ __forceinline__ void mt_hold8(void* base, float* scales, int64_t i, int left, const Hold8& h, const uint32_t d2[8], bool odd) {
   double top = 0.0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const double ax = fabs(h.x[e]);
-    top = fmax(top, ODD ? (ax <= most ? ax : 0.0) : ax);
-  }
-  top = fmax(mt_max16(top), 7.888609052210118e-31);                     // at least 2^-100: the fp32 scale stays normal
-  const double inv = 448.0 / top;
-  uint32_t q[2] = {0u, 0u};
+  for (int e = 0; e < 8; ++e) top = fmax(top, fabs(h.x[e]));
+  const double most = 3.4028234663852886e38, least = 7.888609052210118e-31;        // (at least 2^-100: the fp32 scale stays normal)
+  top = fmax(mt_max16(top), least);
+  double inv = mt_scale8(top);
+  uint32_t hi[8], low = ~0u;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const double ax = fabs(h.x[e]);
-    uint32_t c = mt_code8(ax * inv, d[e]);
-    c = ax == top ? 0x7eu : min(c, 0x7eu);
-    if (UP) c = max(c, ax > 0.0 ? 1u : 0u);
-    if (ODD) c = ax <= most ? c : 0x7fu;
-    c |= (uint32_t)(__builtin_bit_cast(uint64_t, h.x[e]) >> 56) & 0x80u;
-    q[e >> 2] |= c << (8 * (e & 3));
+    hi[e] = (uint32_t)(__builtin_bit_cast(uint64_t, fabs(h.x[e]) * inv) >> 32);
+    low = min(low, hi[e]);
+  }
+  uint32_t q[2] = {0u, 0u};
+  if (!__any(odd || low < MT_ONE8)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      uint32_t c = (hi[e] + d2[e]) >> 17;
+      if (!ROOT) c |= (uint32_t)(__builtin_bit_cast(uint64_t, h.x[e]) >> 56) & 0x80u;
+      q[e >> 2] |= c << (8 * (e & 3));
+    }
+  } else {
+    // small numbers: below 2^-6 the grid keeps its step of 2^-9, as a mantissa does when 2^-6 is added.  What is not finite
+    // counts for no largest value and is held as NaN.
+    if (odd) {
+      top = 0.0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmax(top, fabs(h.x[e]) <= most ? fabs(h.x[e]) : 0.0);
+      top = fmax(mt_max16(top), least);
+      inv = mt_scale8(top);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const double ax = fabs(h.x[e]), y = ax * inv;
+      const bool small = y < 0.015625;
+      const uint32_t z = (uint32_t)(__builtin_bit_cast(uint64_t, small ? y + 0.015625 : y) >> 32);
+      uint32_t c = ((z + d2[e]) >> 17) - (small ? 8u : 0u);
+      if (ROOT) c = max(c, ax > 1e-140 ? 1u : 0u);                     // (the root of MT_SOME stands for 0)
+      if (!(ax <= most)) c = 0x7fu;
+      c |= (uint32_t)(__builtin_bit_cast(uint64_t, h.x[e]) >> 56) & 0x80u;
+      q[e >> 2] |= c << (8 * (e & 3));
+    }
   }
   if (FULL) {
     *reinterpret_cast<u32x2*>((uint8_t*)base + i) = u32x2{q[0], q[1]};
@@ -280,29 +307,24 @@ __device__ __forceinline__ void adamw_pass(const AdamwArgs& a, const MtRec& r, i
     }
     const f32x8 g = mt_float(graw, r.g_t), mf = mt_float8(mc), rf = mt_float8(rc);
     p = mt_float(praw, r.p_t);
-    uint32_t d[8];
+    uint32_t d2[8];
     Hold8 m, rt;
     float odd = 0.f;
     const double am = a.b1d * ms, ag = a.c1d * gs, bv = a.b2d * (vs * vs), bg = a.c2d * gs * gs;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      d[e] = (dw[e >> 1] >> (16 * (e & 1))) & 0xffffu;
+      d2[e] = ((e & 1 ? dw[e >> 1] >> 15 : dw[e >> 1] << 1) & 0x1fffeu) - MT_BIAS8;
       const double ge = (double)g[e];
       m.x[e] = fma((double)mf[e], am, ag * ge);
-      rt.x[e] = mt_root(fma((double)(rf[e] * rf[e]), bv, bg * ge * ge));           // (the square of a code is exact in fp32)
+      rt.x[e] = mt_root(fma(bg * ge, ge, fma((double)(rf[e] * rf[e]), bv, MT_SOME)));           // (the square of a code is exact in fp32)
       const float m32 = (float)m.x[e], r32 = (float)rt.x[e];
-      odd = fmaf(m32, 0.f, fmaf(r32, 0.f, odd));                      // NaN once a value is not finite
-      // (1-ulp reciprocal, of the smallest normal number at least: the step is rounded to the parameter's last bit anyway)
-      const float den = r32 * inv_bc2s + a.eps;
-      p[e] = p[e] * keep - step_size * (m32 * __builtin_amdgcn_rcpf(den < 1.17549435e-38f ? 1.17549435e-38f : den));
+      // (1-ulp reciprocal: the step is rounded to the parameter's last bit anyway; eps8 is a normal number)
+      p[e] = p[e] * keep - step_size * (m32 * __builtin_amdgcn_rcpf(fmaf(r32, inv_bc2s, a.eps8)));
+      odd = fmaf(p[e], 0.f, odd);                                      // NaN once a moment, and so the parameter, is not finite
     }
-    if (__any(odd != 0.f)) {
-      mt_hold8<FULL, false, true>(r.m, r.ms, i, left, m, d);
-      mt_hold8<FULL, true, true>(r.v, r.vs, i, left, rt, d);
-    } else {
-      mt_hold8<FULL, false, false>(r.m, r.ms, i, left, m, d);
-      mt_hold8<FULL, true, false>(r.v, r.vs, i, left, rt, d);
-    }
+    const bool bad = __any(odd != 0.f);
+    mt_hold8<FULL, false>(r.m, r.ms, i, left, m, d2, bad);
+    mt_hold8<FULL, true>(r.v, r.vs, i, left, rt, d2, bad);
   } else {
     const Raw8 mraw = mt_load<FULL>(r.m, i, DPC_F32, left), vraw = mt_load<FULL>(r.v, i, DPC_F32, left);
     const f32x8 g = mt_float(graw, r.g_t);
@@ -461,6 +483,7 @@ extern "C" int dpc_adamw_step(const dpc_multi_info* info, const void* plan, doub
   AdamwArgs a;
   a.pl = mt_view(info, plan);
   a.lr = (float)lr; a.b1 = (float)b1; a.b2 = (float)b2; a.c1 = (float)(1.0 - b1); a.c2 = (float)(1.0 - b2); a.eps = (float)eps;
+  a.eps8 = a.eps < 1.17549435e-38f ? 1.17549435e-38f : a.eps;
   a.b1d = b1; a.b2d = b2; a.c1d = 1.0 - b1; a.c2d = 1.0 - b2;
   a.step_size = a.inv_bc2s = 0.f;
   if (!t_dev) {
