@@ -4,15 +4,17 @@
 //   d_rv = e^(l_rv - lse_r) - [v = t_r],  dh = alpha d W,  dW = alpha d^T h,  alpha = gscale / rows that count.
 //
 // Half-precision operands (bf16, fp16), per piece of rows:
-//   1. logits tiles on the matrix cores, fp32 accumulators.  A wave reduces its 128 (or 64) vocabulary entries of a row to
-//      (max, sum of e^(l - max)) in fp32 and, for training, leaves e^(l - max) in fp16 (values in (0, 1]: 11 bits where a
-//      later bf16 holds 8, so what reaches the gradients is rounded once) in P.
-//   2. per row: lse from the (max, sum) pairs, the loss, p_t - 1 by expm1 (no cancellation for sure rows).
-//   3. P becomes d in the operands' type: e^(max - lse) times what is there, p_t - 1 in the target's place, exactly 0 in
-//      rows that are ignored.
+//   1. logits tiles on the matrix cores, fp32 accumulators.  A wave reduces its 128 (or 64) vocabulary entries of a row, its
+//      slab, to a pair: ref = max l log2 e, rounded, and the sum of x = 2^(l log2 e - ref) in fp32; for training it leaves x
+//      in fp16 (values in [0, 1]: 11 bits where a later bf16 holds 8, so what reaches the gradients is rounded about once) in P.
+//   2. per row: the slabs' pairs become one, lse = ln 2 (ref + log2 sum), loss = ln 2 ((ref - l_t log2 e) + log2 sum) with
+//      one rounding in the difference, p_t - 1 = expm1(-loss): a sure row's small loss keeps its digits.
+//   3. P becomes d in the operands' type: 2^(slab's ref - row's ref) / row's sum times what is there, p_t - 1 in the
+//      target's place, exactly 0 in rows that are ignored.
 //   4. dh and dW as products over d.  dW of several pieces adds up in fp32.
-// That is 6 T V D flops, the least there is without keeping the logits; they bound it: d costs 4 bytes of traffic per
-// logit against 6 D flops.
+// That is 6 T V D flops.  They bound it for widths in the thousands (6 D flops against the 10 bytes per logit that writing
+// P, turning it into d and reading it twice move: 8192 x 2048 x 131072 spends 3.6 + 0.8 + 3.2 + 3.25 ms on steps 1, 3 and
+// 4); below a width of about 500 the traffic does.
 //
 // P's layout [vocabulary / 8][row][8 entries] serves all three products: 16-byte chunks of 8 vocabulary entries are k-runs
 // of the dh product's operand and, transposed on the way out of LDS, m-runs of dW's; step 1 and 3 touch it in runs of
@@ -130,16 +132,24 @@ __device__ __forceinline__ void lce_wait_vm() { asm volatile("s_waitcnt vmcnt(%0
 // The transposing read gives lane i of 16 the column i of a 4 x 16 block whose row r comes from lanes 4r .. 4r+3; the
 // swizzles put what the 32 lanes of one LDS cycle read on different banks.
 //
-// NS tiles are in flight or in use.  Iteration kt: while the products of the wave's upper rows run, its lower rows' fragments
-// are read; then, once tile kt + 1 has landed for every wave and tile kt has been read by all (one barrier), tile kt + NS
-// goes on its way into the freed slot and the next tile's first fragments are read while the lower rows' products run.
-template <typename E, int MODE, int BM, int BN, int WM, int WN, int NS>
+// Three tiles are in use or on their way.  Iteration kt: while the products of the wave's upper rows run, its lower rows'
+// fragments are read; then, once tile kt + 1 has landed for every wave and tile kt has been read by all (one barrier),
+// tile kt + 3 goes on its way into the freed slot and the next tile's first fragments are read while the lower rows'
+// products run.
+//
+// 256 x 256 with 8 waves of 128 x 64 (196 registers, 96 KB of LDS, one block per CU) on 8192 rows, width 2048, vocabulary
+// 131072: 1230 (logits), 1380 (dh) and 1345 (dW) TFLOP/s where a library product of the same shape reaches 1374 to 1594 and
+// nothing but matrix instructions 1946.  The clock is down to 1.82 GHz under that load and the matrix units are busy 72 % of
+// it; LDS is not what they wait for (no bank conflicts, 0.4 of its cycles).  Measured and dropped: 4 waves of 128 x 128
+// (spills, or the same), two 4-wave blocks per CU (dh 1.3 times as long), four and five tiles in LDS (the same), one barrier
+// per 64 k (dW 4 % faster, the others 6 to 9 % slower: less time for the loads), blocks started at different times.
+template <typename E, int MODE, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
   using H = Half<E>;
   constexpr int NT = WM * WN * 64;
   constexpr int SM = BM / WM / 16, SN = BN / WN / 16, SH = SM / 2;
   constexpr int NA = BM * 4 / NT, NB = BN * 4 / NT;
-  constexpr int SLOT = (BM + BN) * 64;
+  constexpr int SLOT = (BM + BN) * 64, NS = 3;
   constexpr bool A_K = MODE == LCE_LOGITS, B_K = MODE != LCE_DW;
   __shared__ __attribute__((aligned(1024))) char lds[NS * SLOT];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -285,11 +295,9 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
       }
     }
   };
-  // The next tile has landed for every wave, with at most `ahead` tiles behind it on their way; this one has been read.
-  const auto meet = [&](int ahead) {
-    constexpr int L = NA + NB;
-    if (ahead >= NS - 2) lce_wait_vm<(NS - 2) * L>();
-    else if (NS > 3 && ahead == NS - 3) lce_wait_vm<(NS - 3) * L>();
+  // The next tile has landed for every wave - `ahead`: another one may be on its way behind it - and this one has been read.
+  const auto meet = [&](bool ahead) {
+    if (ahead) lce_wait_vm<NA + NB>();
     else lce_wait_vm<0>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -297,17 +305,16 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
   };
 
   if (nk > 0) {
-#pragma unroll
-    for (int k = 0; k < NS - 1; ++k)
-      if (k < nk) issue(k, lds + k * SLOT);
-    meet(min(NS - 2, nk - 1));
-    if (NS - 1 < nk) issue(NS - 1, lds + (NS - 1) * SLOT);
+    issue(0, lds);
+    if (nk > 1) issue(1, lds + SLOT);
+    meet(nk > 1);
+    if (nk > 2) issue(2, lds + 2 * SLOT);
 #pragma unroll
     for (int j = 0; j < SN; ++j) b[j] = frag_b(lds, j);
 #pragma unroll
     for (int i = 0; i < SH; ++i) a0[i] = frag_a(lds, i);
     int cur = 0, kt = 0;
-    const auto tile = [&](auto more, auto load, int ahead) {
+    const auto tile = [&](auto more, auto load, bool ahead) {
       const int nxt = cur + 1 == NS ? 0 : cur + 1;
       half_tile(No(), No(), No(), lds + cur * SLOT, 0, nullptr);
       if (decltype(more)::value) meet(ahead);
@@ -315,9 +322,9 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
       half_tile(Yes(), more, load, lds + nxt * SLOT, kt + NS, lds + cur * SLOT);
       cur = nxt;
     };
-    for (; kt + NS < nk; ++kt) tile(Yes(), Yes(), NS - 2);
-    for (; kt + 1 < nk; ++kt) tile(Yes(), No(), nk - 2 - kt);           // nothing more to load
-    tile(No(), No(), 0);
+    for (; kt + NS < nk; ++kt) tile(Yes(), Yes(), true);
+    for (; kt + 1 < nk; ++kt) tile(Yes(), No(), kt + 2 < nk);           // nothing more to load
+    tile(No(), No(), false);
   }
 
   // C layout of a 16 x 16 block: n = lane & 15, m = 4 (lane >> 4) + e
@@ -519,7 +526,9 @@ __global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, c
   const int nb = (int)(prow / 256), slab = blockIdx.x / nb, n = (blockIdx.x - slab * nb) * 256 + threadIdx.x;
   const f32x2 gl = n < rows ? live[n] : f32x2{0.f, 0.f};
   const bool on = gl.y != 0.f;                                         // (NaN is on: such a row keeps its NaN)
-  const float f = on ? __builtin_amdgcn_exp2f(stat[(int64_t)slab * prow + n].x - gl.x) * gl.y * Half<E>::kUp : 0.f;
+  const f32x2 st = on ? stat[(int64_t)slab * prow + n] : f32x2{0.f, 0.f};
+  // (a slab of nothing but -inf has the sum 0 and a reference that may lie far above the row's)
+  const float f = st.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(st.x - gl.x) * gl.y * Half<E>::kUp;
   int at = -1;
   float pt = 0.f;
   if (on) {
@@ -785,7 +794,7 @@ extern "C" int64_t dpc_linear_cross_entropy_ws(int64_t T, int D, int V, int dtyp
   return lce_layout(T, D, V, dtype, grads != 0, dtype != DPC_F32 && !dw_f32, piece_rows).bytes;
 }
 
-template <typename E, int MODE, int BM, int BN, int WM, int WN, int NS>
+template <typename E, int MODE, int BM, int BN, int WM, int WN>
 static void lce_launch_tile(LceArgs& g, int kind, hipStream_t st) {
   g.tiles_m = (int)dpc_cdiv(g.M, BM);
   g.tiles_n = (int)dpc_cdiv(g.N, BN);
@@ -794,28 +803,15 @@ static void lce_launch_tile(LceArgs& g, int kind, hipStream_t st) {
   g.whole = c.whole;
   g.splits = c.splits;
   g.kchunk = (int)lce_up(dpc_cdiv(g.K, g.splits), LCE_BK);
-  hipLaunchKernelGGL((lce_product_kernel<E, MODE, BM, BN, WM, WN, NS>), dim3(g.whole + (tiles - g.whole) * g.splits), dim3(WM * WN * 64), 0, st, g);
+  hipLaunchKernelGGL((lce_product_kernel<E, MODE, BM, BN, WM, WN>), dim3(g.whole + (tiles - g.whole) * g.splits), dim3(WM * WN * 64), 0, st, g);
   if (MODE != LCE_LOGITS && g.whole < tiles)
     hipLaunchKernelGGL((lce_fold_kernel<E, BM, BN>), dim3((tiles - g.whole) * (BM * BN / 1024)), dim3(256), 0, st, g);
 }
-#ifndef LCE_CFG_0
-#define LCE_CFG_0 256, 256, 2, 4, 3
-#endif
-#ifndef LCE_CFG_1
-#define LCE_CFG_1 256, 256, 2, 4, 3
-#endif
-#ifndef LCE_CFG_2
-#define LCE_CFG_2 256, 256, 2, 4, 3
-#endif
 template <typename E, int MODE>
 static void lce_launch(LceArgs& g, int kind, hipStream_t st) {
-  if (kind == LCE_MID) lce_launch_tile<E, MODE, 128, 128, 2, 2, 3>(g, kind, st);
-  else if constexpr (MODE == LCE_LOGITS) {
-    if (kind == LCE_ROW) lce_launch_tile<E, MODE, 128, 64, 2, 1, 3>(g, kind, st);
-    else lce_launch_tile<E, MODE, LCE_CFG_0>(g, kind, st);
-  }
-  else if constexpr (MODE == LCE_DH) lce_launch_tile<E, MODE, LCE_CFG_1>(g, kind, st);
-  else lce_launch_tile<E, MODE, LCE_CFG_2>(g, kind, st);
+  if (kind == LCE_BIG) lce_launch_tile<E, MODE, 256, 256, 2, 4>(g, kind, st);
+  else if (kind == LCE_MID) lce_launch_tile<E, MODE, 128, 128, 2, 2>(g, kind, st);
+  else if constexpr (MODE == LCE_LOGITS) lce_launch_tile<E, MODE, 128, 64, 2, 1>(g, kind, st);
 }
 
 struct LceCall {
@@ -960,12 +956,16 @@ extern "C" int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* 
     DPC_CHECK_ARG(ldh < (1 << 21) && ldw < (1 << 21), "linear_cross_entropy: rows are too long");     // (256 rows within 32-bit offsets)
     DPC_CHECK_ARG((!dh || lddh % 8 == 0) && (!dw || lddw % (dw_f32 ? 4 : 8) == 0), "linear_cross_entropy: gradient rows must be 16-byte aligned");
   }
+  DPC_CHECK_ARG((!dh || (dh != h && dh != w && dh != dw)) && (!dw || (dw != h && dw != w)), "linear_cross_entropy: a gradient must not lie where an operand does");
   DPC_CHECK_ARG(((uintptr_t)ws & 255) == 0, "linear_cross_entropy: the workspace must be 256-byte aligned");
   const bool grads = dh || dw;
   if (piece_rows <= 0) piece_rows = lce_rows_default(T, D, V, dtype, grads, !f32 && !dw_f32);
   const int64_t most = piece_rows < T ? piece_rows : T;
-  DPC_CHECK_ARG(dpc_cdiv(V, 64) * dpc_cdiv(most, 64) < (1ll << 30) && dpc_cdiv(V, LCE_SEG) * most < (1ll << 31), "linear_cross_entropy: the piece is too large");
-  DPC_CHECK_ARG(f32 || !grads || piece_rows <= (1 << 21) || T <= (1 << 21), "linear_cross_entropy: the piece is too large");
+  // (a launch has less than 2^32 threads: 512 for each 256 x 256 tile, one for each row and slab, 256 for 4096 fp32 logits of a row;
+  // and 256 vocabulary entries of P lie within 32-bit offsets)
+  DPC_CHECK_ARG(f32 ? dpc_cdiv(V, LCE_SEG) * most < (1ll << 23) : dpc_cdiv(V, 256) * dpc_cdiv(most > D ? most : D, 256) < (1ll << 22),
+                "linear_cross_entropy: the piece is too large");
+  DPC_CHECK_ARG(f32 || !grads || most <= (1 << 21), "linear_cross_entropy: the piece is too large");
   const LceLayout l = lce_layout(T, D, V, dtype, grads, !f32 && !dw_f32, piece_rows);
   DPC_CHECK_ARG(ws_bytes >= l.bytes, "linear_cross_entropy: the workspace is smaller than dpc_linear_cross_entropy_ws says");
   hipStream_t st = (hipStream_t)stream;

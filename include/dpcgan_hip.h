@@ -464,7 +464,8 @@ int dpc_noise_add_clamp(float* x, int64_t n, float scale, const float* noise_inj
  *   there, and their dh is 0.
  * Sums, softmax statistics and products are in fp32; half precision rounds (softmax - onehot) once to the operands' type,
  * fp16 with a lift of 2^14.  No atomics: the same call gives the same bits.
- * Half precision: D a multiple of 8, every row of every matrix 16-byte aligned.  fp32: any D and row length.
+ * Half precision: D a multiple of 8, every row of every matrix 16-byte aligned.  fp32: any D and row length.  The outputs
+ * overlap neither the operands nor each other.
  * ws: workspace of dpc_linear_cross_entropy_ws bytes for the same arguments (-1 if they are refused), 256-byte aligned, no
  * state between calls; calls that overlap need one each.  piece_rows: rows worked on at a time (0 = what 1 GiB holds);
  * smaller pieces need less workspace, and read and write dw once for each. */

@@ -202,6 +202,22 @@ def test_logits_far_apart(ops, dtype):
     check(call(ops, h, w, target), Oracle(h, w, target))
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('offset', [-400, 400])
+def test_entries_whose_logits_are_all_minus_infinity(ops, dtype, offset):
+    """256 entries (whole slabs) whose logits overflow to -inf take no part, however far from 0 the others lie."""
+    T, D, V = 150, 64, 700
+    h, w, target = inputs(T, D, V, dtype, 6, scale=0.5)
+    h[:, 0], w[:, 0] = 4, offset / 4
+    off = torch.zeros(256, D, dtype=dtype, device=DEV)
+    off[:, 0] = -2.0 ** 127
+    ref = Oracle(h, w, target)
+    o = call(ops, h, torch.cat([off, w]), torch.where(target < 0, target, target + 256))
+    assert (o['dw'][:256] == 0).all()
+    o['dw'] = o['dw'][256:]
+    check(o, ref)
+
+
 @pytest.mark.parametrize('dtype', TYPES)
 def test_a_nan_row_stays_a_row(ops, dtype):
     h, w, target = inputs(100, 64, 300, dtype, 6, ignored=0.0)
