@@ -19,6 +19,8 @@ SITE_NOISE_D, SITE_HOOK, SITE_ENCODE, SITE_DITHER = 7, 8, 9, 10
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # DPC_F32, DPC_BF16, DPC_F16
 _dev_index = None        # GPU of the tensors of the call being assembled (see _stream)
+# the current stream's handle without a torch.cuda.Stream object around it (2.4 us of a call that takes 9)
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _p(t):
@@ -42,11 +44,11 @@ def _stream():
     below converts its tensors (``_p``) before it asks for the stream, so a call whose tensors live on
     another GPU than the current one is refused here instead of being launched on the wrong device's
     stream with pointers into another device's memory."""
-    idx = _dev_index
-    if idx is not None and idx != torch.cuda.current_device():
+    idx, cur = _dev_index, torch.cuda.current_device()
+    if idx is not None and idx != cur:
         raise RuntimeError('dp_cgans_amd.ops: tensors on cuda:%d but the current device is cuda:%d; run under '
-                           '`with torch.cuda.device(%d):`' % (idx, torch.cuda.current_device(), idx))
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+                           '`with torch.cuda.device(%d):`' % (idx, cur, idx))
+    return ctypes.c_void_p(_raw_stream(cur))
 
 
 def _chk(t, dtype, name):
@@ -692,17 +694,18 @@ def linear_cross_entropy(h, w, target, loss, ws, dh=None, dw=None, lse=None, tot
     _chk(w, h.dtype, 'w')
     _chk(target, torch.int64, 'target')
     for t, n, name in ((loss, T, 'loss'), (lse, T, 'lse'), (total, 1, 'total')):
-        _chk(t, torch.float32, name)
-        if t is not None and (t.numel() != n or not t.is_contiguous()):
-            raise ValueError('linear_cross_entropy: %s must be contiguous with %d entries' % (name, n))
+        if t is not None:
+            _chk(t, torch.float32, name)
+            if t.numel() != n or not t.is_contiguous():
+                raise ValueError('linear_cross_entropy: %s must be contiguous with %d entries' % (name, n))
     if target.numel() != T or not target.is_contiguous():
         raise ValueError('linear_cross_entropy: target must be contiguous with %d entries' % T)
-    _chk(dh, h.dtype, 'dh')
     dw_f32 = dw is not None and dw.dtype == torch.float32
-    _chk(dw, torch.float32 if dw_f32 else h.dtype, 'dw')
     for t, like, name in ((dh, h, 'dh'), (dw, w, 'dw')):
-        if t is not None and t.shape != like.shape:
-            raise ValueError('linear_cross_entropy: %s must be %s, got %s' % (name, tuple(like.shape), tuple(t.shape)))
+        if t is not None:
+            _chk(t, torch.float32 if t is dw and dw_f32 else h.dtype, name)
+            if t.shape != like.shape:
+                raise ValueError('linear_cross_entropy: %s must be %s, got %s' % (name, tuple(like.shape), tuple(t.shape)))
     _chk(ws, torch.uint8, 'ws')
     if not ws.is_contiguous():
         raise ValueError('linear_cross_entropy: ws must be contiguous')
@@ -845,6 +848,8 @@ def grad_clip(plan, max_norm, out, gscale=1.0, t_dev=None):
     _chk(t_dev, torch.int32, 't_dev')
     if out.numel() < 2 or not out.is_contiguous():
         raise ValueError('grad_clip: out must be a contiguous fp32 [2]')
+    if t_dev is not None and t_dev.numel() < 1:
+        raise ValueError('grad_clip: t_dev must be an int32 [1]')
     lib().call('dpc_grad_clip', plan._info, _p(plan.table), float(max_norm), float(gscale), _p(out), _p(t_dev), _stream())
     return out
 
@@ -856,6 +861,9 @@ def adamw_step(plan, lr, b1=0.9, b2=0.999, eps=1e-8, coef=None, gscale=1.0, t_de
     _chk(coef, torch.float32, 'coef')
     _chk(t_dev, torch.int32, 't_dev')
     _chk(rng, torch.int64, 'rng')
+    for t, n, name in ((coef, 1, 'coef'), (t_dev, 1, 't_dev'), (rng, 2, 'rng')):
+        if t is not None and t.numel() < n:
+            raise ValueError('adamw_step: %s needs %d entries' % (name, n))
     lib().call('dpc_adamw_step', plan._info, _p(plan.table), float(lr), float(b1), float(b2), float(eps), _p(coef),
                float(gscale), _p(t_dev), int(t_host), _p(rng), site, _stream())
 
