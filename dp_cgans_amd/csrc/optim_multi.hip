@@ -35,6 +35,10 @@ struct MtChunk { int32_t t; int32_t pad; int64_t start; };
 
 struct MtPlan { const MtRec* rec; const MtChunk* chunk; int blocks; };
 
+#define MT_GROUPS 16             // groups of blocks that count their ends apart, each on a line of its own
+#define MT_LINE 64               // words between two counts
+#define MT_COUNTS 4608           // bytes of the counts, (1 + MT_GROUPS) lines
+
 static int64_t mt_align(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
 // 8 consecutive elements, as loaded: two halves of fp32, one of 16 bits.  Loading and converting are apart so that a
@@ -99,8 +103,32 @@ __device__ __forceinline__ void mt_store(void* base, int64_t i, int type, int le
 }
 
 // ---- global norm ---------------------------------------------------------------------------------------------------
+// out = {norm, coef} from the partial sums; a norm that is not finite gives coef 0 (the step that reads it is not taken) and
+// leaves *t alone.
+struct ClipArgs { double max_norm, gscale; float* out; int32_t* t; };
+__device__ __forceinline__ void grad_clip_finish(const double* part, int n, const ClipArgs& a, double* red) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += 256)
+    s += __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<const uint64_t*>(part) + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  s = dpc_block_sum(s, red);
+  if (threadIdx.x == 0) {
+    const double norm = a.gscale * sqrt(s);
+    const bool ok = norm <= 1.7976931348623157e308;        // false for NaN too
+    a.out[0] = (float)norm;
+    a.out[1] = ok ? (float)(norm > a.max_norm ? a.gscale * (a.max_norm / norm) : a.gscale) : 0.f;
+    if (ok && a.t) *a.t += 1;
+  }
+}
+__global__ __launch_bounds__(256) void grad_clip_none_kernel(ClipArgs a) {      // (a plan without elements: norm 0)
+  __shared__ double red[16];
+  grad_clip_finish(nullptr, 0, a, red);
+}
+
 // sum of g^2 in fp64 (the square of an fp32 gradient overflows at 2e19 and vanishes below 1e-23): one partial per
-// block, chunks b, b + gridDim, ... in that order, so the sum does not depend on which block ends first.
+// block, chunks b, b + gridDim, ... in that order; the block that ends last adds up the partials, in theirs, so the sum does
+// not depend on which one that is (with a second launch for it a call took the host 7.0 us instead of 3.5, the GPU as long).
+// What crosses between blocks is written through and read past the XCDs' own L2s, word by word: an acquire and a release,
+// which write back and empty an L2 for every block, made the norm of 0.8 GB 208 us long instead of 124.
 // NT: the gradients are larger than the 256 MB of the last-level cache and are read past it.
 template <bool NT>
 __device__ __forceinline__ Raw8 mt_load_norm(const MtRec& r, int64_t i, int64_t end, bool full) {
@@ -111,9 +139,12 @@ __device__ __forceinline__ Raw8 mt_load_norm(const MtRec& r, int64_t i, int64_t 
   if (r.g_t == DPC_F32) o.b = NT ? __builtin_nontemporal_load(q + 1) : q[1];
   return o;
 }
+__device__ __forceinline__ uint32_t mt_add(uint32_t* p) { return __hip_atomic_fetch_add(p, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void mt_put(uint32_t* p, uint32_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <bool NT>
-__global__ __launch_bounds__(256) void grad_sumsq_kernel(MtPlan pl, double* part) {
+__global__ __launch_bounds__(256) void grad_clip_kernel(MtPlan pl, double* part, uint32_t* ended, ClipArgs a) {
   __shared__ double red[16];
+  __shared__ bool last;
   double s = 0.0;
   // four chunks at a time: their loads are in flight together
   for (int c0 = blockIdx.x * 4; c0 < pl.blocks; c0 += gridDim.x * 4) {
@@ -135,22 +166,22 @@ __global__ __launch_bounds__(256) void grad_sumsq_kernel(MtPlan pl, double* part
     }
   }
   s = dpc_block_sum(s, red);
-  if (threadIdx.x == 0) part[blockIdx.x] = s;
-}
-
-// out = {norm, coef}; a norm that is not finite gives coef 0 (the step that reads it is not taken) and leaves *t alone.
-__global__ __launch_bounds__(256) void grad_clip_kernel(const double* part, int n, double max_norm, double gscale, float* out, int32_t* t) {
-  __shared__ double red[16];
-  double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += 256) s += part[i];
-  s = dpc_block_sum(s, red);
   if (threadIdx.x == 0) {
-    const double norm = gscale * sqrt(s);
-    const bool ok = norm <= 1.7976931348623157e308;        // false for NaN too
-    out[0] = (float)norm;
-    out[1] = ok ? (float)(norm > max_norm ? gscale * (max_norm / norm) : gscale) : 0.f;
-    if (ok && t) *t += 1;
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(part) + blockIdx.x, __builtin_bit_cast(uint64_t, s), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                   // (written through: it is there for every XCD)
+    // (counted in MT_GROUPS groups, then the groups: adds to one word follow one another, 10 ns each)
+    const uint32_t group = blockIdx.x % MT_GROUPS, groups = min(gridDim.x, (uint32_t)MT_GROUPS), size = (gridDim.x - group + MT_GROUPS - 1) / MT_GROUPS;
+    uint32_t* own = ended + (1 + group) * MT_LINE;
+    last = false;
+    if (mt_add(own) + 1 == size) {
+      mt_put(own, 0u);                                                 // for the next call
+      last = mt_add(ended) + 1 == groups;
+      if (last) mt_put(ended, 0u);
+    }
   }
+  __syncthreads();
+  if (!last) return;
+  grad_clip_finish(part, gridDim.x, a, red);
 }
 
 // ---- AdamW ---------------------------------------------------------------------------------------------------------
@@ -380,7 +411,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwArgs a) {
 static int mt_size(int type) { return type == DPC_F32 ? 4 : 2; }
 static bool mt_type_ok(int type) { return type == DPC_F32 || type == DPC_BF16 || type == DPC_F16; }
 static bool mt_al(const void* p, int bytes) { return ((uintptr_t)p % (uintptr_t)bytes) == 0; }
-#define MT_PARTS 2048            // partial sums of the global norm (blocks of its first launch)
+#define MT_PARTS 2048            // partial sums of the global norm: its blocks at most
 
 static int mt_check(const dpc_multi_tensor* t, int count, dpc_multi_info* info) {
   DPC_CHECK_ARG(count >= 0 && (t || count == 0) && info, "multi_plan: null pointer or negative count");
@@ -412,14 +443,14 @@ static int mt_check(const dpc_multi_tensor* t, int count, dpc_multi_info* info) 
   // against 2114)
   int64_t blocks = 0;
   for (int k = 0; k < count; ++k) blocks += dpc_cdiv(t[k].n, MT_SUB);
-  DPC_CHECK_ARG(blocks < (1ll << 31), "multi_plan: too many elements");
+  DPC_CHECK_ARG(blocks < (1ll << 24), "multi_plan: too many elements");      // (a launch has less than 2^32 threads)
   info->kind = kinds;
   info->grad_bytes = grad_bytes;
   info->count = count;
   info->blocks = (int)blocks;
   info->rec_off = 0;
   info->chunk_off = mt_align((int64_t)count * sizeof(MtRec));
-  info->part_off = info->chunk_off + mt_align(blocks * (int64_t)sizeof(MtChunk));
+  info->part_off = info->chunk_off + mt_align(blocks * (int64_t)sizeof(MtChunk)) + MT_COUNTS;      // (before it the counts of blocks that have ended)
   info->bytes = info->part_off + MT_PARTS * sizeof(double);
   return DPC_OK;
 }
@@ -462,11 +493,12 @@ extern "C" int dpc_grad_clip(const dpc_multi_info* info, void* plan, double max_
   DPC_CHECK_ARG(info && plan && out, "grad_clip: null pointer");
   DPC_CHECK_ARG(max_norm > 0.0 && gscale > 0.0 && gscale <= 3.402823466e38, "grad_clip: max_norm and gscale must be positive");
   double* part = (double*)((char*)plan + info->part_off);
+  const ClipArgs a = {max_norm, gscale, out, t_dev};
   const int64_t quads = dpc_cdiv(info->blocks, 4);
   const int nb = (int)(quads < MT_PARTS ? quads : MT_PARTS);
-  const auto sumsq = info->grad_bytes > (256ll << 20) ? grad_sumsq_kernel<true> : grad_sumsq_kernel<false>;
-  if (nb > 0) hipLaunchKernelGGL(sumsq, dim3(nb), dim3(256), 0, (hipStream_t)stream, mt_view(info, plan), part);
-  hipLaunchKernelGGL(grad_clip_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, part, nb, max_norm, gscale, out, t_dev);
+  const auto clip = info->grad_bytes > (256ll << 20) ? grad_clip_kernel<true> : grad_clip_kernel<false>;
+  if (nb > 0) hipLaunchKernelGGL(clip, dim3(nb), dim3(256), 0, (hipStream_t)stream, mt_view(info, plan), part, (uint32_t*)((char*)part - MT_COUNTS), a);
+  else hipLaunchKernelGGL(grad_clip_none_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, a);
   DPC_LAUNCH_CHECK();
   return DPC_OK;
 }

@@ -500,7 +500,8 @@ typedef struct dpc_multi_info {
 /* A plan is built in host memory (t, info, plan: HOST pointers; nothing is launched) and copied by the caller into
  * `bytes` of 256-byte aligned device memory; it holds addresses, so it serves every step while the tensors stay where
  * they are.  The tensors of a plan are all of one kind (gradients only; 32-bit; 8-bit; 8-bit with dither) and none
- * may overlap.  A plan holds grad_clip's partial sums: calls on one plan follow one another. */
+ * may overlap.  A plan holds grad_clip's partial sums and the count of its blocks that have ended
+ * (0 between calls): calls on one plan follow one another. */
 int dpc_multi_plan_size(const dpc_multi_tensor* t, int count, dpc_multi_info* info);
 int dpc_multi_plan(const dpc_multi_tensor* t, int count, const dpc_multi_info* info, void* plan, int64_t bytes);
 /* out fp32 [2] = {norm, coef}: norm = gscale * sqrt(sum of g^2 over all tensors) (fp64 sums, fixed order), coef =

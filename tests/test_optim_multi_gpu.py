@@ -370,6 +370,38 @@ def test_adamw_many_chunks_and_the_norm_of_them(ops):
         assert ((p.double() + 1e-2 * x / (x.abs() + 1e-3)).abs() <= 16 * 2.0 ** -24 * 1e-2).all()
 
 
+@pytest.mark.parametrize('quads', [0.3, 1, 15, 16, 17, 33, 255, 2047, 2048, 2049, 4100])
+def test_norm_of_any_number_of_blocks(ops, quads):
+    """A block works on 4 x 2048 elements at a time; the one that ends last finishes the call and leaves the plan as it was:
+    the same bits time after time, whatever the other plan did in between."""
+    n = int(quads * 8192)
+    g = torch.randn(n, device=DEV, generator=torch.Generator(device=DEV).manual_seed(n))
+    plan, other = ops.grad_plan([g]), ops.grad_plan([g[:n // 2], g[n // 2:]])
+    before = plan.table.clone()
+    want = g.double().square().sum().sqrt().item()
+    outs = []
+    for _ in range(4):
+        out = torch.full((2,), float('nan'), device=DEV)
+        ops.grad_clip(plan, 0.5, out)
+        ops.grad_clip(other, 0.5, torch.empty(2, device=DEV))
+        outs.append(out)
+    # fp64 sums: the result is rounded to fp32 once
+    assert abs(outs[0][0].item() - want) <= 2.0 ** -23 * want and abs(outs[0][1].item() * want - 0.5) <= 2.0 ** -23
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    at = plan.info.part_off
+    assert torch.equal(plan.table[:at], before[:at])
+
+
+def test_small_buffers_are_refused(ops):
+    f = lambda n, t=torch.float32: torch.zeros(n, dtype=t, device=DEV)  # noqa: E731
+    plan = ops.adamw_plan([f(8)], [f(8)], [f(8)], [f(8)])
+    for bad in (dict(coef=f(0)), dict(t_dev=f(0, torch.int32)), dict(rng=f(1, torch.int64))):
+        with pytest.raises(ValueError, match='entries'):
+            ops.adamw_step(plan, 1e-3, **bad)
+    with pytest.raises(ValueError, match='t_dev'):
+        ops.grad_clip(plan, 1.0, f(2), t_dev=f(0, torch.int32))
+
+
 def test_adamw_refusals(ops):
     f = lambda n=256, t=torch.float32: torch.zeros(n, dtype=t, device=DEV)  # noqa: E731
     ok = ops.adamw_plan([f()], [f()], [f()], [f()])
