@@ -132,10 +132,10 @@ __device__ __forceinline__ void lce_wait_vm() { asm volatile("s_waitcnt vmcnt(%0
 // The transposing read gives lane i of 16 the column i of a 4 x 16 block whose row r comes from lanes 4r .. 4r+3; the
 // swizzles put what the 32 lanes of one LDS cycle read on different banks.
 //
-// Three tiles are in use or on their way.  Iteration kt: while the products of the wave's upper rows run, its lower rows'
-// fragments are read; then, once tile kt + 1 has landed for every wave and tile kt has been read by all (one barrier),
-// tile kt + 3 goes on its way into the freed slot and the next tile's first fragments are read while the lower rows'
-// products run.
+// NS = 3 tiles are in use or on their way - 6 for the few rows, where the loads of W are all there is to wait for (4 x 256 x
+// 18000: 8.1 -> 6.5 us).  Iteration kt: while the products of the wave's upper rows run, its lower rows' fragments are
+// read; then, once tile kt + 1 has landed for every wave and tile kt has been read by all (one barrier), tile kt + NS goes
+// on its way into the freed slot and the next tile's first fragments are read while the lower rows' products run.
 //
 // 256 x 256 with 8 waves of 128 x 64 (196 registers, 96 KB of LDS, one block per CU) on 8192 rows, width 2048, vocabulary
 // 131072: 1230 (logits), 1380 (dh) and 1345 (dW) TFLOP/s where a library product of the same shape reaches 1374 to 1594 and
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
   constexpr int NT = WM * WN * 64;
   constexpr int SM = BM / WM / 16, SN = BN / WN / 16, SH = SM / 2;
   constexpr int NA = BM * 4 / NT, NB = BN * 4 / NT;
-  constexpr int SLOT = (BM + BN) * 64, NS = 3;
+  constexpr int SLOT = (BM + BN) * 64, NS = BN == 64 ? 6 : 3;
   constexpr bool A_K = MODE == LCE_LOGITS, B_K = MODE != LCE_DW;
   __shared__ __attribute__((aligned(1024))) char lds[NS * SLOT];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -295,9 +295,9 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
       }
     }
   };
-  // The next tile has landed for every wave - `ahead`: another one may be on its way behind it - and this one has been read.
+  // The next tile has landed for every wave - `ahead`: NS - 2 others may be on their way behind it - and this one has been read.
   const auto meet = [&](bool ahead) {
-    if (ahead) lce_wait_vm<NA + NB>();
+    if (ahead) lce_wait_vm<(NS - 2) * (NA + NB)>();
     else lce_wait_vm<0>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -305,10 +305,11 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
   };
 
   if (nk > 0) {
-    issue(0, lds);
-    if (nk > 1) issue(1, lds + SLOT);
-    meet(nk > 1);
-    if (nk > 2) issue(2, lds + 2 * SLOT);
+#pragma unroll
+    for (int k = 0; k < NS - 1; ++k)
+      if (k < nk) issue(k, lds + k * SLOT);
+    meet(nk >= NS - 1);
+    if (nk >= NS) issue(NS - 1, lds + (NS - 1) * SLOT);
 #pragma unroll
     for (int j = 0; j < SN; ++j) b[j] = frag_b(lds, j);
 #pragma unroll
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
       cur = nxt;
     };
     for (; kt + NS < nk; ++kt) tile(Yes(), Yes(), true);
-    for (; kt + 1 < nk; ++kt) tile(Yes(), No(), kt + 2 < nk);           // nothing more to load
+    for (; kt + 1 < nk; ++kt) tile(Yes(), No(), kt + NS - 1 < nk);           // nothing more to load
     tile(No(), No(), false);
   }
 
@@ -342,6 +343,7 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
 #pragma unroll
     for (int j = 0; j < SN; ++j) {
       const int n = nw + j * 16;
+      if (BN == 64 && n - l16 >= g.N) break;                           // (few rows: the rest of the tile is empty)
       const int64_t t = n < g.N ? g.target[n] : -1;
       if (__any(t >= mw && t < mw + SM * 16)) {
         const int at = t >= mw && t < mw + SM * 16 ? (int)(t - mw) : -1;
@@ -444,7 +446,8 @@ __device__ __forceinline__ f32x2 lce_join(f32x2 x, f32x2 y) {
 }
 
 // Per row: the slabs' pairs become one, lse, the loss and what the gradient needs.  16 rows x 64 runs of slabs per block (with
-// 32 rows x 8 runs a thread's chain of 128 dependent loads and exponents took 65 us for 4096 x 1024 pairs, now 8).
+// 32 rows x 8 runs a thread's chain of 128 dependent loads and exponents took 65 us for 4096 x 1024 pairs, now 8); the runs
+// meet within their waves first and through LDS once.
 struct LceRowArgs {
   const f32x2* stat; int64_t prow; int slabs; int rows; int V;
   const float* lt; const int64_t* target; int64_t ignore;
@@ -455,16 +458,8 @@ struct LceRowArgs {
   float* alpha; float scale; int mean; const int64_t* all; int64_t T;
   float* total;                 // of a call that is one block: the mean (or sum) of the losses; nullable
 };
-// (sum, count) of the losses over the block -> total
-__device__ __forceinline__ void lce_total(double s, int c, int mean, float* total) {
-  __shared__ double red[16];
-  __shared__ int redi[16];
-  s = dpc_block_sum(s, red);
-  c = dpc_block_sum(c, redi);
-  if (threadIdx.x == 0) total[0] = (float)(s / (mean ? (double)max(c, 1) : 1.0));
-}
 __global__ __launch_bounds__(1024) void lce_rows_kernel(LceRowArgs a) {
-  __shared__ f32x2 red[64][16];
+  __shared__ f32x2 red[16][16];
   if (a.alpha && blockIdx.x + 1 == gridDim.x) {
     int c = 0;
     if (a.mean)
@@ -480,11 +475,14 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(LceRowArgs a) {
 #pragma unroll 4
     for (int s = w; s < a.slabs; s += 64) x = lce_join(x, a.stat[(int64_t)s * a.prow + n]);
   }
-  red[w][r] = x;
-  for (int k = 32; k > 0; k >>= 1) {
-    __syncthreads();
-    if (w < k) red[w][r] = x = lce_join(x, red[w + k][r]);
-  }
+  x = lce_join(x, f32x2{__shfl_xor(x.x, 16, 64), __shfl_xor(x.y, 16, 64)});
+  x = lce_join(x, f32x2{__shfl_xor(x.x, 32, 64), __shfl_xor(x.y, 32, 64)});
+  if ((w & 3) == 0) red[w >> 2][r] = x;
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  x = lce_join(lce_join(red[w][r], red[w + 4][r]), lce_join(red[w + 8][r], red[w + 12][r]));
+  x = lce_join(x, f32x2{__shfl_xor(x.x, 16, 64), __shfl_xor(x.y, 16, 64)});
+  x = lce_join(x, f32x2{__shfl_xor(x.x, 32, 64), __shfl_xor(x.y, 32, 64)});
   double sum = 0.0;
   int count = 0;
   if (w == 0 && n < a.rows) {
@@ -503,7 +501,11 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(LceRowArgs a) {
     sum = (double)loss;
     count = !off;
   }
-  if (a.total) lce_total(sum, count, a.mean, a.total);
+  if (a.total) {
+    sum = dpc_wave_sum(sum);
+    count = dpc_wave_sum(count);
+    if (threadIdx.x == 0) a.total[0] = (float)(sum / (a.mean ? (double)max(count, 1) : 1.0));
+  }
 }
 
 // P from e^(l - slab max) in fp16 to d in the operands' type, in place.  One thread per row and slab.
@@ -673,7 +675,11 @@ __global__ __launch_bounds__(1024) void lce_total_kernel(const float* loss, cons
     s += (double)loss[i];
     c += target[i] != ignore;
   }
-  lce_total(s, c, mean, total);
+  __shared__ double red[16];
+  __shared__ int redi[16];
+  s = dpc_block_sum(s, red);
+  c = dpc_block_sum(c, redi);
+  if (threadIdx.x == 0) total[0] = (float)(s / (mean ? (double)max(c, 1) : 1.0));
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------

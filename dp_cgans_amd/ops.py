@@ -60,6 +60,23 @@ def _chk(t, dtype, name):
         raise TypeError('%s must be %s, got %s' % (name, dtype, t.dtype))
 
 
+def _on(t, dev, dtype, name):
+    """Address of a tensor of ``dtype`` on GPU ``dev`` (None for None)."""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise TypeError('%s must be %s, got %s' % (name, dtype, t.dtype))
+    if t.get_device() != dev:
+        raise ValueError('%s must live on the GPU (cuda:%d), got %s' % (name, dev, t.device))
+    return t.data_ptr()
+
+
+def _rows_of(t, name):
+    if t.dim() != 2:
+        raise ValueError('%s must be a matrix, got %s' % (name, tuple(t.shape)))
+    return t.shape
+
+
 def _ld(t):
     """Leading dimension of a 2-D row-major view (unit stride along columns required)."""
     if t.dim() == 1:
@@ -685,33 +702,29 @@ def linear_cross_entropy(h, w, target, loss, ws, dh=None, dw=None, lse=None, tot
     h and w fp32, bf16 or fp16; dh of their type, dw too or fp32 (``accumulate``: added to); target int64 [T].
     ws: uint8 workspace of linear_cross_entropy_ws(T, D, V, h.dtype, grads, dw_f32, piece_rows) bytes.  See
     dpc_linear_cross_entropy for ignored rows, alignment and pieces."""
-    if h.dim() != 2 or w.dim() != 2 or h.shape[1] != w.shape[1]:
+    global _dev_index
+    (T, D), (V, D2) = _rows_of(h, 'h'), _rows_of(w, 'w')
+    if D != D2:
         raise ValueError('linear_cross_entropy: h must be [T, D] and w [V, D], got %s and %s' % (tuple(h.shape), tuple(w.shape)))
-    T, D, V = h.shape[0], h.shape[1], w.shape[0]
-    if h.dtype not in _TYPES:
-        raise TypeError('linear_cross_entropy: h must be fp32, bf16 or fp16, got %s' % h.dtype)
-    _chk(h, h.dtype, 'h')
-    _chk(w, h.dtype, 'w')
-    _chk(target, torch.int64, 'target')
-    for t, n, name in ((loss, T, 'loss'), (lse, T, 'lse'), (total, 1, 'total')):
-        if t is not None:
-            _chk(t, torch.float32, name)
-            if t.numel() != n or not t.is_contiguous():
-                raise ValueError('linear_cross_entropy: %s must be contiguous with %d entries' % (name, n))
-    if target.numel() != T or not target.is_contiguous():
-        raise ValueError('linear_cross_entropy: target must be contiguous with %d entries' % T)
+    dt, dev = h.dtype, h.get_device()
+    if dt not in _TYPES:
+        raise TypeError('linear_cross_entropy: h must be fp32, bf16 or fp16, got %s' % dt)
+    if dev < 0:
+        raise ValueError('h must live on the GPU')
     dw_f32 = dw is not None and dw.dtype == torch.float32
+    flat = [_on(t, dev, ty, name) for t, ty, name in ((target, torch.int64, 'target'), (loss, torch.float32, 'loss'), (lse, torch.float32, 'lse'),
+                                                      (total, torch.float32, 'total'), (ws, torch.uint8, 'ws'))]
+    for t, n, name in ((target, T, 'target'), (loss, T, 'loss'), (lse, T, 'lse'), (total, 1, 'total'), (ws, None, 'ws')):
+        if t is not None and (not t.is_contiguous() or (n is not None and t.numel() != n)):
+            raise ValueError('linear_cross_entropy: %s must be contiguous%s' % (name, '' if n is None else ' with %d entries' % n))
+    mats = [_on(t, dev, ty, name) for t, ty, name in ((h, dt, 'h'), (w, dt, 'w'), (dh, dt, 'dh'), (dw, torch.float32 if dw_f32 else dt, 'dw'))]
     for t, like, name in ((dh, h, 'dh'), (dw, w, 'dw')):
-        if t is not None:
-            _chk(t, torch.float32 if t is dw and dw_f32 else h.dtype, name)
-            if t.shape != like.shape:
-                raise ValueError('linear_cross_entropy: %s must be %s, got %s' % (name, tuple(like.shape), tuple(t.shape)))
-    _chk(ws, torch.uint8, 'ws')
-    if not ws.is_contiguous():
-        raise ValueError('linear_cross_entropy: ws must be contiguous')
-    lib().call('dpc_linear_cross_entropy', _p(h), _ld(h), _p(w), _ld(w), _TYPES[h.dtype], _p(target), int(ignore_index), T, D, V, _p(loss),
-               _p(lse), _p(total), _p(dh), _ld(dh) if dh is not None else 0, _p(dw), _ld(dw) if dw is not None else 0, int(dw_f32),
-               int(bool(accumulate)), float(gscale), int(bool(mean)), int(piece_rows), _p(ws), ws.numel(), _stream())
+        if t is not None and t.shape != like.shape:
+            raise ValueError('linear_cross_entropy: %s must be %s, got %s' % (name, tuple(like.shape), tuple(t.shape)))
+    _dev_index = dev
+    lib().call('dpc_linear_cross_entropy', mats[0], _ld(h), mats[1], _ld(w), _TYPES[dt], flat[0], int(ignore_index), T, D, V, flat[1],
+               flat[2], flat[3], mats[2], _ld(dh) if dh is not None else 0, mats[3], _ld(dw) if dw is not None else 0, int(dw_f32),
+               int(bool(accumulate)), float(gscale), int(bool(mean)), int(piece_rows), flat[4], ws.numel(), _stream())
     return loss
 
 
