@@ -686,14 +686,18 @@ __global__ __launch_bounds__(1024) void lce_total_kernel(const float* loss, cons
 static int64_t lce_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 static int lce_size(int dtype) { return dtype == DPC_F32 ? 4 : 2; }
 
-// Tiles of a product: 256 x 256 wherever that makes at least 192 of them; else 128 x 128, four times as many and three to a
-// CU; at most 64 rows of logits, which are bound by reading W once, 128 entries x 64 rows, four to a CU.
+// Tiles of a product.  256 x 256 where that makes enough of them; else 128 x 128, four times as many and three to a CU; at
+// most 64 rows of logits, which are bound by reading W once, 128 entries x 64 rows.  Enough is half a round of the chip for
+// the logits (width 1024: 500 x 18000, 142 tiles, 32 against 38 us, 256 x 18000, 71 tiles, 30 against 26), and for the
+// gradients, whose K - vocabulary or rows - is cut into ranges, 192 of at least 1024 each (all of the call, width 256:
+// 1531 x 18000, dW with 71, 129 against 124 us; 4096 x 18000, dW with 284, 227 against 248; dh with 4, 73 against 59).
 enum { LCE_BIG = 0, LCE_MID = 1, LCE_ROW = 2 };
 static int64_t lce_tiles(int64_t M, int64_t N, int64_t bm, int64_t bn) { return dpc_cdiv(M, bm) * dpc_cdiv(N, bn); }
-static int lce_tile_kind(int64_t M, int64_t N, bool logits) {
-  if (logits && N <= 64) return LCE_ROW;
-  return lce_tiles(M, N, 256, 256) >= 192 ? LCE_BIG : LCE_MID;
+static int lce_tile_logits(int64_t V, int64_t rows) {
+  if (rows <= 64) return LCE_ROW;
+  return lce_tiles(V, rows, 256, 256) >= 128 ? LCE_BIG : LCE_MID;
 }
+static int lce_tile_grad(int64_t M, int64_t N, int64_t K) { return lce_tiles(M, N, 256, 256) * (K < 1024 ? 1 : K / 1024) >= 192 ? LCE_BIG : LCE_MID; }
 static int lce_slab_rows(int kind) { return kind == LCE_BIG ? 128 : 64; }
 
 // The tiles of a product that make whole rounds of the chip (256 CUs, `per` blocks each), and the K ranges of the others:
@@ -756,14 +760,13 @@ static LceLayout lce_layout(int64_t T, int D, int V, int dtype, bool grads, bool
       l.hm = take(l.rows * (int64_t)D * 4);
     }
   } else {
-    l.tile_l = lce_tile_kind(V, l.rows, true);
+    l.tile_l = lce_tile_logits(V, l.rows);
     l.stat = take(dpc_cdiv(V, lce_slab_rows(l.tile_l)) * l.prow * 8);
     if (grads) {
       l.P = take(lce_up(V, 256) * l.prow * 2);
       l.hm = take(l.prow * (int64_t)D * 2);
-      // (dh's K is the vocabulary: 256 x 256 tiles also where they are few, if K can be cut into as many ranges as fill the chip)
-      l.tile_h = lce_tiles(D, l.rows, 256, 256) * (V / 1024) >= 192 ? LCE_BIG : LCE_MID;
-      l.tile_w = lce_tile_kind(D, V, false);
+      l.tile_h = lce_tile_grad(D, l.rows, V);
+      l.tile_w = lce_tile_grad(D, V, l.prow);
       const LceCut h = lce_cut(lce_tiles(D, l.rows, lce_edge(l.tile_h), lce_edge(l.tile_h)), l.tile_h, V);
       const LceCut w = lce_cut(lce_tiles(D, V, lce_edge(l.tile_w), lce_edge(l.tile_w)), l.tile_w, l.prow);
       // (the last piece has fewer rows: fewer tiles of dh, then cut into more ranges - a round of them at most)
