@@ -20,7 +20,8 @@
 // of the dh product's operand and, transposed on the way out of LDS, m-runs of dW's; step 1 and 3 touch it in runs of
 // consecutive rows.
 //
-// fp32 operands: the products are dpc_gemm_f32_ex's (fp32 matrix cores), the logits of a piece in fp32.
+// fp32 operands: the products are dpc_gemm_f32_ex's (fp32 matrix cores), the logits of a piece in fp32.  Pieces of up to 16 rows
+// have kernels of their own for what reads or writes all of W once.
 #include "dpc_common.h"
 #include "../../include/dpcgan_hip.h"
 #include <math.h>
@@ -651,10 +652,92 @@ __global__ __launch_bounds__(256) void lce_d_f32_kernel(float* logits, int64_t l
 __global__ __launch_bounds__(256) void lce_fold_f32_kernel(const float* slabs, int64_t slab, int splits, int M, float* out, int64_t ldo) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < slab; i += (int64_t)gridDim.x * 256) {
     float v = slabs[i];
-#pragma unroll 4
+#pragma unroll 16
     for (int s = 1; s < splits; ++s) v += slabs[s * slab + i];
     const int64_t n = i / M;
     out[n * ldo + (i - n * M)] = v;
+  }
+}
+
+// At most 16 rows: reading W once - writing dW once - is all there is to it.  The logits take one wave per block and no LDS: a
+// lane's 16 bytes of W are four k-steps of v_mfma_f32_16x16x4_f32 (step s takes element s of every lane, of W and of h alike),
+// and a wave has 16 of them on their way.  One row, width 2048, vocabulary 131072 (1.07 GB): logits 547 -> 250 us (4.3 TB/s), dW
+// 557 -> 161 against the tiled products; dh by these means took what the tiled product with its K cut takes, 260.  With 17 to
+// 64 rows the logits were slower: too few waves for their work.
+#define LCE_FEW 16
+template <bool VEC>
+__device__ __forceinline__ f32x4 lce_load4(const float* p, int left) {               // elements [0, left) of 4, 0 for the others
+  if (VEC) return left > 0 ? *reinterpret_cast<const f32x4*>(p) : f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e < left) x[e] = p[e];
+  return x;
+}
+// logits[n][v] = h w^T, 32 vocabulary entries per wave.  VEC: rows 16-byte aligned, of whole 16 bytes.
+template <bool VEC>
+__global__ __launch_bounds__(64) void lce_few_logits_kernel(const float* w, int64_t ldw, const float* h, int64_t ldh, int rows, int D, int V, float* out,
+                                                            int64_t ldo) {
+  constexpr int NI = 2, U = 8;
+  const int l16 = threadIdx.x & 15, G = threadIdx.x >> 4, v0 = blockIdx.x * 16 * NI;
+  const float *pw[NI], *ph = h + (int64_t)min(l16, rows - 1) * ldh + 4 * G;           // (past the last row: that row again, and not stored)
+#pragma unroll
+  for (int i = 0; i < NI; ++i) pw[i] = w + (int64_t)min(v0 + i * 16 + l16, V - 1) * ldw + 4 * G;
+  f32x4 acc[NI] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  for (int k = 0; k < D; k += 16 * U) {
+    f32x4 a[U][NI];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < NI; ++i) a[u][i] = lce_load4<VEC>(pw[i] + k + 16 * u, D - k - 16 * u - 4 * G);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const f32x4 b = lce_load4<VEC>(ph + k + 16 * u, D - k - 16 * u - 4 * G);
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int i = 0; i < NI; ++i) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[u][i][s], b[s], acc[i], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int v = v0 + i * 16 + 4 * G;                                 // (ldo is a multiple of 4 and holds V)
+    if (l16 < rows && v < V) *reinterpret_cast<f32x4*>(out + (int64_t)l16 * ldo + v) = acc[i];
+  }
+}
+// dw[v][c] (+)= sum over the rows of d[n][v] hm[n][c]: a wave keeps 4 columns of every row per lane and walks 16 vocabulary entries.
+template <int NR, bool VEC>
+__global__ __launch_bounds__(256) void lce_few_dw_kernel(const float* __restrict__ d, int64_t ldd, const float* __restrict__ hm, int rows, int D, int V, int add,
+                                                         float* dw, int64_t lddw) {
+  __shared__ __attribute__((aligned(16))) float dv[64][NR + 4];         // d of this block's 64 entries
+  const int cols = (D + 255) / 256, vb = blockIdx.x / cols, c = (blockIdx.x - vb * cols) * 256 + (threadIdx.x & 63) * 4, left = D - c;
+  for (int i = threadIdx.x; i < 64 * NR; i += 256) {
+    const int n = i >> 6, v = vb * 64 + (i & 63);
+    dv[i & 63][n] = n < rows && v < V ? d[(int64_t)n * ldd + v] : 0.f;
+  }
+  f32x4 x[NR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) x[n] = lce_load4<VEC>(hm + (int64_t)n * D + c, n < rows ? left : 0);
+  __syncthreads();
+  if (left <= 0) return;
+  const int first = (threadIdx.x >> 6) * 16;
+  for (int k = first; k < first + 16 && vb * 64 + k < V; ++k) {
+    float* o = dw + (int64_t)(vb * 64 + k) * lddw + c;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < NR; n += 4) {
+      const f32x4 q = *reinterpret_cast<const f32x4*>(&dv[k][n]);
+#pragma unroll
+      for (int m = 0; m < 4; ++m) y += q[m] * x[n + m];
+    }
+    if (add) y += lce_load4<VEC>(o, left);
+    if (VEC) {
+      *reinterpret_cast<f32x4*>(o) = y;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) o[e] = y[e];
+    }
   }
 }
 
@@ -917,10 +1000,18 @@ static int lce_full(const LceCall& c, const LceLayout& l, hipStream_t st) {
     ra.stat = (f32x2*)(c.ws + l.stat); ra.prow = l.prow; ra.slabs = segs; ra.rows = rows; ra.V = c.V; ra.lt = (float*)(c.ws + l.lt);
     ra.target = c.target + r0; ra.ignore = c.ignore; ra.loss = c.loss + r0; ra.lse = c.lse ? c.lse + r0 : nullptr;
     ra.live = grads ? (f32x2*)(c.ws + l.live) : nullptr; ra.pm1 = (float*)(c.ws + l.pm1);
-    // (64 x 64 tiles below 768 of 128 x 128: 500 x 18000 x 256 56 against 71 us; 4000 x 4000 x 512 166 against 162)
-    dpc_gemm_desc lg = lce_desc(rows, c.V, c.D, h, c.ldh, 1, w, 1, c.ldw, 0.f, P, l.ldp);
-    lg.tile = lce_tiles(rows, c.V, 128, 128) < 768 ? 64 : 128;
-    int rc = dpc_gemm_f32_ex(&lg, 1, st);
+    const bool few = l.rows <= LCE_FEW;
+    const bool vec = (((uintptr_t)h | (uintptr_t)w) & 15) == 0 && ((c.ldh | c.ldw | c.D) & 3) == 0;
+    int rc = DPC_OK;
+    if (few) {
+      const auto k = vec ? lce_few_logits_kernel<true> : lce_few_logits_kernel<false>;
+      hipLaunchKernelGGL(k, dim3((unsigned)dpc_cdiv(c.V, 32)), dim3(64), 0, st, w, c.ldw, h, c.ldh, rows, c.D, c.V, P, l.ldp);
+    } else {
+      // (64 x 64 tiles below 768 of 128 x 128: 500 x 18000 x 256 56 against 71 us; 4000 x 4000 x 512 166 against 162)
+      dpc_gemm_desc lg = lce_desc(rows, c.V, c.D, h, c.ldh, 1, w, 1, c.ldw, 0.f, P, l.ldp);
+      lg.tile = lce_tiles(rows, c.V, 128, 128) < 768 ? 64 : 128;
+      rc = dpc_gemm_f32_ex(&lg, 1, st);
+    }
     if (rc != DPC_OK) return rc;
     hipLaunchKernelGGL(lce_stat_f32_kernel, dim3((unsigned)segs * rows), dim3(256), 0, st, P, l.ldp, c.V, ra.target, (f32x2*)(c.ws + l.stat), l.prow,
                        (float*)(c.ws + l.lt));
@@ -932,15 +1023,21 @@ static int lce_full(const LceCall& c, const LceLayout& l, hipStream_t st) {
     if (c.dh) {
       float* dh = (float*)c.dh + r0 * c.lddh;
       const bool cut = l.splits > 1;
+      const int64_t slab = (int64_t)rows * c.D;
       dpc_gemm_desc d = lce_desc(rows, c.D, c.V, P, l.ldp, 1, w, c.ldw, 1, 0.f, cut ? (float*)(c.ws + l.part) : dh, cut ? c.D : c.lddh);
-      if (cut) { d.splitk = l.splits; d.tile = 64; d.split_slab = (int64_t)rows * c.D; }
+      if (cut) { d.splitk = l.splits; d.tile = 64; d.split_slab = slab; }
       rc = dpc_gemm_f32_ex(&d, 1, st);
       if (rc != DPC_OK) return rc;
       if (cut)
-        hipLaunchKernelGGL(lce_fold_f32_kernel, dim3(dpc_grid(d.split_slab, 256)), dim3(256), 0, st, (const float*)(c.ws + l.part), d.split_slab, l.splits,
-                           c.D, dh, c.lddh);
+        hipLaunchKernelGGL(lce_fold_f32_kernel, dim3(dpc_grid(slab, 256)), dim3(256), 0, st, (const float*)(c.ws + l.part), slab, l.splits, c.D, dh, c.lddh);
     }
-    if (c.dw) {
+    if (c.dw && few) {
+      const bool wide = ((uintptr_t)c.dw & 15) == 0 && ((c.lddw | c.D) & 3) == 0;
+      const auto k = rows <= 4 ? (wide ? lce_few_dw_kernel<4, true> : lce_few_dw_kernel<4, false>)
+                               : (wide ? lce_few_dw_kernel<16, true> : lce_few_dw_kernel<16, false>);
+      hipLaunchKernelGGL(k, dim3((unsigned)(dpc_cdiv(c.D, 256) * dpc_cdiv(c.V, 64))), dim3(256), 0, st, P, l.ldp, hm, rows, c.D, c.V, p > 0 || c.accumulate,
+                         (float*)c.dw, c.lddw);
+    } else if (c.dw) {
       const dpc_gemm_desc d = lce_desc(c.V, c.D, rows, P, 1, l.ldp, hm, c.D, 1, p > 0 || c.accumulate ? 1.f : 0.f, (float*)c.dw, c.lddw);
       rc = dpc_gemm_f32_ex(&d, 1, st);
       if (rc != DPC_OK) return rc;

@@ -124,6 +124,23 @@ def test_fp32_takes_any_width(ops, D, V):
     check(call(ops, h, w, target), Oracle(h, w, target))
 
 
+@pytest.mark.parametrize('T', [1, 4, 5, 16, 17])
+@pytest.mark.parametrize('D,V', [(1, 1), (4, 31), (3, 33), (64, 700), (100, 129), (257, 5000), (260, 64), (1000, 4097), (1024, 20000)])
+def test_few_rows_in_fp32(ops, T, D, V):
+    """Up to 16 rows, in whole 16 bytes or not; in rows that start anywhere; in pieces of 16; dW added to what is there."""
+    h, w, target = inputs(T, D, V, torch.float32, T + D + V)
+    ref = Oracle(h, w, target)
+    check(call(ops, h, w, target), ref)
+    apart = lambda x: torch.full((x.shape[0], D + 3), 7.0, device=DEV)[:, 1:1 + D].copy_(x)  # noqa: E731
+    check(call(ops, apart(h), apart(w), target, dh=apart(h), dw=apart(w)), ref)
+    big = torch.cat([h] * 3 + [h[:1]]), torch.cat([target] * 3 + [target[:1]])
+    more = Oracle(big[0], w, big[1])
+    dw = torch.randn(V, D, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    more.dw = more.dw + dw.double()
+    more.edw32 = more.edw32 + 8 * U * (more.dw.abs() + dw.double().abs())          # (each of at most four pieces adds with one rounding)
+    check(call(ops, big[0], w, big[1], dw=dw, accumulate=True, piece_rows=16), more)
+
+
 @pytest.mark.parametrize('dtype', TYPES)
 def test_strided_rows_and_what_lies_between_them(ops, dtype):
     """Rows inside wider buffers; everything outside the outputs' own columns keeps its bits."""
