@@ -41,6 +41,8 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 #define LCE_LOG2E 1.4426950408889634f
 #define LCE_LN2 0.6931471805599453f
 
+#define LCE_FEW 16              // rows of a piece that the few-rows kernels take: one 16 x 16 block of a matrix instruction
+
 enum { LCE_LOGITS = 0, LCE_DH = 1, LCE_DW = 2 };
 
 // 16-bit element types and their matrix instruction.  16 x 16 x 32 and not 32 x 32 x 16: the chip lowers its clock under
@@ -125,6 +127,70 @@ typedef std::integral_constant<bool, false> No;
 template <int N>
 __device__ __forceinline__ void lce_wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
+// A wave's 16 SM x 16 SN logits: (reference, sum) of its slab for each row, the target's logit, and what is left of them in P.
+// C layout of a 16 x 16 block: n = lane & 15 (nw has it), m = 4 (lane >> 4) + e.
+template <int SM, int SN>
+__device__ __forceinline__ void lce_logits_end(const LceArgs& g, f32x4 (&acc)[SM][SN], int mw, int nw, int G) {
+  if (mw + SM * 16 > g.M) {
+#pragma unroll
+    for (int i = 0; i < SM; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (mw + i * 16 + 4 * G + e >= g.M)
+#pragma unroll
+          for (int j = 0; j < SN; ++j) acc[i][j][e] = -INFINITY;
+  }
+#pragma unroll
+  for (int j = 0; j < SN; ++j) {
+    const int n = nw + j * 16;
+    const int64_t t = n < g.N ? g.target[n] : -1;
+    if (__any(t >= mw && t < mw + SM * 16)) {
+      const int at = t >= mw && t < mw + SM * 16 ? (int)(t - mw) : -1;
+#pragma unroll
+      for (int i = 0; i < SM; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (at == i * 16 + 4 * G + e) g.lt[n] = acc[i][j][e];
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < SM; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64)) * LCE_LOG2E;
+    // the reference: the largest logit, rounded; what follows is exact relative to it.  (All -inf: 2^(l - 0) = 0, not NaN.)
+    const float ref = top == -INFINITY ? 0.f : top;
+    f32x4 run = {0.f, 0.f, 0.f, 0.f};                                // (four short sums: a sure row's is 1 and what little there is beside it)
+#pragma unroll
+    for (int i = 0; i < SM; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], LCE_LOG2E, -ref));
+      run += acc[i][j];
+    }
+    float sum = (run.x + run.y) + (run.z + run.w);
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (G == 0 && mw < g.M) g.stat[(int64_t)(mw / (SM * 16)) * g.prow + n] = f32x2{ref, sum};
+    if (g.grads) {
+#pragma unroll
+      for (int i = 0; i < SM; i += 2) {
+        u32x2 x[2];
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const f16x2 v = {(_Float16)acc[i + w][j][2 * c], (_Float16)acc[i + w][j][2 * c + 1]};
+            x[w][c] = __builtin_bit_cast(uint32_t, v);
+          }
+        // (past the caches: nothing reads P before all of it is there - 8192 x 131072: 3.84 -> 3.57 ms)
+        __builtin_nontemporal_store(lce_pair(x[0], x[1]),
+                                    reinterpret_cast<u32x4*>(g.P + ((int64_t)((mw + (i + (G & 1)) * 16) / 8 + (G >> 1)) * g.prow + n) * 16));
+      }
+    }
+  }
+}
+
 // One BM x BN tile of a product, WM x WN waves.  A tile of an operand is 32 k; it goes from memory straight into LDS, 16
 // bytes per lane, in one of three images:
 //   k-runs  (W and h of LOGITS, P of DH): [row][4 chunks of 8 k], chunk c of row r at c ^ (r / 2 & 3) - read 16 bytes a lane
@@ -133,10 +199,10 @@ __device__ __forceinline__ void lce_wait_vm() { asm volatile("s_waitcnt vmcnt(%0
 // The transposing read gives lane i of 16 the column i of a 4 x 16 block whose row r comes from lanes 4r .. 4r+3; the
 // swizzles put what the 32 lanes of one LDS cycle read on different banks.
 //
-// NS = 3 tiles are in use or on their way - 6 for the few rows, where the loads of W are all there is to wait for (4 x 256 x
-// 18000: 8.1 -> 6.5 us).  Iteration kt: while the products of the wave's upper rows run, its lower rows' fragments are
-// read; then, once tile kt + 1 has landed for every wave and tile kt has been read by all (one barrier), tile kt + NS goes
-// on its way into the freed slot and the next tile's first fragments are read while the lower rows' products run.
+// NS = 3 tiles are in use or on their way.  Iteration kt: while the products of the wave's upper rows run, its lower rows'
+// fragments are read; then, once tile kt + 1 has landed for every wave and tile kt has been read by all (one barrier),
+// tile kt + NS goes on its way into the freed slot and the next tile's first fragments are read while the lower rows'
+// products run.
 //
 // 256 x 256 with 8 waves of 128 x 64 (196 registers, 96 KB of LDS, one block per CU) on 8192 rows, width 2048, vocabulary
 // 131072: 1230 (logits), 1380 (dh) and 1345 (dW) TFLOP/s where a library product of the same shape reaches 1374 to 1594 and
@@ -150,7 +216,7 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
   constexpr int NT = WM * WN * 64;
   constexpr int SM = BM / WM / 16, SN = BN / WN / 16, SH = SM / 2;
   constexpr int NA = BM * 4 / NT, NB = BN * 4 / NT;
-  constexpr int SLOT = (BM + BN) * 64, NS = BN == 64 ? 6 : 3;
+  constexpr int SLOT = (BM + BN) * 64, NS = 3;
   constexpr bool A_K = MODE == LCE_LOGITS, B_K = MODE != LCE_DW;
   __shared__ __attribute__((aligned(1024))) char lds[NS * SLOT];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -332,65 +398,7 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
   // C layout of a 16 x 16 block: n = lane & 15, m = 4 (lane >> 4) + e
   const int mw = m0 + wm * SM * 16, nw = n0 + wn * SN * 16 + l16;
   if (MODE == LCE_LOGITS) {
-    if (mw + SM * 16 > g.M) {
-#pragma unroll
-      for (int i = 0; i < SM; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (mw + i * 16 + 4 * G + e >= g.M)
-#pragma unroll
-            for (int j = 0; j < SN; ++j) acc[i][j][e] = -INFINITY;
-    }
-#pragma unroll
-    for (int j = 0; j < SN; ++j) {
-      const int n = nw + j * 16;
-      if (BN == 64 && n - l16 >= g.N) break;                           // (few rows: the rest of the tile is empty)
-      const int64_t t = n < g.N ? g.target[n] : -1;
-      if (__any(t >= mw && t < mw + SM * 16)) {
-        const int at = t >= mw && t < mw + SM * 16 ? (int)(t - mw) : -1;
-#pragma unroll
-        for (int i = 0; i < SM; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (at == i * 16 + 4 * G + e) g.lt[n] = acc[i][j][e];
-      }
-      float top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < SM; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64)) * LCE_LOG2E;
-      // the reference: the largest logit, rounded; what follows is exact relative to it.  (All -inf: 2^(l - 0) = 0, not NaN.)
-      const float ref = top == -INFINITY ? 0.f : top;
-      f32x4 run = {0.f, 0.f, 0.f, 0.f};                                // (four short sums: a sure row's is 1 and what little there is beside it)
-#pragma unroll
-      for (int i = 0; i < SM; ++i) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], LCE_LOG2E, -ref));
-        run += acc[i][j];
-      }
-      float sum = (run.x + run.y) + (run.z + run.w);
-      sum += __shfl_xor(sum, 16, 64);
-      sum += __shfl_xor(sum, 32, 64);
-      if (G == 0 && mw < g.M) g.stat[(int64_t)(mw / (SM * 16)) * g.prow + n] = f32x2{ref, sum};
-      if (g.grads) {
-#pragma unroll
-        for (int i = 0; i < SM; i += 2) {
-          u32x2 x[2];
-#pragma unroll
-          for (int w = 0; w < 2; ++w)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const f16x2 v = {(_Float16)acc[i + w][j][2 * c], (_Float16)acc[i + w][j][2 * c + 1]};
-              x[w][c] = __builtin_bit_cast(uint32_t, v);
-            }
-          // (past the caches: nothing reads P before all of it is there - 8192 x 131072: 3.84 -> 3.57 ms)
-          __builtin_nontemporal_store(lce_pair(x[0], x[1]),
-                                      reinterpret_cast<u32x4*>(g.P + ((int64_t)((mw + (i + (G & 1)) * 16) / 8 + (G >> 1)) * g.prow + n) * 16));
-        }
-      }
-    }
+    lce_logits_end<SM, SN>(g, acc, mw, nw, G);
   } else {
     if (tl >= g.whole) {
       float* q = g.part + ((int64_t)(split * rest + tl - g.whole) * BN + wn * SN * 16 + l16) * BM + wm * SM * 16 + 4 * G;
@@ -435,6 +443,38 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
       }
     }
   }
+}
+
+// Logits of at most 16 rows: reading W once is all there is to it.  One wave per block takes 64 vocabulary entries and no LDS: a
+// lane's 16 bytes of W are one operand of a matrix instruction, and 32 of them are on their way.  One row, vocabulary 131072,
+// width 2048: 135 us for the call (4.0 TB/s), 144 with tiles through LDS; 4 x 256 x 18000 in a graph 8.9 against 10.0 us.
+template <typename E>
+__global__ __launch_bounds__(64) void lce_few_kernel(LceArgs g) {
+  using H = Half<E>;
+  constexpr int SM = 4, U = 8;
+  const int l16 = threadIdx.x & 15, G = threadIdx.x >> 4, mw = blockIdx.x * 16 * SM;
+  const char *pa[SM], *pb = g.B + (int64_t)min(l16, g.N - 1) * g.ldb + G * 16;        // (past the last row or entry: that one again, and not used)
+#pragma unroll
+  for (int i = 0; i < SM; ++i) pa[i] = g.A + (int64_t)min(mw + i * 16 + l16, g.M - 1) * g.lda + G * 16;
+  f32x4 acc[SM][1];
+#pragma unroll
+  for (int i = 0; i < SM; ++i) acc[i][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < g.K; k += 32 * U) {
+    u32x4 a[U][SM], b[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = k + 32 * u + 8 * G < g.K;
+      b[u] = in ? *reinterpret_cast<const u32x4*>(pb + (k + 32 * u) * 2) : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int i = 0; i < SM; ++i) a[u][i] = in ? *reinterpret_cast<const u32x4*>(pa[i] + (k + 32 * u) * 2) : u32x4{0u, 0u, 0u, 0u};
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < SM; ++i)
+        acc[i][0] = H::mfma(__builtin_bit_cast(typename H::v8, a[u][i]), __builtin_bit_cast(typename H::v8, b[u]), acc[i][0]);
+  }
+  lce_logits_end<SM, 1>(g, acc, mw, l16, G);
 }
 
 // ---- the passes between the products --------------------------------------------------------------------------------
@@ -664,7 +704,6 @@ __global__ __launch_bounds__(256) void lce_fold_f32_kernel(const float* slabs, i
 // and a wave has 16 of them on their way.  One row, width 2048, vocabulary 131072 (1.07 GB): logits 547 -> 250 us (4.3 TB/s), dW
 // 557 -> 161 against the tiled products; dh by these means took what the tiled product with its K cut takes, 260.  With 17 to
 // 64 rows the logits were slower: too few waves for their work.
-#define LCE_FEW 16
 template <bool VEC>
 __device__ __forceinline__ f32x4 lce_load4(const float* p, int left) {               // elements [0, left) of 4, 0 for the others
   if (VEC) return left > 0 ? *reinterpret_cast<const f32x4*>(p) : f32x4{0.f, 0.f, 0.f, 0.f};
@@ -769,15 +808,15 @@ __global__ __launch_bounds__(1024) void lce_total_kernel(const float* loss, cons
 static int64_t lce_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 static int lce_size(int dtype) { return dtype == DPC_F32 ? 4 : 2; }
 
-// Tiles of a product.  256 x 256 where that makes enough of them; else 128 x 128, four times as many and three to a CU; at
-// most 64 rows of logits, which are bound by reading W once, 128 entries x 64 rows.  Enough is half a round of the chip for
+// Tiles of a product.  256 x 256 where that makes enough of them; else 128 x 128, four times as many and three to a CU; a
+// kernel of their own for few rows of logits.  Enough is half a round of the chip for
 // the logits (width 1024: 500 x 18000, 142 tiles, 32 against 38 us, 256 x 18000, 71 tiles, 30 against 26), and for the
 // gradients, whose K - vocabulary or rows - is cut into ranges, 192 of at least 1024 each (all of the call, width 256:
 // 1531 x 18000, dW with 71, 129 against 124 us; 4096 x 18000, dW with 284, 227 against 248; dh with 4, 73 against 59).
 enum { LCE_BIG = 0, LCE_MID = 1, LCE_ROW = 2 };
 static int64_t lce_tiles(int64_t M, int64_t N, int64_t bm, int64_t bn) { return dpc_cdiv(M, bm) * dpc_cdiv(N, bn); }
 static int lce_tile_logits(int64_t V, int64_t rows) {
-  if (rows <= 64) return LCE_ROW;
+  if (rows <= LCE_FEW) return LCE_ROW;
   return lce_tiles(V, rows, 256, 256) >= 128 ? LCE_BIG : LCE_MID;
 }
 static int lce_tile_grad(int64_t M, int64_t N, int64_t K) { return lce_tiles(M, N, 256, 256) * (K < 1024 ? 1 : K / 1024) >= 192 ? LCE_BIG : LCE_MID; }
@@ -903,7 +942,7 @@ template <typename E, int MODE>
 static void lce_launch(LceArgs& g, int kind, hipStream_t st) {
   if (kind == LCE_BIG) lce_launch_tile<E, MODE, 256, 256, 2, 4>(g, kind, st);
   else if (kind == LCE_MID) lce_launch_tile<E, MODE, 128, 128, 2, 2>(g, kind, st);
-  else if constexpr (MODE == LCE_LOGITS) lce_launch_tile<E, MODE, 128, 64, 2, 1>(g, kind, st);
+  else if constexpr (MODE == LCE_LOGITS) hipLaunchKernelGGL(lce_few_kernel<E>, dim3((unsigned)dpc_cdiv(g.M, 64)), dim3(64), 0, st, g);
 }
 
 struct LceCall {

@@ -141,6 +141,21 @@ def test_few_rows_in_fp32(ops, T, D, V):
     check(call(ops, big[0], w, big[1], dw=dw, accumulate=True, piece_rows=16), more)
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('T', [1, 5, 16, 17])
+@pytest.mark.parametrize('D,V', [(8, 1), (8, 63), (40, 65), (256, 129), (264, 5000), (1032, 700)])
+def test_few_rows_in_half_precision(ops, T, D, V, dtype):
+    """Up to 16 rows, also as pieces of a longer call."""
+    h, w, target = inputs(T, D, V, dtype, T + D + V)
+    ref = Oracle(h, w, target)
+    o = call(ops, h, w, target)
+    check(o, ref)
+    alone = call(ops, h, w, target, grads=False)
+    assert torch.equal(alone['loss'], o['loss']) and torch.equal(alone['lse'], o['lse']) and torch.equal(alone['total'], o['total'])
+    big = torch.cat([h] * 2 + [h[:1]]), torch.cat([target] * 2 + [target[:1]])
+    check(call(ops, big[0], w, big[1], piece_rows=16), Oracle(big[0], w, big[1]))
+
+
 @pytest.mark.parametrize('dtype', TYPES)
 def test_strided_rows_and_what_lies_between_them(ops, dtype):
     """Rows inside wider buffers; everything outside the outputs' own columns keeps its bits."""
