@@ -13,7 +13,7 @@
 //      target's place, exactly 0 in rows that are ignored.
 //   4. dh and dW as products over d.  dW of several pieces adds up in fp32.
 // That is 6 T V D flops.  They bound it for widths in the thousands (6 D flops against the 10 bytes per logit that writing
-// P, turning it into d and reading it twice move: 8192 x 2048 x 131072 spends 3.6 + 0.8 + 3.2 + 3.25 ms on steps 1, 3 and
+// P, turning it into d and reading it twice move: 8192 x 2048 x 131072 spends 3.6 + 0.8 + 3.0 + 3.1 ms on steps 1, 3 and
 // 4); below a width of about 500 the traffic does.
 //
 // P's layout [vocabulary / 8][row][8 entries] serves all three products: 16-byte chunks of 8 vocabulary entries are k-runs
@@ -204,12 +204,15 @@ __device__ __forceinline__ void lce_logits_end(const LceArgs& g, f32x4 (&acc)[SM
 // tile kt + NS goes on its way into the freed slot and the next tile's first fragments are read while the lower rows'
 // products run.
 //
-// 256 x 256 with 8 waves of 128 x 64 (196 registers, 96 KB of LDS, one block per CU) on 8192 rows, width 2048, vocabulary
-// 131072: 1230 (logits), 1380 (dh) and 1345 (dW) TFLOP/s where a library product of the same shape reaches 1374 to 1594 and
-// nothing but matrix instructions 1946.  The clock is down to 1.82 GHz under that load and the matrix units are busy 72 % of
-// it; LDS is not what they wait for (no bank conflicts, 0.4 of its cycles).  Measured and dropped: 4 waves of 128 x 128
-// (spills, or the same), two 4-wave blocks per CU (dh 1.3 times as long), four and five tiles in LDS (the same), one barrier
-// per 64 k (dW 4 % faster, the others 6 to 9 % slower: less time for the loads), blocks started at different times.
+// 256 x 256 with 8 waves of 128 x 64 for the logits (a wave's 128 entries are a slab) and of 64 x 128 for the gradients, whose
+// transposed reads of A take two instructions each (dh 2 % faster); 200 registers, 96 KB of LDS, one block per CU.  On 8192
+// rows, width 2048, vocabulary 131072: 1225 (logits), 1470 (dh) and 1430 (dW) TFLOP/s where a library product of the same shape
+// reaches 1374 to 1594 and nothing but matrix instructions 1946.  What limits it is power first: the clock falls to 1.8 GHz,
+// and with all operands 0 the same instructions take 17 to 24 % less time at 2.4.  Then the steps between the products: the
+// matrix units are busy 75 % of the cycles, 80 % without the reads of LDS, 97 % without loads and reads.  Measured and
+// dropped: 4 waves of 128 x 128 (spills, or the same), two 4-wave blocks per CU (dh 1.3 times as long), four and five tiles in
+// LDS (the same), one barrier per 64 k (dW 4 % faster, the others 6 to 9 % slower), blocks started at different times, both
+// halves of W's lines at once (half the requests to L2, logits 2 % slower), slots as constants in a loop over three tiles (spills).
 template <typename E, int MODE, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
   using H = Half<E>;
@@ -338,9 +341,10 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
 #pragma unroll
     for (int j = 0; j < SN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   typename H::v8 a0[SH], a1[SH], b[SN];
-  // One half of a tile's products with the reads of the next half, and a tile's loads, between them: a wave that waits for
-  // the matrix unit has them behind it.  In this order, pinned: what stands before the first product after a barrier holds
-  // up every wave at once.  Column by column, so that b[j] is free for the next tile's once its products have been issued.
+  // One half of a tile's products with the reads of the next half, and a tile's loads, evenly between them: a wave that waits
+  // for the matrix unit has them behind it.  In this order, pinned, each product first: what stands before the first one
+  // after a barrier holds up every wave at once.  Column by column, so that b[j] is free for the next tile's once its products
+  // have been issued.
   const auto half_tile = [&](auto lower, auto more, auto load, const char* buf, int kt, char* into) {
     constexpr bool LOW = decltype(lower)::value, MORE = decltype(more)::value, LOAD = decltype(load)::value;
     constexpr int SLOTS = SH * SN, L = NA + NB;
@@ -349,14 +353,19 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
 #pragma unroll
       for (int i = 0; i < SH; ++i) {
         acc[(LOW ? SH : 0) + i][j] = H::mfma((LOW ? a1 : a0)[i], b[j], acc[(LOW ? SH : 0) + i][j]);
+        __builtin_amdgcn_sched_barrier(0);
         const int p = j * SH + i;
-        if (!LOW && p < SH) a1[p < SH ? p : 0] = frag_a(buf, SH + p);
-        if (LOW && MORE && (p & 1) == 0 && p / 2 < SH) a0[p / 2 < SH ? p / 2 : 0] = frag_a(buf, p / 2);
+#pragma unroll
+        for (int q = 0; q < SH; ++q)
+          if (p == q * SLOTS / SH) {
+            if (!LOW) a1[q] = frag_a(buf, SH + q);
+            else if (MORE) a0[q] = frag_a(buf, q);
+          }
         if (LOW && MORE && i == SH - 1) b[j] = frag_b(buf, j);
         if (LOAD) {
 #pragma unroll
           for (int l = 0; l < L; ++l)
-            if (l * SLOTS / L + 1 == p) issue_one(kt, into, l);
+            if (l * SLOTS / L + SLOTS / L / 2 == p) issue_one(kt, into, l);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -386,11 +395,14 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
       const int nxt = cur + 1 == NS ? 0 : cur + 1;
       half_tile(No(), No(), No(), lds + cur * SLOT, 0, nullptr);
       if (decltype(more)::value) meet(ahead);
-      if (decltype(load)::value && kt + NS == kt_cut) cut();
       half_tile(Yes(), more, load, lds + nxt * SLOT, kt + NS, lds + cur * SLOT);
       cur = nxt;
     };
-    for (; kt + NS < nk; ++kt) tile(Yes(), Yes(), true);
+    // (where K ends inside a tile the offsets of its loads change before them - outside of the loop, in which the test cost 1 %)
+    for (int pass = kt_cut < NS; pass < 2; ++pass) {
+      if (pass && kt_cut >= NS) cut();
+      for (const int end = (pass ? nk : kt_cut) - NS; kt < end; ++kt) tile(Yes(), Yes(), true);
+    }
     for (; kt + 1 < nk; ++kt) tile(Yes(), No(), kt + NS - 1 < nk);           // nothing more to load
     tile(No(), No(), false);
   }
@@ -940,7 +952,7 @@ static void lce_launch_tile(LceArgs& g, int kind, hipStream_t st) {
 }
 template <typename E, int MODE>
 static void lce_launch(LceArgs& g, int kind, hipStream_t st) {
-  if (kind == LCE_BIG) lce_launch_tile<E, MODE, 256, 256, 2, 4>(g, kind, st);
+  if (kind == LCE_BIG) lce_launch_tile<E, MODE, 256, 256, MODE == LCE_LOGITS ? 2 : 4, MODE == LCE_LOGITS ? 4 : 2>(g, kind, st);
   else if (kind == LCE_MID) lce_launch_tile<E, MODE, 128, 128, 2, 2>(g, kind, st);
   else if constexpr (MODE == LCE_LOGITS) hipLaunchKernelGGL(lce_few_kernel<E>, dim3((unsigned)dpc_cdiv(g.M, 64)), dim3(64), 0, st, g);
 }
