@@ -561,16 +561,41 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(LceRowArgs a) {
   }
 }
 
+// The losses of all rows of the call as one: their sum, over the rows that count if `mean`.  One block, in a fixed order: a launch
+// of its own for the loss alone, a block beside those that turn logits into d otherwise (a launch less: 5 us of 174 for fp32
+// 500 x 256 x 18000).
+struct LceTotal { const float* loss; const int64_t* target; int64_t T, ignore; int mean; float* total; };
+template <int NT>
+__device__ __forceinline__ void lce_total(const LceTotal& a) {
+  __shared__ double red[16];
+  __shared__ int redi[16];
+  double s = 0.0;
+  int c = 0;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < a.T; i += NT) {
+    s += (double)a.loss[i];
+    c += a.target[i] != a.ignore;
+  }
+  s = dpc_block_sum(s, red);
+  c = dpc_block_sum(c, redi);
+  if (threadIdx.x == 0) a.total[0] = (float)(s / (a.mean ? (double)max(c, 1) : 1.0));
+}
+
 // P from e^(l - slab max) in fp16 to d in the operands' type, in place.  One thread per row and slab.
 // NT: P is much larger than the 256 MB of the last-level cache - read and written past it (2 GB: 846 -> 780 us; 0.3 GB: 96 -> 103 us).
-// Blocks from `slabs` * prow / 256 on copy h with its ignored rows, and the rows up to the end of the piece's last tile, set to
-// 0: what such a row holds must not reach dW (0 x NaN).
+// `copies` blocks from `slabs` * prow / 256 on copy h with its ignored rows, and the rows up to the end of the piece's last tile,
+// set to 0: what such a row holds must not reach dW (0 x NaN).  One more of the last piece: the total.
 template <typename E, bool NT>
 __global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, const f32x2* stat, int slabs, int rows, int slab_rows, const f32x2* live,
-                                                        const float* pm1, const int64_t* target, const char* h, int64_t ldh, int row16, char* hm) {
+                                                        const float* pm1, const int64_t* target, const char* h, int64_t ldh, int row16, char* hm, int copies,
+                                                        LceTotal all) {
   const int first = slabs * (int)(prow / 256);
+  if ((int)blockIdx.x >= first + copies) {
+    lce_total<256>(all);
+    return;
+  }
   if ((int)blockIdx.x >= first) {
-    for (int64_t i = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x; i < prow * row16; i += (int64_t)(gridDim.x - first) * 256) {
+    for (int64_t i = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x; i < prow * row16; i += (int64_t)copies * 256) {
       const int n = (int)(i / row16), c = (int)(i - (int64_t)n * row16);
       u32x4 v = {0u, 0u, 0u, 0u};
       if (n < rows && live[n].y != 0.f) v = *reinterpret_cast<const u32x4*>(h + (int64_t)n * ldh + c * 16);
@@ -672,12 +697,16 @@ __global__ __launch_bounds__(256) void lce_stat_f32_kernel(const float* logits, 
   }
 }
 
-// Logits to alpha * d, in place; the blocks behind them copy h with its ignored rows set to 0.
+// Logits to alpha * d, in place; the `copies` blocks behind them copy h with its ignored rows set to 0, one more takes the total.
 __global__ __launch_bounds__(256) void lce_d_f32_kernel(float* logits, int64_t ld, int rows, int V, const int64_t* target, const f32x2* live, const float* pm1,
-                                                        const float* alpha, const float* h, int64_t ldh, int D, float* hm) {
+                                                        const float* alpha, const float* h, int64_t ldh, int D, float* hm, int copies, LceTotal all) {
   const int first = rows * ((V + LCE_SEG - 1) / LCE_SEG);
+  if ((int)blockIdx.x >= first + copies) {
+    lce_total<256>(all);
+    return;
+  }
   if ((int)blockIdx.x >= first) {
-    for (int64_t i = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x; i < (int64_t)rows * D; i += (int64_t)(gridDim.x - first) * 256) {
+    for (int64_t i = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x; i < (int64_t)rows * D; i += (int64_t)copies * 256) {
       const int64_t n = i / D;
       hm[i] = live[n].y != 0.f ? h[n * ldh + (i - n * D)] : 0.f;
     }
@@ -800,21 +829,7 @@ __global__ __launch_bounds__(256) void lce_zero_kernel(uint16_t* out, int64_t ld
   }
 }
 
-// sum of the rows' losses, over the rows that count if `mean` (one block, fixed order)
-__global__ __launch_bounds__(1024) void lce_total_kernel(const float* loss, const int64_t* target, int64_t T, int64_t ignore, int mean, float* total) {
-  double s = 0.0;
-  int c = 0;
-#pragma unroll 8
-  for (int64_t i = threadIdx.x; i < T; i += 1024) {
-    s += (double)loss[i];
-    c += target[i] != ignore;
-  }
-  __shared__ double red[16];
-  __shared__ int redi[16];
-  s = dpc_block_sum(s, red);
-  c = dpc_block_sum(c, redi);
-  if (threadIdx.x == 0) total[0] = (float)(s / (mean ? (double)max(c, 1) : 1.0));
-}
+__global__ __launch_bounds__(1024) void lce_total_kernel(LceTotal a) { lce_total<1024>(a); }
 
 // ---- host ------------------------------------------------------------------------------------------------------------
 static int64_t lce_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
@@ -966,6 +981,10 @@ struct LceCall {
   char* ws;
 };
 
+static LceTotal lce_all(const LceCall& c) { return LceTotal{c.loss, c.target, c.T, c.ignore, c.mean, c.total}; }
+// Whether piece `p` takes the total in the pass between the products.
+static int lce_takes_total(const LceCall& c, const LceLayout& l, int p) { return c.total && p + 1 == l.pieces && !(c.T <= 16 && l.pieces == 1); }
+
 // Rows of a piece: with the first one's the call's alpha, and the total where one block sees all rows.
 static void lce_rows(const LceCall& c, LceRowArgs& a, int piece, const LceLayout& l, hipStream_t st) {
   const bool begin = piece == 0 && (c.dh || c.dw);
@@ -1001,8 +1020,8 @@ static int lce_half(const LceCall& c, const LceLayout& l, hipStream_t st) {
     const auto scale = lce_up(c.V, 256) * l.prow * 2 > (1ll << 30) ? lce_scale_kernel<E, true> : lce_scale_kernel<E, false>;
     const int row16 = c.D / 8, copies = c.dw ? dpc_grid(l.prow * row16, 256) : 0;
     char* hm = c.ws + l.hm;
-    hipLaunchKernelGGL(scale, dim3((unsigned)(l.prow / 256 * slabs + copies)), dim3(256), 0, st, g.P, l.prow, g.stat, slabs, rows, slab_rows, ra.live,
-                       ra.pm1, g.target, h, c.ldh * 2, row16, hm);
+    hipLaunchKernelGGL(scale, dim3((unsigned)(l.prow / 256 * slabs + copies + lce_takes_total(c, l, p))), dim3(256), 0, st, g.P, l.prow, g.stat, slabs, rows,
+                       slab_rows, ra.live, ra.pm1, g.target, h, c.ldh * 2, row16, hm, copies, lce_all(c));
     if (c.dh) {
       LceArgs d = g;
       d.A = c.w; d.lda = c.ldw * 2; d.M = c.D; d.N = rows; d.K = c.V;
@@ -1069,8 +1088,8 @@ static int lce_full(const LceCall& c, const LceLayout& l, hipStream_t st) {
     lce_rows(c, ra, p, l, st);
     if (!grads) continue;
     const int copies = c.dw ? dpc_grid((int64_t)rows * c.D, 256) : 0;
-    hipLaunchKernelGGL(lce_d_f32_kernel, dim3((unsigned)segs * rows + copies), dim3(256), 0, st, P, l.ldp, rows, c.V, ra.target, ra.live, ra.pm1, head, h,
-                       c.ldh, c.D, hm);
+    hipLaunchKernelGGL(lce_d_f32_kernel, dim3((unsigned)segs * rows + copies + lce_takes_total(c, l, p)), dim3(256), 0, st, P, l.ldp, rows, c.V, ra.target, ra.live,
+                       ra.pm1, head, h, c.ldh, c.D, hm, copies, lce_all(c));
     if (c.dh) {
       float* dh = (float*)c.dh + r0 * c.lddh;
       const bool cut = l.splits > 1;
@@ -1135,7 +1154,7 @@ extern "C" int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* 
                        c.dw_f32 ? 2 * D : D);
   const int rc = T == 0 ? DPC_OK : f32 ? lce_full(c, l, st) : (dtype == DPC_BF16 ? lce_half<__bf16>(c, l, st) : lce_half<_Float16>(c, l, st));
   if (rc != DPC_OK) return rc;
-  if (total && (T == 0 || T > 16 || l.pieces > 1)) hipLaunchKernelGGL(lce_total_kernel, dim3(1), dim3(1024), 0, st, loss, target, T, ignore_index, mean, total);
+  if (total && (T == 0 || (!grads && (T > 16 || l.pieces > 1)))) hipLaunchKernelGGL(lce_total_kernel, dim3(1), dim3(1024), 0, st, lce_all(c));
   DPC_LAUNCH_CHECK();
   return DPC_OK;
 }
