@@ -71,6 +71,14 @@ def _on(t, dev, dtype, name):
     return t.data_ptr()
 
 
+def _vec(t, n, dev, dtype, name):
+    """Address of a contiguous tensor of n entries (any number if None)."""
+    p = _on(t, dev, dtype, name)
+    if t is not None and (not t.is_contiguous() or (n is not None and t.numel() != n)):
+        raise ValueError('%s must be contiguous%s' % (name, '' if n is None else ' with %d entries' % n))
+    return p
+
+
 def _rows_of(t, name):
     if t.dim() != 2:
         raise ValueError('%s must be a matrix, got %s' % (name, tuple(t.shape)))
@@ -711,20 +719,18 @@ def linear_cross_entropy(h, w, target, loss, ws, dh=None, dw=None, lse=None, tot
         raise TypeError('linear_cross_entropy: h must be fp32, bf16 or fp16, got %s' % dt)
     if dev < 0:
         raise ValueError('h must live on the GPU')
-    dw_f32 = dw is not None and dw.dtype == torch.float32
-    flat = [_on(t, dev, ty, name) for t, ty, name in ((target, torch.int64, 'target'), (loss, torch.float32, 'loss'), (lse, torch.float32, 'lse'),
-                                                      (total, torch.float32, 'total'), (ws, torch.uint8, 'ws'))]
-    for t, n, name in ((target, T, 'target'), (loss, T, 'loss'), (lse, T, 'lse'), (total, 1, 'total'), (ws, None, 'ws')):
-        if t is not None and (not t.is_contiguous() or (n is not None and t.numel() != n)):
-            raise ValueError('linear_cross_entropy: %s must be contiguous%s' % (name, '' if n is None else ' with %d entries' % n))
-    mats = [_on(t, dev, ty, name) for t, ty, name in ((h, dt, 'h'), (w, dt, 'w'), (dh, dt, 'dh'), (dw, torch.float32 if dw_f32 else dt, 'dw'))]
+    f32 = torch.float32
+    dw_f32 = dw is not None and dw.dtype == f32
+    addr = (_on(h, dev, dt, 'h'), _on(w, dev, dt, 'w'), _vec(target, T, dev, torch.int64, 'target'), _vec(loss, T, dev, f32, 'loss'),
+            _vec(lse, T, dev, f32, 'lse'), _vec(total, 1, dev, f32, 'total'), _on(dh, dev, dt, 'dh'), _on(dw, dev, f32 if dw_f32 else dt, 'dw'),
+            _vec(ws, None, dev, torch.uint8, 'ws'))
     for t, like, name in ((dh, h, 'dh'), (dw, w, 'dw')):
         if t is not None and t.shape != like.shape:
             raise ValueError('linear_cross_entropy: %s must be %s, got %s' % (name, tuple(like.shape), tuple(t.shape)))
     _dev_index = dev
-    lib().call('dpc_linear_cross_entropy', mats[0], _ld(h), mats[1], _ld(w), _TYPES[dt], flat[0], int(ignore_index), T, D, V, flat[1],
-               flat[2], flat[3], mats[2], _ld(dh) if dh is not None else 0, mats[3], _ld(dw) if dw is not None else 0, int(dw_f32),
-               int(bool(accumulate)), float(gscale), int(bool(mean)), int(piece_rows), flat[4], ws.numel(), _stream())
+    lib().call('dpc_linear_cross_entropy', addr[0], _ld(h), addr[1], _ld(w), _TYPES[dt], addr[2], int(ignore_index), T, D, V, addr[3],
+               addr[4], addr[5], addr[6], _ld(dh) if dh is not None else 0, addr[7], _ld(dw) if dw is not None else 0, int(dw_f32),
+               int(bool(accumulate)), float(gscale), int(bool(mean)), int(piece_rows), addr[8], ws.numel(), _stream())
     return loss
 
 
