@@ -636,6 +636,14 @@ __global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, c
   }
 }
 
+// Rows of `row16` 16-byte chunks to another pitch.
+__global__ __launch_bounds__(256) void lce_pitch_kernel(const char* h, int64_t ldh, int rows, int row16, char* to, int64_t ldt) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)rows * row16; i += (int64_t)gridDim.x * 256) {
+    const int64_t n = i / row16, c = i - n * row16;
+    *reinterpret_cast<u32x4*>(to + n * ldt + c * 16) = *reinterpret_cast<const u32x4*>(h + n * ldh + c * 16);
+  }
+}
+
 // C[n][m] = alpha * (sum of the K ranges' slabs, in their order) [+ add] for the tiles that were cut.  One block per 1024 entries.
 template <typename E, int BM, int BN>
 __global__ __launch_bounds__(256) void lce_fold_kernel(LceArgs g) {
@@ -873,7 +881,7 @@ static int lce_edge(int kind) { return kind == LCE_BIG ? 256 : 128; }
 // Where things lie in the workspace for pieces of `rows` rows.
 struct LceLayout {
   int64_t rows, prow;           // rows of a piece; padded to whole tiles
-  int64_t stat, lt, live, pm1, P, ldp, hm, part, acc, bytes;   // byte offsets (ldp: fp32 logits' row length), and the whole
+  int64_t stat, lt, live, pm1, P, ldp, hm, hp, part, acc, bytes;   // byte offsets (ldp: fp32 logits' row length), and the whole
   int tile_l, tile_h, tile_w;   // kinds of the three products' tiles
   int splits;                   // fp32: K ranges of dh
   int pieces;
@@ -911,6 +919,10 @@ static LceLayout lce_layout(int64_t T, int D, int V, int dtype, bool grads, bool
   } else {
     l.tile_l = lce_tile_logits(V, l.rows);
     l.stat = take(dpc_cdiv(V, lce_slab_rows(l.tile_l)) * l.prow * 8);
+    // Rows that do not start on 64 bytes: a K-tile's 64 bytes of them lie across two lines of the cache every so often.  h is
+    // small and laid out anew for the logits where they are at least 2^36 multiplications (1531 x 1160 x 50021 in fp16: 239
+    // -> 199 us, in bf16 200 -> 186, and 4 for the copy; W laid out anew would take off as much again, and cost 48).
+    if (D % 32 != 0 && l.rows * D >= (1ll << 36) / V) l.hp = take(l.rows * lce_up(D, 32) * 2);
     if (grads) {
       l.P = take(lce_up(V, 256) * l.prow * 2);
       l.hm = take(l.prow * (int64_t)D * 2);
@@ -1009,6 +1021,10 @@ static int lce_half(const LceCall& c, const LceLayout& l, hipStream_t st) {
     g.P = c.ws + l.P; g.prow = l.prow; g.alpha = head; g.target = c.target + r0;
     g.stat = (f32x2*)(c.ws + l.stat); g.lt = (float*)(c.ws + l.lt); g.grads = grads;
     g.A = c.w; g.lda = c.ldw * 2; g.B = h; g.ldb = c.ldh * 2;
+    if (l.hp && (((uintptr_t)h | (uintptr_t)g.ldb) & 63)) {
+      g.B = c.ws + l.hp; g.ldb = lce_up(c.D, 32) * 2;
+      hipLaunchKernelGGL(lce_pitch_kernel, dim3(dpc_grid((int64_t)rows * (c.D / 8), 256)), dim3(256), 0, st, h, c.ldh * 2, rows, c.D / 8, c.ws + l.hp, g.ldb);
+    }
     g.M = c.V; g.N = rows; g.K = c.D;
     lce_launch<E, LCE_LOGITS>(g, l.tile_l, st);
     LceRowArgs ra;

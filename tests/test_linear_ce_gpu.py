@@ -365,6 +365,18 @@ def test_captured_and_replayed_on_another_stream(ops, dtype):
                 assert torch.equal(s[3][k], e[k]), (i, k)
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_wide_rows_that_start_inside_a_line(ops, dtype):
+    """2^36 multiplications and more on rows of 2000 bytes: the same bits as on rows of 2048, whatever lies between those."""
+    T, D, V = 2048, 1000, 34000
+    h, w, target = inputs(T, D, V, dtype, 9)
+    apart = torch.full((T, 1024), float('nan'), dtype=dtype, device=DEV)
+    apart[:, :D] = h
+    a, b = call(ops, h, w, target), call(ops, apart[:, :D], w, target)
+    check(a, Oracle(h, w, target))
+    assert all(torch.equal(a[k], b[k]) for k in a)
+
+
 def test_a_vocabulary_of_many_tiles(ops):
     """Rows of several tiles, tails in every direction, against fp64 on samples of the gradients."""
     T, D, V = 1300, 320, 40009
