@@ -206,7 +206,7 @@ __device__ __forceinline__ void lce_logits_end(const LceArgs& g, f32x4 (&acc)[SM
 //
 // 256 x 256 with 8 waves of 128 x 64 for the logits (a wave's 128 entries are a slab) and of 64 x 128 for the gradients, whose
 // transposed reads of A take two instructions each (dh 2 % faster); 200 registers, 96 KB of LDS, one block per CU.  On 8192
-// rows, width 2048, vocabulary 131072: 1225 (logits), 1470 (dh) and 1430 (dW) TFLOP/s where a library product of the same shape
+// rows, width 2048, vocabulary 131072: 1240 (logits), 1490 (dh) and 1440 (dW) TFLOP/s where a library product of the same shape
 // reaches 1374 to 1594 and nothing but matrix instructions 1946.  What limits it is power first: the clock falls to 1.8 GHz,
 // and with all operands 0 the same instructions take 17 to 24 % less time at 2.4.  Then the steps between the products: the
 // matrix units are busy 75 % of the cycles, 80 % without the reads of LDS, 97 % without loads and reads.  Measured and
