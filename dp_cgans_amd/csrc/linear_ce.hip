@@ -950,14 +950,19 @@ static int lce_check(int64_t T, int D, int V, int dtype) {
   return DPC_OK;
 }
 
-// Rows of a piece where the caller names none: as many whole tiles as 1 GiB holds of what a row leaves (d, or the slabs'
-// pairs alone) - and all of them where the fp32 sums of dW over several pieces would take the rest's place.
+#define LCE_ROWS (1 << 21)      // rows of a piece at most (half precision, gradients: P's chunks within 32-bit offsets)
+// Rows of a piece where the caller names none: pieces of about the same size, whole tiles, of as many rows as 1 GiB - or twice
+// the fp32 sums of dW, which each piece reads and writes - holds of what a row leaves (d, or the slabs' pairs alone); all of
+// them where the sums would take the rest's place.  (32768 x 2048 x 131072 in pieces of 4096 rows 45.1 ms, of 8192 43.4, at once
+// 43.6; 32768 x 1024 x 50021 in 4 x 8192 rows 9.5, in 3 x 10496 and 1280 10.6, at once 9.1.)
 static int64_t lce_rows_default(int64_t T, int D, int V, int dtype, bool grads, bool dw16) {
   const int64_t row = grads || dtype == DPC_F32 ? (int64_t)V * lce_size(dtype) : dpc_cdiv(V, 64) * 8;
-  const int64_t room = 1ll << 30;
-  if (T * row <= room + (grads && dw16 ? (int64_t)V * D * 4 : 0)) return T < 1 ? 1 : T;
-  const int64_t rows = room / row / 256 * 256;
-  return rows < 256 ? 256 : rows;
+  const int64_t sums = grads ? 2 * (int64_t)V * D * 4 : 0, room = sums > (1ll << 30) ? sums : 1ll << 30;
+  if (T <= LCE_ROWS && T * row <= room + (grads && dw16 ? (int64_t)V * D * 4 : 0)) return T < 1 ? 1 : T;
+  int64_t most = room / row / 256 * 256;
+  most = most < 256 ? 256 : most > LCE_ROWS ? LCE_ROWS : most;
+  const int64_t pieces = dpc_cdiv(T, most);
+  return lce_up(dpc_cdiv(T, pieces), 256);
 }
 
 extern "C" int64_t dpc_linear_cross_entropy_ws(int64_t T, int D, int V, int dtype, int grads, int dw_f32, int64_t piece_rows) {
@@ -1159,7 +1164,7 @@ extern "C" int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* 
   // and 256 vocabulary entries of P lie within 32-bit offsets)
   DPC_CHECK_ARG(f32 ? dpc_cdiv(V, LCE_SEG) * most < (1ll << 23) : dpc_cdiv(V, 256) * dpc_cdiv(most > D ? most : D, 256) < (1ll << 22),
                 "linear_cross_entropy: the piece is too large");
-  DPC_CHECK_ARG(f32 || !grads || most <= (1 << 21), "linear_cross_entropy: the piece is too large");
+  DPC_CHECK_ARG(f32 || !grads || most <= LCE_ROWS, "linear_cross_entropy: the piece is too large");
   const LceLayout l = lce_layout(T, D, V, dtype, grads, !f32 && !dw_f32, piece_rows);
   DPC_CHECK_ARG(ws_bytes >= l.bytes, "linear_cross_entropy: the workspace is smaller than dpc_linear_cross_entropy_ws says");
   hipStream_t st = (hipStream_t)stream;

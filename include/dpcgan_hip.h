@@ -467,8 +467,9 @@ int dpc_noise_add_clamp(float* x, int64_t n, float scale, const float* noise_inj
  * Half precision: D a multiple of 8, every row of every matrix 16-byte aligned.  fp32: any D and row length.  The outputs
  * overlap neither the operands nor each other.
  * ws: workspace of dpc_linear_cross_entropy_ws bytes for the same arguments (-1 if they are refused), 256-byte aligned, no
- * state between calls; calls that overlap need one each.  piece_rows: rows worked on at a time (0 = what 1 GiB holds);
- * smaller pieces need less workspace, and read and write dw once for each. */
+ * state between calls; calls that overlap need one each.  piece_rows: rows worked on at a time (0 = what 1 GiB or twice the
+ * fp32 size of dw holds; at most 2^21 with gradients in half precision); smaller pieces need less workspace, and read and
+ * write dw once for each. */
 int64_t dpc_linear_cross_entropy_ws(int64_t T, int D, int V, int dtype, int grads, int dw_f32, int64_t piece_rows);
 int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, const int64_t* target,
                              int64_t ignore_index, int64_t T, int D, int V, float* loss, float* lse, float* total,

@@ -384,6 +384,15 @@ def test_a_vocabulary_of_many_tiles(ops):
     check(call(ops, h, w, target), Oracle(h, w, target))
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_millions_of_rows(ops, dtype):
+    """More rows than a piece holds, few classes."""
+    T, D, V = (1 << 21) + 300, 8, 40
+    h, w, target = inputs(T, D, V, dtype, 21)
+    check(call(ops, h, w, target), Oracle(h, w, target))
+    check(call(ops, h, w, target, grads=False), Oracle(h, w, target), grads=False)
+
+
 def test_a_vocabulary_of_millions(ops):
     """More slabs than a grid's second dimension holds; three rows."""
     T, D, V = 3, 8, 4200011
