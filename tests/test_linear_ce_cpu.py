@@ -36,3 +36,14 @@ def test_refused_arguments(change, match):
     a.update(change)
     with pytest.raises(RuntimeError, match=match):
         lib().call('dpc_linear_cross_entropy', *a.values())
+
+
+@pytest.mark.parametrize('change', [dict(dh=0x10000), dict(dh=0x20000), dict(dw=0x10000), dict(dw=0x20000), dict(dw=0x60000)])
+def test_a_gradient_over_an_operand_is_refused(change):
+    test_refused_arguments(change, 'must not lie')
+
+
+@pytest.mark.parametrize('change', [dict(T=(1 << 21) + 1, V=8, piece=1 << 30), dict(dtype=0, T=(1 << 23) + 1, V=1, piece=1 << 30, D=1),
+                                    dict(T=1 << 20, V=1 << 26, D=8, piece=1 << 20)])
+def test_pieces_past_a_launch_are_refused(change):
+    test_refused_arguments(dict(change, ws_bytes=1 << 62), 'piece is too large')

@@ -384,6 +384,18 @@ def test_a_vocabulary_of_many_tiles(ops):
     check(call(ops, h, w, target), Oracle(h, w, target))
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('ignore', [0, 3, 2 ** 32 + 3])
+def test_an_ignored_class_and_odd_pieces(ops, dtype, ignore):
+    """ignore_index may be a class, or share its low half with one; pieces need not be whole tiles."""
+    T, D, V = 330, 64, 40
+    h, w, target = inputs(T, D, V, dtype, 31, ignored=0.0)
+    target[::7] = ignore
+    ref = Oracle(h, w, target, ignore=ignore)
+    for rows in (0, 100, 33, 16):
+        check(call(ops, h, w, target, ignore_index=ignore, piece_rows=rows), ref)
+
+
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
 def test_millions_of_rows(ops, dtype):
     """More rows than a piece holds, few classes."""
