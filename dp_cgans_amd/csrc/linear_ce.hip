@@ -10,7 +10,7 @@
 //   2. per row: the slabs' pairs become one, lse = ln 2 (ref + log2 sum), loss = ln 2 ((ref - l_t log2 e) + log2 sum) with
 //      one rounding in the difference, p_t - 1 = expm1(-loss): a sure row's small loss keeps its digits.
 //   3. P becomes d in the operands' type: 2^(slab's ref - row's ref) / row's sum times what is there, p_t - 1 in the
-//      target's place, exactly 0 in rows that are ignored.
+//      target's place, exactly 0 in rows that are ignored.  (Up to 16 rows: to the sum of two such numbers.)
 //   4. dh and dW as products over d.  dW of several pieces adds up in fp32.
 // That is 6 T V D flops.  They bound it for widths in the thousands (6 D flops against the 10 bytes per logit that writing
 // P, turning it into d and reading it twice move: 8192 x 2048 x 131072 spends 3.6 + 0.8 + 3.0 + 3.1 ms on steps 1, 3 and
@@ -638,6 +638,58 @@ __global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, c
   }
 }
 
+// The same for at most LCE_FEW rows.  A gradient there may hang on two or three entries of d, whose roundings to 8 bits do not
+// average out, so d is held as the sum of two numbers of the operands' type, in the rows n and n + LCE_FEW, and h twice
+// beside them: dW comes out of one product over 2 LCE_FEW rows, dh of the sum of its rows - a product of 32 rows costs what one
+// of 16 does, and the rest of P's 256 rows is not touched (1 x 2048 x 131072 467 -> 460 us, 16 x 256 x 18000 38 -> 36).  16
+// chunks of 8 entries per block.
+template <typename E>
+__global__ __launch_bounds__(256) void lce_few_scale_kernel(char* P, int64_t prow, const f32x2* stat, int slabs, int rows, const f32x2* live, const float* pm1,
+                                                            const int64_t* target, const char* h, int64_t ldh, int row16, char* hm, int copies, LceTotal all) {
+  const int first = (slabs + 1) / 2;
+  if ((int)blockIdx.x >= first + copies) {
+    lce_total<256>(all);
+    return;
+  }
+  if ((int)blockIdx.x >= first) {
+    for (int i = (blockIdx.x - first) * 256 + threadIdx.x; i < LCE_FEW * row16; i += copies * 256) {
+      const int n = i / row16, c = i - n * row16;
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if (n < rows && live[n].y != 0.f) v = *reinterpret_cast<const u32x4*>(h + (int64_t)n * ldh + c * 16);
+      *reinterpret_cast<u32x4*>(hm + (int64_t)i * 16) = v;
+      *reinterpret_cast<u32x4*>(hm + ((int64_t)LCE_FEW * row16 + i) * 16) = v;
+    }
+    return;
+  }
+  const int n = threadIdx.x % LCE_FEW, chunk = blockIdx.x * 16 + threadIdx.x / LCE_FEW, slab = chunk / 8;
+  if (slab >= slabs) return;
+  const f32x2 gl = n < rows ? live[n] : f32x2{0.f, 0.f};
+  const bool on = gl.y != 0.f;
+  const f32x2 st = on ? stat[(int64_t)slab * prow + n] : f32x2{0.f, 0.f};
+  const float f = st.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(st.x - gl.x) * gl.y * Half<E>::kUp;
+  const int64_t t = on ? target[n] - (int64_t)chunk * 8 : -1;
+  u32x4* at = reinterpret_cast<u32x4*>(P + ((int64_t)chunk * prow + n) * 16);
+  const f16x8 x = __builtin_bit_cast(f16x8, *at);
+  typename Half<E>::v8 y, z;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float d = on ? (t == e ? pm1[n] * Half<E>::kUp : (float)x[e] * f) : 0.f;
+    const E hi = (E)d;
+    y[e] = hi;
+    z[e] = (E)(d - (float)hi);
+  }
+  at[0] = __builtin_bit_cast(u32x4, y);
+  at[LCE_FEW] = __builtin_bit_cast(u32x4, z);
+}
+// dh[n] = x[n] + x[n + LCE_FEW]
+template <typename E>
+__global__ __launch_bounds__(256) void lce_few_join_kernel(const float* x, int rows, int D, E* dh, int64_t lddh) {
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < rows * D; i += gridDim.x * 256) {
+    const int n = i / D, c = i - n * D;
+    dh[(int64_t)n * lddh + c] = (E)(x[i] + x[i + LCE_FEW * D]);
+  }
+}
+
 // Rows of `row16` 16-byte chunks to another pitch.
 __global__ __launch_bounds__(256) void lce_pitch_kernel(const char* h, int64_t ldh, int rows, int row16, char* to, int64_t ldt) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)rows * row16; i += (int64_t)gridDim.x * 256) {
@@ -883,7 +935,7 @@ static int lce_edge(int kind) { return kind == LCE_BIG ? 256 : 128; }
 // Where things lie in the workspace for pieces of `rows` rows.
 struct LceLayout {
   int64_t rows, prow;           // rows of a piece; padded to whole tiles
-  int64_t stat, lt, live, pm1, P, ldp, hm, hp, part, acc, bytes;   // byte offsets (ldp: fp32 logits' row length), and the whole
+  int64_t stat, lt, live, pm1, P, ldp, hm, hp, two, part, acc, bytes;   // byte offsets (ldp: fp32 logits' row length), and the whole
   int tile_l, tile_h, tile_w;   // kinds of the three products' tiles
   int splits;                   // fp32: K ranges of dh
   int pieces;
@@ -928,6 +980,7 @@ static LceLayout lce_layout(int64_t T, int D, int V, int dtype, bool grads, bool
     if (grads) {
       l.P = take(lce_up(V, 256) * l.prow * 2);
       l.hm = take(l.prow * (int64_t)D * 2);
+      if (l.tile_l == LCE_ROW) l.two = take(2 * LCE_FEW * (int64_t)D * 4);
       l.tile_h = lce_tile_grad(D, l.rows, V);
       l.tile_w = lce_tile_grad(D, V, l.prow);
       const LceCut h = lce_cut(lce_tiles(D, l.rows, lce_edge(l.tile_h), lce_edge(l.tile_h)), l.tile_h, V);
@@ -1040,20 +1093,32 @@ static int lce_half(const LceCall& c, const LceLayout& l, hipStream_t st) {
     ra.live = grads ? (f32x2*)(c.ws + l.live) : nullptr; ra.pm1 = (float*)(c.ws + l.pm1);
     lce_rows(c, ra, p, l, st);
     if (!grads) continue;
-    const auto scale = lce_up(c.V, 256) * l.prow * 2 > (1ll << 30) ? lce_scale_kernel<E, true> : lce_scale_kernel<E, false>;
-    const int row16 = c.D / 8, copies = c.dw ? dpc_grid(l.prow * row16, 256) : 0;
+    const int row16 = c.D / 8;
+    const bool few = l.tile_l == LCE_ROW;
     char* hm = c.ws + l.hm;
-    hipLaunchKernelGGL(scale, dim3((unsigned)(l.prow / 256 * slabs + copies + lce_takes_total(c, l, p))), dim3(256), 0, st, g.P, l.prow, g.stat, slabs, rows,
-                       slab_rows, ra.live, ra.pm1, g.target, h, c.ldh * 2, row16, hm, copies, lce_all(c));
+    if (few) {
+      const int copies = c.dw ? dpc_grid(LCE_FEW * row16, 256) : 0;
+      hipLaunchKernelGGL(lce_few_scale_kernel<E>, dim3((unsigned)(dpc_cdiv(slabs, 2) + copies + lce_takes_total(c, l, p))), dim3(256), 0, st, g.P, l.prow,
+                         g.stat, slabs, rows, ra.live, ra.pm1, g.target, h, c.ldh * 2, row16, hm, copies, lce_all(c));
+    } else {
+      const auto scale = lce_up(c.V, 256) * l.prow * 2 > (1ll << 30) ? lce_scale_kernel<E, true> : lce_scale_kernel<E, false>;
+      const int copies = c.dw ? dpc_grid(l.prow * row16, 256) : 0;
+      hipLaunchKernelGGL(scale, dim3((unsigned)(l.prow / 256 * slabs + copies + lce_takes_total(c, l, p))), dim3(256), 0, st, g.P, l.prow, g.stat, slabs, rows,
+                         slab_rows, ra.live, ra.pm1, g.target, h, c.ldh * 2, row16, hm, copies, lce_all(c));
+    }
     if (c.dh) {
       LceArgs d = g;
       d.A = c.w; d.lda = c.ldw * 2; d.M = c.D; d.N = rows; d.K = c.V;
-      d.C = c.dh + r0 * c.lddh * 2; d.ldc = c.lddh; d.part = (float*)(c.ws + l.part);
+      E* dh = (E*)c.dh + r0 * c.lddh;
+      float* two = (float*)(c.ws + l.two);
+      d.C = few ? (void*)two : (void*)dh; d.ldc = few ? c.D : c.lddh; d.c_f32 = few; d.part = (float*)(c.ws + l.part);
+      if (few) d.N = 2 * LCE_FEW;
       lce_launch<E, LCE_DH>(d, l.tile_h, st);
+      if (few) hipLaunchKernelGGL(lce_few_join_kernel<E>, dim3(dpc_grid((int64_t)rows * c.D, 256)), dim3(256), 0, st, two, rows, c.D, dh, c.lddh);
     }
     if (c.dw) {
       LceArgs d = g;
-      d.A = hm; d.lda = (int64_t)c.D * 2; d.M = c.D; d.N = c.V; d.K = (int)lce_up(rows, LCE_BK); d.part = (float*)(c.ws + l.part);
+      d.A = hm; d.lda = (int64_t)c.D * 2; d.M = c.D; d.N = c.V; d.K = few ? 2 * LCE_FEW : (int)lce_up(rows, LCE_BK); d.part = (float*)(c.ws + l.part);
       // where the piece's share goes: dW itself, or the fp32 sums over the pieces until the last one
       const bool last = p + 1 == l.pieces, via = !c.dw_f32 && l.pieces > 1;
       float* acc = (float*)(c.ws + l.acc);

@@ -156,6 +156,25 @@ def test_few_rows_in_half_precision(ops, T, D, V, dtype):
     check(call(ops, big[0], w, big[1], piece_rows=16), Oracle(big[0], w, big[1]))
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('T,D,V', [(1, 64, 233), (2, 64, 233), (5, 1032, 5000), (16, 256, 18000)])
+def test_gradients_of_few_rows_are_rounded_once(ops, T, D, V, dtype):
+    """d is within 2^-11 (its first form in fp16) and e^2 (two numbers of the type) here: what is left is the result's rounding e."""
+    for seed in range(8):
+        h, w, target = inputs(T, D, V, dtype, seed, ignored=0.0)
+        ref = Oracle(h, w, target)
+        o = call(ops, h, w, target)
+        p = torch.softmax(h.double() @ w.double().t(), 1)
+        d = p.clone()
+        d.scatter_(1, target[:, None], torch.expm1(-ref.loss)[:, None])
+        e = E[dtype]
+        ed = d.abs() * (2.0 ** -11 + e * e + 2 * ref.el[:, None]) + 2.0 ** -25
+        ed.scatter_add_(1, target[:, None], 2 * ref.el[:, None])
+        for name, want, other, terms in (('dh', ref.dh, lambda x: x @ w.double().abs(), V), ('dw', ref.dw, lambda x: x.t() @ h.double().abs(), T)):
+            err = other(ed + 2 * terms * U * d.abs()) / T
+            within(o[name], want, err + e * (want.abs() + err) + TINY[dtype], name)
+
+
 @pytest.mark.parametrize('dtype', TYPES)
 def test_strided_rows_and_what_lies_between_them(ops, dtype):
     """Rows inside wider buffers; everything outside the outputs' own columns keeps its bits."""
