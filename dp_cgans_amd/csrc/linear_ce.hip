@@ -1165,9 +1165,10 @@ static int lce_full(const LceCall& c, const LceLayout& l, hipStream_t st) {
       const auto k = vec ? lce_few_logits_kernel<true> : lce_few_logits_kernel<false>;
       hipLaunchKernelGGL(k, dim3((unsigned)dpc_cdiv(c.V, 32)), dim3(64), 0, st, w, c.ldw, h, c.ldh, rows, c.D, c.V, P, l.ldp);
     } else {
-      // (64 x 64 tiles below 768 of 128 x 128: 500 x 18000 x 256 56 against 71 us; 4000 x 4000 x 512 166 against 162)
+      // (64 x 64 tiles below 1024 of 128 x 128: 500 x 18000 x 256 55 against 70 us, 700 x 18000 x 1024 226 against 259; 4096 x
+      // 5000 x 512 193 against 180, 3000 x 18000 x 1024 940 against 884)
       dpc_gemm_desc lg = lce_desc(rows, c.V, c.D, h, c.ldh, 1, w, 1, c.ldw, 0.f, P, l.ldp);
-      lg.tile = lce_tiles(rows, c.V, 128, 128) < 768 ? 64 : 128;
+      lg.tile = lce_tiles(rows, c.V, 128, 128) < 1024 ? 64 : 128;
       rc = dpc_gemm_f32_ex(&lg, 1, st);
     }
     if (rc != DPC_OK) return rc;
@@ -1196,7 +1197,9 @@ static int lce_full(const LceCall& c, const LceLayout& l, hipStream_t st) {
       hipLaunchKernelGGL(k, dim3((unsigned)(dpc_cdiv(c.D, 256) * dpc_cdiv(c.V, 64))), dim3(256), 0, st, P, l.ldp, hm, rows, c.D, c.V, p > 0 || c.accumulate,
                          (float*)c.dw, c.lddw);
     } else if (c.dw) {
-      const dpc_gemm_desc d = lce_desc(c.V, c.D, rows, P, 1, l.ldp, hm, c.D, 1, p > 0 || c.accumulate ? 1.f : 0.f, (float*)c.dw, c.lddw);
+      // (64 x 64 tiles: 2 to 9 % less than the product's own choice at 500 x 256 x 18000, 700 x 1024 x 18000, 4096 x 512 x 5000)
+      dpc_gemm_desc d = lce_desc(c.V, c.D, rows, P, 1, l.ldp, hm, c.D, 1, p > 0 || c.accumulate ? 1.f : 0.f, (float*)c.dw, c.lddw);
+      d.tile = 64;
       rc = dpc_gemm_f32_ex(&d, 1, st);
       if (rc != DPC_OK) return rc;
     }
