@@ -5,11 +5,11 @@
 //
 // Half-precision operands (bf16, fp16), per piece of rows:
 //   1. logits tiles on the matrix cores, fp32 accumulators.  A wave reduces its 128 (or 64) vocabulary entries of a row, its
-//      slab, to a pair: ref = max l log2 e, rounded, and the sum of x = 2^(l log2 e - ref) in fp32; for training it leaves x
+//      slab, to a pair: ref = max l and the sum of x = e^(l - ref) in fp32; for training it leaves x
 //      in fp16 (values in [0, 1]: 11 bits where a later bf16 holds 8, so what reaches the gradients is rounded about once) in P.
-//   2. per row: the slabs' pairs become one, lse = ln 2 (ref + log2 sum), loss = ln 2 ((ref - l_t log2 e) + log2 sum) with
-//      one rounding in the difference, p_t - 1 = expm1(-loss): a sure row's small loss keeps its digits.
-//   3. P becomes d in the operands' type: 2^(slab's ref - row's ref) / row's sum times what is there, p_t - 1 in the
+//   2. per row: the slabs' pairs become one, lse = ref + log sum, loss = (ref - l_t) + log sum, p_t - 1 = expm1(-loss): a
+//      sure row's small loss keeps its digits.
+//   3. P becomes d in the operands' type: e^(slab's ref - row's ref) / row's sum times what is there, p_t - 1 in the
 //      target's place, exactly 0 in rows that are ignored.  (Up to 16 rows: to the sum of two such numbers.)
 //   4. dh and dW as products over d.  dW of several pieces adds up in fp32.
 // That is 6 T V D flops.  They bound it for widths in the thousands (6 D flops against the 10 bytes per logit that writing
@@ -41,6 +41,11 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 #define LCE_LOG2E 1.4426950408889634f
 #define LCE_LN2 0.6931471805599453f
 
+// e^(l - ref), l <= ref.  The difference first: it is exact near ref and never above 0, whatever the size of the logits.  (With
+// l log2 e - ref log2 e as one multiply-add the rounding of the product with ref stays in the exponent: up to 1 for logits of
+// 2^24, and 2^8, which no fp32 sum holds, for those of 2^32.)
+__device__ __forceinline__ float lce_exp(float l, float ref) { return __builtin_amdgcn_exp2f((l - ref) * LCE_LOG2E); }
+
 #define LCE_FEW 16              // rows of a piece that the few-rows kernels take: one 16 x 16 block of a matrix instruction
 
 enum { LCE_LOGITS = 0, LCE_DH = 1, LCE_DW = 2 };
@@ -68,7 +73,7 @@ struct LceArgs {
   int M, N, K;
   int tiles_m, tiles_n;
   // LOGITS
-  f32x2* stat;                    // [slab][prow] (reference, sum of 2^(l log2 e - reference)); a slab is a wave's vocabulary entries
+  f32x2* stat;                    // [slab][prow] (reference, sum of e^(l - reference)); a slab is a wave's vocabulary entries
   float* lt;                      // [row] logit of the target
   const int64_t* target;
   int grads;
@@ -158,14 +163,14 @@ __device__ __forceinline__ void lce_logits_end(const LceArgs& g, f32x4 (&acc)[SM
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);
     top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64)) * LCE_LOG2E;
-    // the reference: the largest logit, rounded; what follows is exact relative to it.  (All -inf: 2^(l - 0) = 0, not NaN.)
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    // the reference: the largest logit.  (All -inf: e^(l - 0) = 0, not NaN.)
     const float ref = top == -INFINITY ? 0.f : top;
     f32x4 run = {0.f, 0.f, 0.f, 0.f};                                // (four short sums: a sure row's is 1 and what little there is beside it)
 #pragma unroll
     for (int i = 0; i < SM; ++i) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], LCE_LOG2E, -ref));
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = lce_exp(acc[i][j][e], ref);
       run += acc[i][j];
     }
     float sum = (run.x + run.y) + (run.z + run.w);
@@ -497,7 +502,7 @@ __device__ __forceinline__ f32x2 lce_join(f32x2 x, f32x2 y) {
   if (x.y == 0.f) return y;
   if (y.y == 0.f) return x;
   const float m = fmaxf(x.x, y.x);
-  return f32x2{m, x.y * __builtin_amdgcn_exp2f(x.x - m) + y.y * __builtin_amdgcn_exp2f(y.x - m)};
+  return f32x2{m, x.y * lce_exp(x.x, m) + y.y * lce_exp(y.x, m)};
 }
 
 // Per row: the slabs' pairs become one, lse, the loss and what the gradient needs.  16 rows x 64 runs of slabs per block (with
@@ -543,12 +548,12 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(LceRowArgs a) {
   if (w == 0 && n < a.rows) {
     const int64_t t = a.target[n];
     const bool off = t == a.ignore, bad = !off && (t < 0 || t >= a.V);
-    // The loss from what is exact near it: where the target is the row's largest logit the difference of the references is
-    // the rounding of one product, and the loss the logarithm of the sum - not the difference of two numbers of the logits' size.
+    // The loss from what is exact near it: where the target is the row's largest logit it is the logarithm of the sum - not
+    // the difference of two numbers of the logits' size.
     const float l2 = log2f(x.y);
-    const float loss = off ? 0.f : (bad ? NAN : LCE_LN2 * (fmaf(-a.lt[n], LCE_LOG2E, x.x) + l2));
+    const float loss = off ? 0.f : (bad ? NAN : fmaf(LCE_LN2, l2, x.x - a.lt[n]));
     a.loss[n] = loss;
-    if (a.lse) a.lse[n] = LCE_LN2 * (x.x + l2);
+    if (a.lse) a.lse[n] = fmaf(LCE_LN2, l2, x.x);
     if (a.live) {
       a.live[n] = off || bad ? f32x2{0.f, 0.f} : f32x2{x.x, 1.f / x.y};
       a.pm1[n] = off || bad ? 0.f : expm1f(-loss);
@@ -610,7 +615,7 @@ __global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, c
   const bool on = gl.y != 0.f;                                         // (NaN is on: such a row keeps its NaN)
   const f32x2 st = on ? stat[(int64_t)slab * prow + n] : f32x2{0.f, 0.f};
   // (a slab of nothing but -inf has the sum 0 and a reference that may lie far above the row's)
-  const float f = st.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(st.x - gl.x) * gl.y * Half<E>::kUp;
+  const float f = st.y == 0.f ? 0.f : lce_exp(st.x, gl.x) * gl.y * Half<E>::kUp;
   int at = -1;
   float pt = 0.f;
   if (on) {
@@ -666,7 +671,7 @@ __global__ __launch_bounds__(256) void lce_few_scale_kernel(char* P, int64_t pro
   const f32x2 gl = n < rows ? live[n] : f32x2{0.f, 0.f};
   const bool on = gl.y != 0.f;
   const f32x2 st = on ? stat[(int64_t)slab * prow + n] : f32x2{0.f, 0.f};
-  const float f = st.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(st.x - gl.x) * gl.y * Half<E>::kUp;
+  const float f = st.y == 0.f ? 0.f : lce_exp(st.x, gl.x) * gl.y * Half<E>::kUp;
   const int64_t t = on ? target[n] - (int64_t)chunk * 8 : -1;
   u32x4* at = reinterpret_cast<u32x4*>(P + ((int64_t)chunk * prow + n) * 16);
   const f16x8 x = __builtin_bit_cast(f16x8, *at);
@@ -744,13 +749,13 @@ __global__ __launch_bounds__(256) void lce_stat_f32_kernel(const float* logits, 
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) * LCE_LOG2E;
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   const float ref = top == -INFINITY ? 0.f : top;
   f32x4 run = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < 4; ++k)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) run[e] += __builtin_amdgcn_exp2f(fmaf(q[k][e], LCE_LOG2E, -ref));
+    for (int e = 0; e < 4; ++e) run[e] += lce_exp(q[k][e], ref);
   const float sum = dpc_block_sum((run.x + run.y) + (run.z + run.w), red);
   if (threadIdx.x == 0) {
     stat[(int64_t)seg * prow + n] = f32x2{ref, sum};
@@ -786,7 +791,7 @@ __global__ __launch_bounds__(256) void lce_d_f32_kernel(float* logits, int64_t l
     if (v >= V) break;
     f32x4 q = *reinterpret_cast<const f32x4*>(x + v);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q[e] = on ? (v + e == t ? pt : f * __builtin_amdgcn_exp2f(fmaf(q[e], LCE_LOG2E, -gl.x))) : 0.f;
+    for (int e = 0; e < 4; ++e) q[e] = on ? (v + e == t ? pt : f * lce_exp(q[e], gl.x)) : 0.f;
     *reinterpret_cast<f32x4*>(x + v) = q;
   }
 }
