@@ -5,8 +5,9 @@
 //
 // Half-precision operands (bf16, fp16), per piece of rows:
 //   1. logits tiles on the matrix cores, fp32 accumulators.  A wave reduces its 128 (or 64) vocabulary entries of a row, its
-//      slab, to a pair: ref = max l and the sum of x = e^(l - ref) in fp32; for training it leaves x
-//      in fp16 (values in [0, 1]: 11 bits where a later bf16 holds 8, so what reaches the gradients is rounded about once) in P.
+//      slab, to a pair: ref = max l and the sum of x = e^(l - ref) in fp32; for training it leaves
+//      2^15 x in fp16 in P: 11 bits down to 2^-29 of the slab's largest, where a later bf16 holds 8, and 2^-40 of it in all.  (x
+//      itself would have 11 bits to 2^-14 and nothing below 2^-25: beside a sure target, all the rest of the row.)
 //   2. per row: the slabs' pairs become one, lse = ref + log sum, loss = (ref - l_t) + log sum, p_t - 1 = expm1(-loss): a
 //      sure row's small loss keeps its digits.
 //   3. P becomes d in the operands' type: e^(slab's ref - row's ref) / row's sum times what is there, p_t - 1 in the
@@ -46,6 +47,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 // 2^24, and 2^8, which no fp32 sum holds, for those of 2^32.)
 __device__ __forceinline__ float lce_exp(float l, float ref) { return __builtin_amdgcn_exp2f((l - ref) * LCE_LOG2E); }
 
+#define LCE_HELD 32768.f        // e^(l - max) in [0, 1] in fp16, whose largest number is 65504
 #define LCE_FEW 16              // rows of a piece that the few-rows kernels take: one 16 x 16 block of a matrix instruction
 
 enum { LCE_LOGITS = 0, LCE_DH = 1, LCE_DW = 2 };
@@ -62,7 +64,7 @@ template <> struct Half<__bf16> {
 template <> struct Half<_Float16> {
   typedef f16x8 v8;
   static __device__ __forceinline__ f32x4 mfma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-  static constexpr float kUp = 16384.f;     // |d| <= 1 lifted by 2^14: probabilities stay normal numbers down to 2^-28
+  static constexpr float kUp = 16384.f;     // |d| <= 1 lifted by 2^14: normal numbers down to 2^-28, steps of 2^-38 below
 };
 
 // What a product reads and writes.  The result is C[n][m]: m is the contiguous axis of the output.
@@ -185,7 +187,7 @@ __device__ __forceinline__ void lce_logits_end(const LceArgs& g, f32x4 (&acc)[SM
         for (int w = 0; w < 2; ++w)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const f16x2 v = {(_Float16)acc[i + w][j][2 * c], (_Float16)acc[i + w][j][2 * c + 1]};
+            const f16x2 v = {(_Float16)(acc[i + w][j][2 * c] * LCE_HELD), (_Float16)(acc[i + w][j][2 * c + 1] * LCE_HELD)};
             x[w][c] = __builtin_bit_cast(uint32_t, v);
           }
         // (past the caches: nothing reads P before all of it is there - 8192 x 131072: 3.84 -> 3.57 ms)
@@ -588,7 +590,7 @@ __device__ __forceinline__ void lce_total(const LceTotal& a) {
   if (threadIdx.x == 0) a.total[0] = (float)(s / (a.mean ? (double)max(c, 1) : 1.0));
 }
 
-// P from e^(l - slab max) in fp16 to d in the operands' type, in place.  One thread per row and slab.
+// P from 2^15 e^(l - slab max) in fp16 to d in the operands' type, in place.  One thread per row and slab.
 // NT: P is much larger than the 256 MB of the last-level cache - read and written past it (2 GB: 846 -> 780 us; 0.3 GB: 96 -> 103 us).
 // `copies` blocks from `slabs` * prow / 256 on copy h with its ignored rows, and the rows up to the end of the piece's last tile,
 // set to 0: what such a row holds must not reach dW (0 x NaN).  One more of the last piece: the total.
@@ -615,7 +617,7 @@ __global__ __launch_bounds__(256) void lce_scale_kernel(char* P, int64_t prow, c
   const bool on = gl.y != 0.f;                                         // (NaN is on: such a row keeps its NaN)
   const f32x2 st = on ? stat[(int64_t)slab * prow + n] : f32x2{0.f, 0.f};
   // (a slab of nothing but -inf has the sum 0 and a reference that may lie far above the row's)
-  const float f = st.y == 0.f ? 0.f : lce_exp(st.x, gl.x) * gl.y * Half<E>::kUp;
+  const float f = st.y == 0.f ? 0.f : lce_exp(st.x, gl.x) * gl.y * (Half<E>::kUp / LCE_HELD);
   int at = -1;
   float pt = 0.f;
   if (on) {
@@ -671,7 +673,7 @@ __global__ __launch_bounds__(256) void lce_few_scale_kernel(char* P, int64_t pro
   const f32x2 gl = n < rows ? live[n] : f32x2{0.f, 0.f};
   const bool on = gl.y != 0.f;
   const f32x2 st = on ? stat[(int64_t)slab * prow + n] : f32x2{0.f, 0.f};
-  const float f = st.y == 0.f ? 0.f : lce_exp(st.x, gl.x) * gl.y * Half<E>::kUp;
+  const float f = st.y == 0.f ? 0.f : lce_exp(st.x, gl.x) * gl.y * (Half<E>::kUp / LCE_HELD);
   const int64_t t = on ? target[n] - (int64_t)chunk * 8 : -1;
   u32x4* at = reinterpret_cast<u32x4*>(P + ((int64_t)chunk * prow + n) * 16);
   const f16x8 x = __builtin_bit_cast(f16x8, *at);

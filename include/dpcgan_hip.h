@@ -463,7 +463,8 @@ int dpc_noise_add_clamp(float* x, int64_t n, float scale, const float* noise_inj
  *   then added to what dw holds if accumulate.  Rows ignored or with a bad target take no part in dw, whatever h holds
  *   there, and their dh is 0.
  * Sums, softmax statistics and products are in fp32; half precision rounds (softmax - onehot) to the operands' type, fp16
- * with a lift of 2^14 - pieces of up to 16 rows to the sum of two numbers of it.  No atomics: the same call gives the same bits.
+ * with a lift of 2^14 - pieces of up to 16 rows to the sum of two numbers of it - from e^(logit - largest of 64 or 128 classes)
+ * in 11 bits (2^-40 of that largest below 2^-29 of it).  No atomics: the same call gives the same bits.
  * Half precision: D a multiple of 8, every row of every matrix 16-byte aligned.  fp32: any D and row length.  The outputs
  * overlap neither the operands nor each other.
  * ws: workspace of dpc_linear_cross_entropy_ws bytes for the same arguments (-1 if they are refused), 256-byte aligned, no
