@@ -1011,6 +1011,13 @@ static int lce_check(int64_t T, int D, int V, int dtype) {
 }
 
 #define LCE_ROWS (1 << 21)      // rows of a piece at most (half precision, gradients: P's chunks within 32-bit offsets)
+// Rows of the largest piece: a launch has less than 2^32 threads.  512 for each 256 x 256 tile (and one for each row and slab), 64 for
+// each row's slabs; fp32: 256 for 4096 logits of a row.
+static int64_t lce_rows_most(int V, int dtype, bool grads) {
+  if (dtype == DPC_F32) return ((1ll << 23) - 1) / dpc_cdiv(V, LCE_SEG);
+  const int64_t tiles = ((1ll << 22) - 1) / dpc_cdiv(V, 256) * 256, rows = grads ? LCE_ROWS : ((1ll << 22) - 2) * 16;
+  return tiles < rows ? tiles : rows;
+}
 // Rows of a piece where the caller names none: pieces of about the same size, whole tiles, of as many rows as 1 GiB - or twice
 // the fp32 sums of dW, which each piece reads and writes - holds of what a row leaves (d, or the slabs' pairs alone); all of
 // them where the sums would take the rest's place.  (32768 x 2048 x 131072 in pieces of 4096 rows 45.1 ms, of 8192 43.4, at once
@@ -1018,16 +1025,28 @@ static int lce_check(int64_t T, int D, int V, int dtype) {
 static int64_t lce_rows_default(int64_t T, int D, int V, int dtype, bool grads, bool dw16) {
   const int64_t row = grads || dtype == DPC_F32 ? (int64_t)V * lce_size(dtype) : dpc_cdiv(V, 64) * 8;
   const int64_t sums = grads ? 2 * (int64_t)V * D * 4 : 0, room = sums > (1ll << 30) ? sums : 1ll << 30;
-  if (T <= LCE_ROWS && T * row <= room + (grads && dw16 ? (int64_t)V * D * 4 : 0)) return T < 1 ? 1 : T;
-  int64_t most = room / row / 256 * 256;
-  most = most < 256 ? 256 : most > LCE_ROWS ? LCE_ROWS : most;
+  int64_t limit = lce_rows_most(V, dtype, grads);
+  if (limit > LCE_ROWS) limit = LCE_ROWS;
+  if (T <= limit && T * row <= room + (grads && dw16 ? (int64_t)V * D * 4 : 0)) return T < 1 ? 1 : T;
+  if (limit < 256) return limit;                                       // (fp32, V from 2^27 on)
+  int64_t most = room / row;
+  most = most < 256 ? 256 : (most > limit ? limit : most) / 256 * 256;
   const int64_t pieces = dpc_cdiv(T, most);
   return lce_up(dpc_cdiv(T, pieces), 256);
 }
 
+// Whether the sizes and the piece, as the caller names it or by default, are ones that a call takes.
+static int lce_check_piece(int64_t T, int D, int V, int dtype, bool grads, bool dw16, int64_t& piece_rows) {
+  const int rc = lce_check(T, D, V, dtype);
+  if (rc != DPC_OK) return rc;
+  if (piece_rows <= 0) piece_rows = lce_rows_default(T, D, V, dtype, grads, dw16);
+  DPC_CHECK_ARG((piece_rows < T ? piece_rows : T) <= lce_rows_most(V, dtype, grads) && (dtype == DPC_F32 || dpc_cdiv(V, 256) * dpc_cdiv(D, 256) < (1ll << 22)),
+                "linear_cross_entropy: the piece is too large");
+  return DPC_OK;
+}
+
 extern "C" int64_t dpc_linear_cross_entropy_ws(int64_t T, int D, int V, int dtype, int grads, int dw_f32, int64_t piece_rows) {
-  if (lce_check(T, D, V, dtype) != DPC_OK) return -1;
-  if (piece_rows <= 0) piece_rows = lce_rows_default(T, D, V, dtype, grads != 0, dtype != DPC_F32 && !dw_f32);
+  if (lce_check_piece(T, D, V, dtype, grads != 0, dtype != DPC_F32 && !dw_f32, piece_rows) != DPC_OK) return -1;
   return lce_layout(T, D, V, dtype, grads != 0, dtype != DPC_F32 && !dw_f32, piece_rows).bytes;
 }
 
@@ -1218,12 +1237,12 @@ extern "C" int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* 
                                         int64_t ignore_index, int64_t T, int D, int V, float* loss, float* lse, float* total, void* dh,
                                         int64_t lddh, void* dw, int64_t lddw, int dw_f32, int accumulate, float gscale, int mean,
                                         int64_t piece_rows, void* ws, int64_t ws_bytes, void* stream) {
-  const int rc0 = lce_check(T, D, V, dtype);
+  const bool f32 = dtype == DPC_F32, grads = dh || dw;
+  const int rc0 = lce_check_piece(T, D, V, dtype, grads, !f32 && !dw_f32, piece_rows);
   if (rc0 != DPC_OK) return rc0;
   DPC_CHECK_ARG(w && ws && (T == 0 || (h && target && loss)), "linear_cross_entropy: null pointer");
   DPC_CHECK_ARG(ldh >= D && ldw >= D && (!dh || lddh >= D) && (!dw || lddw >= D), "linear_cross_entropy: a leading dimension is smaller than the width");
   DPC_CHECK_ARG(!accumulate || (dw && (dw_f32 || dtype == DPC_F32)), "linear_cross_entropy: accumulation goes into an fp32 dw");
-  const bool f32 = dtype == DPC_F32;
   if (!f32) {
     const uintptr_t al = (uintptr_t)h | (uintptr_t)w | (uintptr_t)dh | (uintptr_t)dw | (uintptr_t)(ldh * 2) | (uintptr_t)(ldw * 2);
     DPC_CHECK_ARG((al & 15) == 0, "linear_cross_entropy: half-precision rows must be 16-byte aligned");
@@ -1232,14 +1251,6 @@ extern "C" int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* 
   }
   DPC_CHECK_ARG((!dh || (dh != h && dh != w && dh != dw)) && (!dw || (dw != h && dw != w)), "linear_cross_entropy: a gradient must not lie where an operand does");
   DPC_CHECK_ARG(((uintptr_t)ws & 255) == 0, "linear_cross_entropy: the workspace must be 256-byte aligned");
-  const bool grads = dh || dw;
-  if (piece_rows <= 0) piece_rows = lce_rows_default(T, D, V, dtype, grads, !f32 && !dw_f32);
-  const int64_t most = piece_rows < T ? piece_rows : T;
-  // (a launch has less than 2^32 threads: 512 for each 256 x 256 tile, one for each row and slab, 256 for 4096 fp32 logits of a row;
-  // and 256 vocabulary entries of P lie within 32-bit offsets)
-  DPC_CHECK_ARG(f32 ? dpc_cdiv(V, LCE_SEG) * most < (1ll << 23) : dpc_cdiv(V, 256) * dpc_cdiv(most > D ? most : D, 256) < (1ll << 22),
-                "linear_cross_entropy: the piece is too large");
-  DPC_CHECK_ARG(f32 || !grads || most <= LCE_ROWS, "linear_cross_entropy: the piece is too large");
   const LceLayout l = lce_layout(T, D, V, dtype, grads, !f32 && !dw_f32, piece_rows);
   DPC_CHECK_ARG(ws_bytes >= l.bytes, "linear_cross_entropy: the workspace is smaller than dpc_linear_cross_entropy_ws says");
   hipStream_t st = (hipStream_t)stream;
