@@ -1233,6 +1233,25 @@ static int lce_full(const LceCall& c, const LceLayout& l, hipStream_t st) {
   return DPC_OK;
 }
 
+// Rows of `width` bytes every `pitch` bytes, and whether two such lie over each other anywhere.
+struct LceSpan { uintptr_t at; int64_t rows, width, pitch; };
+static LceSpan lce_span(const void* p, int64_t rows, int64_t width, int64_t pitch) { return LceSpan{(uintptr_t)p, p && width ? rows : 0, width, pitch}; }
+static bool lce_row_meets(uintptr_t at, int64_t width, const LceSpan& y) {
+  const int64_t from = (int64_t)(at - y.at) - y.width;                 // the first row of y that ends behind `at`
+  const int64_t j = from < 0 ? 0 : from / y.pitch + 1;
+  return j < y.rows && y.at + j * y.pitch < at + width;
+}
+static bool lce_meet(const LceSpan& x, const LceSpan& y) {
+  if (x.rows <= 0 || y.rows <= 0) return false;
+  if (x.at + (x.rows - 1) * x.pitch + x.width <= y.at || y.at + (y.rows - 1) * y.pitch + y.width <= x.at) return false;
+  if (x.rows > y.rows) return lce_meet(y, x);
+  // (of one pitch: rows that meet are the same number of rows apart everywhere, so one of them is a first row somewhere)
+  if (x.pitch == y.pitch) return lce_row_meets(x.at, x.width, y) || lce_row_meets(y.at, y.width, x);
+  for (int64_t i = 0; i < x.rows; ++i)
+    if (lce_row_meets(x.at + i * x.pitch, x.width, y)) return true;
+  return false;
+}
+
 extern "C" int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* w, int64_t ldw, int dtype, const int64_t* target,
                                         int64_t ignore_index, int64_t T, int D, int V, float* loss, float* lse, float* total, void* dh,
                                         int64_t lddh, void* dw, int64_t lddw, int dw_f32, int accumulate, float gscale, int mean,
@@ -1249,9 +1268,15 @@ extern "C" int dpc_linear_cross_entropy(const void* h, int64_t ldh, const void* 
     DPC_CHECK_ARG(ldh < (1 << 21) && ldw < (1 << 21), "linear_cross_entropy: rows are too long");     // (256 rows within 32-bit offsets)
     DPC_CHECK_ARG((!dh || lddh % 8 == 0) && (!dw || lddw % (dw_f32 ? 4 : 8) == 0), "linear_cross_entropy: gradient rows must be 16-byte aligned");
   }
-  DPC_CHECK_ARG((!dh || (dh != h && dh != w && dh != dw)) && (!dw || (dw != h && dw != w)), "linear_cross_entropy: a gradient must not lie where an operand does");
   DPC_CHECK_ARG(((uintptr_t)ws & 255) == 0, "linear_cross_entropy: the workspace must be 256-byte aligned");
   const LceLayout l = lce_layout(T, D, V, dtype, grads, !f32 && !dw_f32, piece_rows);
+  const int64_t size = lce_size(dtype), size_w = dw_f32 ? 4 : size;
+  const LceSpan spans[] = {lce_span(ws, 1, l.bytes, l.bytes), lce_span(loss, 1, T * 4, T * 4), lce_span(lse, 1, T * 4, T * 4), lce_span(total, 1, 4, 4),
+                           lce_span(dh, T, D * size, lddh * size), lce_span(dw, V, D * size_w, lddw * size_w),                 // what is written: 6
+                           lce_span(h, T, D * size, ldh * size), lce_span(w, V, D * size, ldw * size), lce_span(target, 1, T * 8, T * 8)};
+  for (int i = 0; i < 6; ++i)
+    for (int j = i + 1; j < 9; ++j)
+      DPC_CHECK_ARG(!lce_meet(spans[i], spans[j]), "linear_cross_entropy: an output or the workspace must not lie over an operand or another output");
   DPC_CHECK_ARG(ws_bytes >= l.bytes, "linear_cross_entropy: the workspace is smaller than dpc_linear_cross_entropy_ws says");
   hipStream_t st = (hipStream_t)stream;
   LceCall c;

@@ -465,8 +465,8 @@ int dpc_noise_add_clamp(float* x, int64_t n, float scale, const float* noise_inj
  * Sums, softmax statistics and products are in fp32; half precision rounds (softmax - onehot) to the operands' type, fp16
  * with a lift of 2^14 - pieces of up to 16 rows to the sum of two numbers of it - from e^(logit - largest of 64 or 128 classes)
  * in 11 bits (2^-40 of that largest below 2^-29 of it).  No atomics: the same call gives the same bits.
- * Half precision: D a multiple of 8, every row of every matrix 16-byte aligned.  fp32: any D and row length.  The outputs
- * overlap neither the operands nor each other.
+ * Half precision: D a multiple of 8, every row of every matrix 16-byte aligned.  fp32: any D and row length.  Outputs and
+ * workspace lie over neither the operands nor each other (refused; between another matrix's rows is fine).
  * ws: workspace of dpc_linear_cross_entropy_ws bytes for the same arguments (-1 if they are refused), 256-byte aligned, no
  * state between calls; calls that overlap need one each.  piece_rows: rows worked on at a time (0 = what 1 GiB or twice the
  * fp32 size of dw holds; at most 2^21 with gradients in half precision); smaller pieces need less workspace, and read and
