@@ -54,6 +54,11 @@ class _Lib(object):
             fn = getattr(self.cdll, name)      # AttributeError if the .so lacks a declared symbol
             fn.restype = restype
             fn.argtypes = argtypes
+        with open(HEADER_PATH) as f:
+            want = int(re.search(r'^#define DPC_VERSION (\d+)', f.read(), flags=re.M).group(1))
+        if self.cdll.dpc_version() != want:
+            raise ImportError('dp_cgans_amd: %s is version %d, its header %d. Build it again: make -C dp_cgans_amd/csrc'
+                              % (LIB_PATH, self.cdll.dpc_version(), want))
 
     # When set to a list, every call is appended as (name, args) - bench.py uses it to issue the launches of one
     # training step again (replay) for the per-kernel roofline figures.  Measurement aid only.

@@ -1,6 +1,7 @@
 // Philox fills (the same idx -> draw mapping the fused kernels use) and the fused
 // noise + Adam + clamp parameter update.
 #include "dpc_common.h"
+#include "../../include/dpcgan_hip.h"
 #include <string.h>
 
 static thread_local char g_err[256] = "";
@@ -9,7 +10,7 @@ extern "C" void dpc_set_error(const char* msg) {
   g_err[sizeof(g_err) - 1] = 0;
 }
 extern "C" const char* dpc_last_error(void) { return g_err; }
-extern "C" int dpc_version(void) { return 100; }
+extern "C" int dpc_version(void) { return DPC_VERSION; }
 
 __global__ void rng_advance_kernel(uint64_t* rng_a, uint64_t* rng_b, int32_t* t_a, int add_a, int32_t* t_b, int add_b) {
   if (threadIdx.x == 0 && blockIdx.x == 0) {

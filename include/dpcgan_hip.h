@@ -35,6 +35,9 @@ extern "C" {
 #define DPC_BF16 1
 #define DPC_F16 2
 
+/* Version of this header; dpc_version() is the library's.  The structs below grow at their ends, and an entry point reads them
+ * whole: a caller that mirrors them compares the two before its first call.  (100: dpc_gemm_desc without split_slab.) */
+#define DPC_VERSION 101
 int dpc_version(void);
 const char* dpc_last_error(void);
 
