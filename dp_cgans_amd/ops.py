@@ -863,13 +863,15 @@ def grad_clip(plan, max_norm, out, gscale=1.0, t_dev=None):
     """out [2] <- (norm, coef): the norm of gscale times all gradients of ``plan`` and the factor that brings them to at
     most ``max_norm``, for adamw_step's ``coef``; nothing is read back.  A norm that is not finite gives coef 0 (the
     step is skipped); otherwise the device step count ``t_dev`` (int32 [1], optional) goes up by one."""
-    _chk(out, torch.float32, 'out')
-    _chk(t_dev, torch.int32, 't_dev')
+    global _dev_index
+    dev = plan.table.get_device()
+    addr = _on(out, dev, torch.float32, 'out'), _on(t_dev, dev, torch.int32, 't_dev')
     if out.numel() < 2 or not out.is_contiguous():
         raise ValueError('grad_clip: out must be a contiguous fp32 [2]')
     if t_dev is not None and t_dev.numel() < 1:
         raise ValueError('grad_clip: t_dev must be an int32 [1]')
-    lib().call('dpc_grad_clip', plan._info, _p(plan.table), float(max_norm), float(gscale), _p(out), _p(t_dev), _stream())
+    _dev_index = dev
+    lib().call('dpc_grad_clip', plan._info, plan.table.data_ptr(), float(max_norm), float(gscale), *addr, _stream())
     return out
 
 
@@ -877,14 +879,17 @@ def adamw_step(plan, lr, b1=0.9, b2=0.999, eps=1e-8, coef=None, gscale=1.0, t_de
                site=SITE_DITHER):
     """One AdamW step over the tensors of ``plan`` in one launch.  coef: fp32 device factor of the gradients (grad_clip's
     out[1:]; 0 skips the step).  Step count (t_dev's value + t_host) >= 1; rng: required by 8-bit states without dither."""
-    _chk(coef, torch.float32, 'coef')
-    _chk(t_dev, torch.int32, 't_dev')
-    _chk(rng, torch.int64, 'rng')
+    global _dev_index
+    dev = plan.table.get_device()
+    addr = _on(coef, dev, torch.float32, 'coef'), _on(t_dev, dev, torch.int32, 't_dev'), _on(rng, dev, torch.int64, 'rng')
     for t, n, name in ((coef, 1, 'coef'), (t_dev, 1, 't_dev'), (rng, 2, 'rng')):
         if t is not None and t.numel() < n:
             raise ValueError('adamw_step: %s needs %d entries' % (name, n))
-    lib().call('dpc_adamw_step', plan._info, _p(plan.table), float(lr), float(b1), float(b2), float(eps), _p(coef),
-               float(gscale), _p(t_dev), int(t_host), _p(rng), site, _stream())
+    if rng is not None and not rng.is_contiguous():
+        raise ValueError('adamw_step: rng must be contiguous')
+    _dev_index = dev
+    lib().call('dpc_adamw_step', plan._info, plan.table.data_ptr(), float(lr), float(b1), float(b2), float(eps), addr[0],
+               float(gscale), addr[1], int(t_host), addr[2], site, _stream())
 
 
 def noise_add_clamp(x, scale, noise_inj=None, rng=None, site=SITE_NOISE_D, clamp=0.0):
