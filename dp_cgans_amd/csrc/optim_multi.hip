@@ -115,7 +115,8 @@ __device__ __forceinline__ void grad_clip_finish(const double* part, int n, cons
     const double norm = a.gscale * sqrt(s);
     const bool ok = norm <= 1.7976931348623157e308;        // false for NaN too
     a.out[0] = (float)norm;
-    a.out[1] = ok ? (float)(norm > a.max_norm ? a.gscale * (a.max_norm / norm) : a.gscale) : 0.f;
+    // (never 0 for a finite norm, however small the factor: 0 skips the step)
+    a.out[1] = ok ? fmaxf((float)(norm > a.max_norm ? a.gscale * (a.max_norm / norm) : a.gscale), 1.17549435e-38f) : 0.f;
     if (ok && a.t) *a.t += 1;
   }
 }

@@ -510,7 +510,7 @@ typedef struct dpc_multi_info {
 int dpc_multi_plan_size(const dpc_multi_tensor* t, int count, dpc_multi_info* info);
 int dpc_multi_plan(const dpc_multi_tensor* t, int count, const dpc_multi_info* info, void* plan, int64_t bytes);
 /* out fp32 [2] = {norm, coef}: norm = gscale * sqrt(sum of g^2 over all tensors) (fp64 sums, fixed order), coef =
- * gscale * min(1, max_norm / norm).  A norm that is not finite gives coef 0 - dpc_adamw_step then writes nothing - and
+ * gscale * min(1, max_norm / norm), 2^-126 at least.  A norm that is not finite gives coef 0 - dpc_adamw_step then writes nothing - and
  * is the only case in which *t_dev (nullable, device step count) does not go up by 1. */
 int dpc_grad_clip(const dpc_multi_info* info, void* plan, double max_norm, double gscale, float* out, int32_t* t_dev,
                   void* stream);
