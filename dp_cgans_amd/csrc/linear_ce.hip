@@ -1,4 +1,7 @@
-// Softmax cross entropy of a Linear layer over a large vocabulary, with its gradients, logits never whole in memory.
+// Softmax cross entropy of a Linear layer over a large vocabulary, with its gradients, a piece of rows at a time.  What a piece keeps
+// of its logits: half precision for the loss alone, 8 bytes for every 64 or 128 of them; with gradients, 2 bytes each; fp32, 4
+// bytes each.  (A piece is all rows up to 1 GiB of that or twice the fp32 size of dW: 8192 x 131072 in half precision, 2.1 GB.  The
+// caller may ask for smaller ones.)
 //
 //   l = h W^T,  lse_r = log sum_v e^(l_rv),  loss_r = lse_r - l_(r, t_r),
 //   d_rv = e^(l_rv - lse_r) - [v = t_r],  dh = alpha d W,  dW = alpha d^T h,  alpha = gscale / rows that count.
@@ -10,8 +13,10 @@
 //      itself would have 11 bits to 2^-14 and nothing below 2^-25: beside a sure target, all the rest of the row.)
 //   2. per row: the slabs' pairs become one, lse = ref + log sum, loss = (ref - l_t) + log sum, p_t - 1 = expm1(-loss): a
 //      sure row's small loss keeps its digits.
-//   3. P becomes d in the operands' type: e^(slab's ref - row's ref) / row's sum times what is there, p_t - 1 in the
-//      target's place, exactly 0 in rows that are ignored.  (Up to 16 rows: to the sum of two such numbers.)
+//   3. P becomes d in the operands' type, which the matrix instruction asks for: e^(slab's ref - row's ref) / row's sum times
+//      what is there, p_t - 1 in the target's place, exactly 0 in rows that are ignored.  (Up to 16 rows: to the sum of two such
+//      numbers.)  With the result's own rounding this leaves dh and dW 0.0019 off in bf16, 0.00072 in fp16, where the
+//      result's rounding alone makes 0.0017 and 0.00071.
 //   4. dh and dW as products over d.  dW of several pieces adds up in fp32.
 // That is 6 T V D flops.  They bound it for widths in the thousands (6 D flops against the 10 bytes per logit that writing
 // P, turning it into d and reading it twice move: 8192 x 2048 x 131072 spends 3.6 + 0.8 + 3.0 + 3.1 ms on steps 1, 3 and
@@ -213,7 +218,7 @@ __device__ __forceinline__ void lce_logits_end(const LceArgs& g, f32x4 (&acc)[SM
 //
 // 256 x 256 with 8 waves of 128 x 64 for the logits (a wave's 128 entries are a slab) and of 64 x 128 for the gradients, whose
 // transposed reads of A take two instructions each (dh 2 % faster); 200 registers, 96 KB of LDS, one block per CU.  On 8192
-// rows, width 2048, vocabulary 131072: 1240 (logits), 1490 (dh) and 1440 (dW) TFLOP/s where a library product of the same shape
+// rows, width 2048, vocabulary 131072: 1227 (logits), 1475 (dh) and 1427 (dW) TFLOP/s where a library product of the same shape
 // reaches 1374 to 1594 and nothing but matrix instructions 1946.  What limits it is power first: the clock falls to 1.8 GHz,
 // and with all operands 0 the same instructions take 17 to 24 % less time at 2.4.  Then the steps between the products: the
 // matrix units are busy 75 % of the cycles, 80 % without the reads of LDS, 97 % without loads and reads.  Measured and
@@ -468,7 +473,7 @@ __global__ __launch_bounds__(WM * WN * 64) void lce_product_kernel(LceArgs g) {
 
 // Logits of at most 16 rows: reading W once is all there is to it.  One wave per block takes 64 vocabulary entries and no LDS: a
 // lane's 16 bytes of W are one operand of a matrix instruction, and 32 of them are on their way.  One row, vocabulary 131072,
-// width 2048: 135 us for the call (4.0 TB/s), 144 with tiles through LDS; 4 x 256 x 18000 in a graph 8.9 against 10.0 us.
+// width 2048: 136 us for the call (4.0 TB/s), 144 with tiles through LDS; 4 x 256 x 18000 in a graph 8.9 against 10.0 us.
 template <typename E>
 __global__ __launch_bounds__(64) void lce_few_kernel(LceArgs g) {
   using H = Half<E>;
@@ -571,8 +576,8 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(LceRowArgs a) {
 }
 
 // The losses of all rows of the call as one: their sum, over the rows that count if `mean`.  One block, in a fixed order: a launch
-// of its own for the loss alone, a block beside those that turn logits into d otherwise (a launch less: 5 us of 174 for fp32
-// 500 x 256 x 18000).
+// of its own for the loss alone, a block beside those that turn logits into d otherwise (a launch less: fp32 500 x 256 x
+// 18000 175 -> 172 us).
 struct LceTotal { const float* loss; const int64_t* target; int64_t T, ignore; int mean; float* total; };
 template <int NT>
 __device__ __forceinline__ void lce_total(const LceTotal& a) {
@@ -811,7 +816,7 @@ __global__ __launch_bounds__(256) void lce_fold_f32_kernel(const float* slabs, i
 
 // At most 16 rows: reading W once - writing dW once - is all there is to it.  The logits take one wave per block and no LDS: a
 // lane's 16 bytes of W are four k-steps of v_mfma_f32_16x16x4_f32 (step s takes element s of every lane, of W and of h alike),
-// and a wave has 16 of them on their way.  One row, width 2048, vocabulary 131072 (1.07 GB): logits 547 -> 250 us (4.3 TB/s), dW
+// and a wave has 16 of them on their way.  One row, width 2048, vocabulary 131072 (1.07 GB): logits 547 -> 241 us (4.5 TB/s), dW
 // 557 -> 161 against the tiled products; dh by these means took what the tiled product with its K cut takes, 260.  With 17 to
 // 64 rows the logits were slower: too few waves for their work.
 template <bool VEC>
@@ -919,8 +924,9 @@ static int lce_tile_grad(int64_t M, int64_t N, int64_t K) { return lce_tiles(M, 
 static int lce_slab_rows(int kind) { return kind == LCE_BIG ? 128 : 64; }
 
 // The tiles of a product that make whole rounds of the chip (256 CUs, `per` blocks each), and the K ranges of the others:
-// as many as fill a round, none shorter than `least`; not cut at all where two would be (a round of them saves less
-// than writing and adding up their sums costs).
+// as many as fill a round, none shorter than `least`, 32 at most; not cut at all where two would be (a round of them saves less
+// than writing and adding up their sums costs).  (Loss and dh in bf16, 32 ranges at most against 128: 4 x 64 x 18000 29 against 31 us, 64 x 128 x
+// 18000 35 both, but 4 x 128 x 131072 80 against 60, 100 x 512 x 131072 156 against 127.)
 struct LceCut { int whole, splits; int64_t part; };
 static LceCut lce_cut(int64_t tiles, int kind, int64_t K) {
   const int64_t slots = kind == LCE_BIG ? 256 : 512, least = kind == LCE_BIG ? 1024 : 512;
@@ -966,7 +972,8 @@ static LceLayout lce_layout(int64_t T, int D, int V, int dtype, bool grads, bool
     l.stat = take(dpc_cdiv(V, LCE_SEG) * l.prow * 8);
     l.P = take(l.rows * l.ldp * 4);
     if (grads) {
-      // 64 x 64 tiles, three to a CU; no range shorter than 256, none empty
+      // 64 x 64 tiles, three to a CU; no range shorter than 256, none empty, 32 at most (loss and dh, 32 against 128: 100 x 512 x
+      // 131072 324 against 327 us, 64 x 128 x 18000 42 against 40, 4 x 128 x 131072 100 against 55)
       const int64_t tiles = lce_tiles(D, l.rows, 64, 64), kt = dpc_cdiv(V, 32);
       int64_t s = 768 / tiles;
       if (s > V / 256) s = V / 256;
@@ -981,8 +988,11 @@ static LceLayout lce_layout(int64_t T, int D, int V, int dtype, bool grads, bool
     l.tile_l = lce_tile_logits(V, l.rows);
     l.stat = take(dpc_cdiv(V, lce_slab_rows(l.tile_l)) * l.prow * 8);
     // Rows that do not start on 64 bytes: a K-tile's 64 bytes of them lie across two lines of the cache every so often.  h is
-    // small and laid out anew for the logits where they are at least 2^36 multiplications (1531 x 1160 x 50021 in fp16: 239
-    // -> 199 us, in bf16 200 -> 186, and 4 for the copy; W laid out anew would take off as much again, and cost 48).
+    // small and laid out anew for the logits where they are at least 2^36 multiplications.  The loss alone, with the copy and
+    // without: bf16 1531 x 1160 x 50021 181 against 187 us, 4096 x 1160 x 50021 450 against 474, 900 x 2040 x 50021 208 against
+    // 218, 8192 x 1000 x 18000 284 against 293; below the limit, 1024 x 1160 x 50021 142 against 148, 400 x 2040 x 50021 108 against 117,
+    // 600 x 520 x 50021 61 against 59, 256 x 1000 x 30000 38 against 39 (fp16 the same within 2 %): wide rows gain there too,
+    // narrow ones lose, small calls neither.
     if (D % 32 != 0 && l.rows * D >= (1ll << 36) / V) l.hp = take(l.rows * lce_up(D, 32) * 2);
     if (grads) {
       l.P = take(lce_up(V, 256) * l.prow * 2);

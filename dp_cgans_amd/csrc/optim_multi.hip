@@ -322,8 +322,9 @@ __device__ __forceinline__ void mt_hold8(void* base, float* scales, int64_t i, i
 }
 
 // lr / (1 - b1^t) and 1 / sqrt(1 - b2^t): of the host, or of the step count on the device by repeated squaring, as in
-// dpc_adam_step's kernel, one thread's work.  8-bit states: with the block's loads on their way (404 M parameters 1282 -> 1232
-// us, 1182 with the host's count); 32-bit states: before them (2111 us against 2149, and 2105).
+// dpc_adam_step's kernel, one thread's work.  8-bit states: with the block's loads on their way (404 M fp32 parameters and gradients,
+// Philox bits: 1282 -> 1234 us; now 1220, and 1160 with the host's count); 32-bit states: before them (2111 us against 2149, and
+// 2105 with the host's).
 struct AdamwBias { float step_size, inv_bc2s; };
 __device__ __forceinline__ AdamwBias adamw_bias(const AdamwArgs& a, float* bc) {
   if (!a.t_dev) return AdamwBias{a.step_size, a.inv_bc2s};

@@ -705,8 +705,9 @@ def linear_cross_entropy_ws(T, D, V, dtype, grads=True, dw_f32=False, piece_rows
 
 def linear_cross_entropy(h, w, target, loss, ws, dh=None, dw=None, lse=None, total=None, ignore_index=-100, mean=True,
                          gscale=1.0, accumulate=False, piece_rows=0):
-    """Softmax cross entropy of the rows of h [T, D] against w [V, D]: loss [T] (and lse [T], total [1]) of logits h w^T that
-    never lie in memory as a whole; with dh [T, D] / dw [V, D] also the gradients of gscale * total in the same call.
+    """Softmax cross entropy of the rows of h [T, D] against w [V, D]: loss [T] (and lse [T], total [1]) of the logits
+    h w^T, which the workspace holds for a piece of rows at a time (half precision, the loss alone: not at all); with dh [T, D] /
+    dw [V, D] also the gradients of gscale * total in the same call.
     h and w fp32, bf16 or fp16; dh of their type, dw too or fp32 (``accumulate``: added to); target int64 [T].
     ws: uint8 workspace of linear_cross_entropy_ws(T, D, V, h.dtype, grads, dw_f32, piece_rows) bytes.  See
     dpc_linear_cross_entropy for ignored rows, alignment and pieces."""

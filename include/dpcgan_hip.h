@@ -459,7 +459,9 @@ int dpc_noise_add_clamp(float* x, int64_t n, float scale, const float* noise_inj
 
 /* ---- cross entropy of a Linear layer over a large vocabulary (no counterpart in the reference, whose _cond_loss_pair,
  * dp_cgan.py:330-389, compares two-way columns: dpc_cond_loss) ------------------------------------------------------ */
-/* logits = h w^T, h [T][ldh], w [V][ldw] (D columns; dtype DPC_F32, DPC_BF16 or DPC_F16 for both), never whole in memory.
+/* logits = h w^T, h [T][ldh], w [V][ldw] (D columns; dtype DPC_F32, DPC_BF16 or DPC_F16 for both), a piece of rows at a time: of a
+ * piece's logits the workspace holds 8 bytes for every 64 or 128 (half precision, the loss alone), 2 bytes each (half precision
+ * with gradients) or 4 (fp32).
  *   loss[r] = lse_r - logit[r][target[r]], 0 where target[r] == ignore_index, NaN for any other target outside [0, V);
  *   lse (nullable) [T], of every row; total (nullable) [1] = sum of loss, divided by the rows not ignored if mean;
  *   dh (nullable) [T][lddh], dw (nullable) [V][lddw] = gradients of gscale * total: of h's type, dw fp32 if dw_f32 and
